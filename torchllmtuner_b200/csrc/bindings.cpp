@@ -1035,6 +1035,419 @@ variable_list qk_norm_rope_node(const Tensor& q, const Tensor& k, const OptTenso
   return {NativeQKNormRope::apply(q, qw, cosb, sinb, eps), NativeQKNormRope::apply(k, kw, cosb, sinb, eps)};
 }
 
+// ---- linear layers with an epilogue, LayerNorm, rotary positions: kernels behind C++ nodes. What a kernel cannot serve goes back to Python:
+// a backward that builds a graph of its own, or whose upstream gradients have no memory to read (a vmap over them), is computed from the same
+// op as tensor expressions (`statement(name, inputs, config, need, grads)`).
+PyObject* g_statement = nullptr;          // reference kept for the life of the process
+void set_statement_hook(const py::object& fn) {
+  py::object f = fn;
+  Py_XDECREF(g_statement);
+  g_statement = f.release().ptr();
+}
+bool plain_memory(const Tensor& t) {
+  const auto ks = t.key_set();
+  return t.unsafeGetTensorImpl()->has_storage() && !ks.has(c10::DispatchKey::FuncTorchBatched) && !ks.has(c10::DispatchKey::Batched) &&
+         !ks.has(c10::DispatchKey::Python) && !ks.has(c10::DispatchKey::FuncTorchGradWrapper);
+}
+bool beyond_kernels(const variable_list& grads) {
+  if (at::GradMode::is_enabled()) return true;
+  for (const Tensor& g : grads)
+    if (g.defined() && !plain_memory(g)) return true;
+  return false;
+}
+// Gradients of the inputs that `need` names, from the tensor expressions.
+variable_list through_statement(const char* name, const std::vector<OptTensor>& inputs, const py::object& config, const std::vector<bool>& need,
+                                const variable_list& grads) {
+  TORCH_CHECK(g_statement != nullptr, "set_statement_hook was not called");
+  try {
+    py::object fn = py::reinterpret_borrow<py::object>(g_statement);
+    std::vector<OptTensor> gs;
+    for (const Tensor& g : grads) gs.push_back(g.defined() ? OptTensor(g) : OptTensor());
+    auto r = fn(name, inputs, config, need, gs).cast<std::vector<OptTensor>>();
+    variable_list out;
+    for (auto& t : r) out.push_back(t.has_value() ? *t : Tensor());
+    return out;
+  } catch (py::error_already_set& e) {
+    e.restore();
+    throw python_error();
+  }
+}
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
+void check_rows_type(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || is_f32(t)), name, " must be a bfloat16 or float32 CUDA tensor");
+}
+int int_of(int64_t v, const char* what) {
+  TORCH_CHECK(v >= 0 && v <= 0x7fffffff, what, " is out of the kernels' range: ", v);
+  return (int)v;
+}
+
+// -------- LayerNorm
+int64_t layer_norm_max_width(bool f32) { return llmt_layer_norm_max_width(f32); }
+// Rows as the kernels take them: unit inner stride, and a row stride and start whose 16-byte granules match those of a dense result.
+Tensor norm_rows(const Tensor& t) {
+  const int64_t D = t.size(-1), V = 16 / t.element_size();
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, D});
+  const bool ok = (D == 1 || r.stride(1) == 1) && (r.size(0) <= 1 || (r.stride(0) >= D && (r.stride(0) - D) % V == 0)) &&
+                  reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 == 0;
+  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+struct NativeLayerNorm : public torch::autograd::Function<NativeLayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rows_type(x, "x");
+    TORCH_CHECK(w.scalar_type() == x.scalar_type() && b.scalar_type() == x.scalar_type() && w.device() == x.device() && b.device() == x.device(),
+                "weight and bias must have x's type and device");
+    const int64_t D = x.size(-1);
+    TORCH_CHECK(D > 0 && w.dim() == 1 && b.dim() == 1 && w.size(0) == D && b.size(0) == D, "weight and bias must have x's last size");
+    Tensor xr = norm_rows(x), wc = w.contiguous(), bc = b.contiguous();
+    const int R = int_of(xr.size(0), "rows");
+    Tensor y = torch::empty(x.sizes(), x.options());
+    Tensor stats = torch::empty({2, R}, x.options().dtype(at::kFloat));
+    check_rc(llmt_layer_norm_fwd(xr.data_ptr(), R > 1 ? xr.stride(0) : D, wc.data_ptr(), bc.data_ptr(), y.data_ptr(), stats.data_ptr<float>(),
+                                 stats.data_ptr<float>() + R, R, int_of(D, "width"), (float)eps, is_f32(x), cur_stream()),
+             "llmt_layer_norm_fwd", R > 0);
+    ctx->save_for_backward({x, w, b, stats});
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1], &b = s[2], &stats = s[3];
+    if (beyond_kernels(d)) {
+      py::gil_scoped_acquire gil;
+      auto r = through_statement("layer_norm", {x, w, b}, py::make_tuple(ctx->saved_data["eps"].toDouble()),
+                                 {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)}, d);
+      return {r[0], r[1], r[2], Tensor()};
+    }
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t D = x.size(-1);
+    Tensor xr = norm_rows(x), wc = w.contiguous();
+    Tensor dy = d[0].to(x.scalar_type());
+    if (!dy.is_contiguous() || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone(at::MemoryFormat::Contiguous);
+    const int R = (int)xr.size(0);
+    Tensor dx = torch::empty(x.sizes(), x.options());
+    if (R == 0) return {dx, torch::zeros_like(w), torch::zeros_like(b), Tensor()};
+    Tensor dw = torch::empty({D}, w.options()), db = torch::empty({D}, b.options());
+    const int P = llmt_layer_norm_bwd_partials(R, (int)D, is_f32(x));
+    Tensor part = torch::empty({P, 2, D}, stats.options());
+    check_rc(llmt_layer_norm_bwd(dy.data_ptr(), xr.data_ptr(), R > 1 ? xr.stride(0) : D, wc.data_ptr(), stats.data_ptr<float>(),
+                                 stats.data_ptr<float>() + R, dx.data_ptr(), part.data_ptr<float>(), P, dw.data_ptr(), db.data_ptr(), R, (int)D,
+                                 is_f32(x), cur_stream()),
+             "llmt_layer_norm_bwd", 2);
+    return {dx, dw, db, Tensor()};
+  }
+};
+Tensor layer_norm_node(const Tensor& x, const Tensor& w, const Tensor& b, double eps) { return NativeLayerNorm::apply(x, w, b, eps); }
+
+// -------- rotary positions
+struct RotaryConfig {                      // of one call: which channels rotate, and how
+  int64_t off;
+  bool interleaved;
+};
+Tensor unit_inner(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+void check_rotary(const Tensor& x, const Tensor& cosb, const Tensor& sinb, const RotaryConfig& c, const char* name) {
+  check_rows_type(x, name);
+  TORCH_CHECK(x.dim() == 3, name, " must be [T, H, d]");
+  TORCH_CHECK(cosb.is_cuda() && sinb.is_cuda() && is_f32(cosb) && is_f32(sinb) && cosb.dim() == 2 && cosb.sizes() == sinb.sizes() &&
+                  cosb.device() == x.device() && sinb.device() == x.device(),
+              "cos and sin must be float32 [T, P] on the operand's device");
+  TORCH_CHECK(cosb.size(0) == x.size(0) && cosb.size(1) > 0 && c.off >= 0 && c.off + 2 * cosb.size(1) <= x.size(2),
+              "the rotated channels [offset, offset + 2 P) must lie in the head, one table row per token");
+}
+LlmtRopeShape rope_shape(const Tensor& x, const Tensor& cosb, const Tensor& sinb, const RotaryConfig& c, float sign) {
+  LlmtRopeShape s{};
+  s.T = int_of(x.size(0), "tokens"); s.d = int_of(x.size(2), "head width"); s.off = (int)c.off; s.P = (int)cosb.size(1); s.interleaved = c.interleaved;
+  s.cosb = cosb.data_ptr<float>(); s.sinb = sinb.data_ptr<float>(); s.ldt = s.T > 1 ? cosb.stride(0) : s.P; s.sign = sign;
+  return s;
+}
+// The tables as the kernels take them: unit inner stride, one row stride for both.
+void same_tables(Tensor& cosb, Tensor& sinb) {
+  cosb = unit_inner(cosb);
+  sinb = unit_inner(sinb);
+  if (cosb.size(0) > 1 && (cosb.stride(0) != sinb.stride(0) || cosb.stride(0) < cosb.size(1))) {
+    cosb = cosb.contiguous();
+    sinb = sinb.contiguous();
+  }
+}
+LlmtHeads heads_of(const Tensor& x, const Tensor& y) {
+  LlmtHeads h{};
+  h.x = x.data_ptr(); h.x_tok = x.stride(0); h.x_head = x.stride(1);
+  h.y = y.data_ptr(); h.y_tok = y.stride(0); h.y_head = y.stride(1);
+  h.H = int_of(x.size(1), "heads");
+  return h;
+}
+std::vector<Tensor> rope_run(const Tensor& a, const OptTensor& b, Tensor cosb, Tensor sinb, const RotaryConfig& c, float sign) {
+  c10::cuda::CUDAGuard guard(a.device());
+  check_rotary(a, cosb, sinb, c, "x");
+  same_tables(cosb, sinb);
+  Tensor xa = unit_inner(a), ya = torch::empty(a.sizes(), a.options()), xb, yb;
+  LlmtHeads ha = heads_of(xa, ya), hb{};
+  if (b.has_value()) {
+    check_rotary(*b, cosb, sinb, c, "k");
+    TORCH_CHECK(b->scalar_type() == a.scalar_type() && b->size(2) == a.size(2), "both operands must have one type and head width");
+    xb = unit_inner(*b);
+    yb = torch::empty(b->sizes(), b->options());
+    hb = heads_of(xb, yb);
+  }
+  const LlmtRopeShape s = rope_shape(a, cosb, sinb, c, sign);
+  check_rc(llmt_rope(&s, &ha, b.has_value() ? &hb : nullptr, is_f32(a), cur_stream()), "llmt_rope", a.size(0) > 0);
+  if (b.has_value()) return {ya, yb};
+  return {ya};
+}
+// An output that was computed before its node: operands that share a launch have a node each.
+struct Computed { Tensor t; };
+struct NativeRope : public torch::autograd::Function<NativeRope> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& cosb, const Tensor& sinb, int64_t off, bool interleaved, double sign,
+                        const Computed& done) {
+    ctx->save_for_backward({cosb, sinb});
+    ctx->saved_data["off"] = off;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["sign"] = sign;
+    return done.t.defined() ? done.t : rope_run(x, c10::nullopt, cosb, sinb, {off, interleaved}, (float)sign)[0];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const variable_list s = ctx->get_saved_variables();
+    const int64_t off = ctx->saved_data["off"].toInt();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool();
+    const double sign = ctx->saved_data["sign"].toDouble();
+    variable_list out(7);
+    if (beyond_kernels(d)) {
+      py::gil_scoped_acquire gil;
+      out[0] = through_statement("rope", {d[0], s[0], s[1]}, py::make_tuple(off, interleaved, -sign), {true}, {})[0];
+    } else {
+      out[0] = rope_run(d[0], c10::nullopt, s[0], s[1], {off, interleaved}, (float)-sign)[0];
+    }
+    return out;
+  }
+};
+Tensor rope_node(const Tensor& x, const Tensor& cosb, const Tensor& sinb, int64_t off, bool interleaved, bool inverse) {
+  return NativeRope::apply(x, cosb, sinb, off, interleaved, inverse ? -1.0 : 1.0, Computed{});
+}
+variable_list rope_pair_node(const Tensor& q, const Tensor& k, const Tensor& cosb, const Tensor& sinb, int64_t off, bool interleaved) {
+  std::vector<Tensor> y;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    y = rope_run(q, k, cosb, sinb, {off, interleaved}, 1.f);
+  }
+  return {NativeRope::apply(q, cosb, sinb, off, interleaved, 1.0, Computed{y[0]}),
+          NativeRope::apply(k, cosb, sinb, off, interleaved, 1.0, Computed{y[1]})};
+}
+
+// -------- per-head norm + rotation of part of the head
+int64_t qk_norm_rope_part_max_dim() { return llmt_qk_norm_rope_part_max_dim(); }
+void check_head_weight(const OptTensor& w, const Tensor& x) {
+  if (w.has_value())
+    TORCH_CHECK(w->device() == x.device() && w->scalar_type() == x.scalar_type() && w->dim() == 1 && w->size(0) == x.size(2),
+                "norm weights must be [d] with the operand's type and device");
+}
+struct NativeHeadNormRope : public torch::autograd::Function<NativeHeadNormRope> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const Tensor& cosb, const Tensor& sinb, int64_t off, bool interleaved,
+                        double eps, double shift, const Computed& done) {
+    ctx->save_for_backward({x, w.has_value() ? *w : Tensor(), cosb, sinb});
+    ctx->saved_data["off"] = off;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["shift"] = shift;
+    return done.t;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1];
+    Tensor cosb = s[2], sinb = s[3];
+    const RotaryConfig c{ctx->saved_data["off"].toInt(), ctx->saved_data["interleaved"].toBool()};
+    const double eps = ctx->saved_data["eps"].toDouble(), shift = ctx->saved_data["shift"].toDouble();
+    variable_list out(9);
+    if (beyond_kernels(d)) {
+      py::gil_scoped_acquire gil;
+      auto r = through_statement("head_norm_rope", {x, opt(w), cosb, sinb}, py::make_tuple(c.off, c.interleaved, eps, shift),
+                                 {ctx->needs_input_grad(0), w.defined() && ctx->needs_input_grad(1)}, d);
+      out[0] = r[0];
+      out[1] = r[1];
+      return out;
+    }
+    c10::cuda::CUDAGuard guard(x.device());
+    same_tables(cosb, sinb);
+    const bool need_w = w.defined() && ctx->needs_input_grad(1);
+    Tensor xi = unit_inner(x), dy = unit_inner(d[0]), dx = torch::empty(x.sizes(), x.options()), dw, part;
+    if (need_w) dw = x.numel() > 0 ? torch::empty(w.sizes(), w.options()) : torch::zeros(w.sizes(), w.options());
+    out[0] = dx;
+    out[1] = dw;
+    if (x.numel() == 0) return out;
+    const Tensor wc = w.defined() ? w.contiguous() : w;
+    LlmtHeads h = heads_of(xi, dx);
+    h.w = wc.defined() ? wc.data_ptr() : nullptr;
+    h.dy = dy.data_ptr(); h.dy_tok = dy.stride(0); h.dy_head = dy.stride(1);
+    int P = 0;
+    if (need_w) {
+      P = llmt_qk_norm_rope_part_partials((int)x.size(0), h.H, 0, (int)x.size(2));
+      part = torch::empty({P, 2, x.size(2)}, x.options().dtype(at::kFloat));
+    }
+    const LlmtRopeShape rs = rope_shape(x, cosb, sinb, c, 1.f);
+    check_rc(llmt_qk_norm_rope_part_bwd(&rs, &h, nullptr, (float)eps, (float)shift, need_w ? part.data_ptr<float>() : nullptr, P,
+                                        need_w ? dw.data_ptr() : nullptr, nullptr, is_f32(x), cur_stream()),
+             "llmt_qk_norm_rope_part_bwd", need_w ? 2 : 1);
+    return out;
+  }
+};
+// Queries and keys normalised and rotated by one launch; a node for each, so that either can be differentiated without the other.
+variable_list qk_norm_rope_part_node(const Tensor& q, const Tensor& k, const OptTensor& qw, const OptTensor& kw, const Tensor& cosb0, const Tensor& sinb0,
+                                     double eps, int64_t off, bool interleaved, double shift) {
+  Tensor yq, yk;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::cuda::CUDAGuard guard(q.device());
+    const RotaryConfig c{off, interleaved};
+    check_rotary(q, cosb0, sinb0, c, "q");
+    check_rotary(k, cosb0, sinb0, c, "k");
+    TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.size(2) == k.size(2), "q and k must have one type and head width");
+    check_head_weight(qw, q);
+    check_head_weight(kw, k);
+    Tensor cosb = cosb0, sinb = sinb0;
+    same_tables(cosb, sinb);
+    Tensor xq = unit_inner(q), xk = unit_inner(k), wq = qw.has_value() ? qw->contiguous() : Tensor(), wk = kw.has_value() ? kw->contiguous() : Tensor();
+    yq = torch::empty(q.sizes(), q.options());
+    yk = torch::empty(k.sizes(), k.options());
+    LlmtHeads hq = heads_of(xq, yq), hk = heads_of(xk, yk);
+    hq.w = wq.defined() ? wq.data_ptr() : nullptr;
+    hk.w = wk.defined() ? wk.data_ptr() : nullptr;
+    const LlmtRopeShape s = rope_shape(q, cosb, sinb, c, 1.f);
+    check_rc(llmt_qk_norm_rope_part_fwd(&s, &hq, &hk, (float)eps, (float)shift, is_f32(q), cur_stream()), "llmt_qk_norm_rope_part_fwd", q.size(0) > 0);
+  }
+  return {NativeHeadNormRope::apply(q, qw, cosb0, sinb0, off, interleaved, eps, shift, Computed{yq}),
+          NativeHeadNormRope::apply(k, kw, cosb0, sinb0, off, interleaved, eps, shift, Computed{yk})};
+}
+
+std::vector<Tensor> rope_tables(const Tensor& positions, const std::vector<double>& inv, double factor) {
+  c10::cuda::CUDAGuard guard(positions.device());
+  TORCH_CHECK(positions.is_cuda() && positions.scalar_type() == at::kLong && positions.dim() == 1, "positions must be int64 [T] on the device");
+  const Tensor p = positions.contiguous();
+  const int64_t P = (int64_t)inv.size();
+  auto o = positions.options().dtype(at::kFloat);
+  Tensor cosb = torch::empty({p.size(0), P}, o), sinb = torch::empty({p.size(0), P}, o);
+  check_rc(llmt_rope_tables(p.data_ptr<int64_t>(), inv.data(), int_of(P, "frequencies"), factor, cosb.data_ptr<float>(), sinb.data_ptr<float>(),
+                            p.size(0), cur_stream()),
+           "llmt_rope_tables", p.size(0) > 0);
+  return {cosb, sinb};
+}
+
+// -------- linear layers with an epilogue
+// Rows as TMA reads them: unit inner stride, row stride a multiple of 8, 16-byte start; otherwise a copy with padded rows (the padding is never
+// read: the tensor map ends at the last column).
+Tensor tma_rows(const Tensor& t) {
+  if ((t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
+  Tensor r = torch::empty({t.size(0), (t.size(1) + 7) / 8 * 8}, t.options()).narrow(1, 0, t.size(1));
+  r.copy_(t);
+  return r;
+}
+struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, int64_t act, bool keep) {
+    c10::cuda::CUDAGuard guard(x.device());
+    check_bf16(x, "x");
+    check_bf16(w, "w");
+    TORCH_CHECK(w.dim() == 2 && x.size(-1) == w.size(1) && w.device() == x.device(), "x [..., K] and w [N, K] must agree");
+    const int64_t N = w.size(0), K = w.size(1);
+    Tensor x2 = tma_rows(rows_2d(x)), w2 = tma_rows(w.stride(1) == 1 ? w : w.contiguous());
+    const int64_t M = x2.size(0);
+    Tensor y = like_rows(x, N), bc, r2, pre;
+    if (b.has_value()) {
+      TORCH_CHECK(b->device() == x.device() && (b->scalar_type() == at::kBFloat16 || is_f32(*b)) && b->dim() == 1 && b->size(0) == N,
+                  "bias must be [N], bfloat16 or float32");
+      bc = b->contiguous();
+    }
+    if (r.has_value()) {
+      check_bf16(*r, "residual");
+      TORCH_CHECK(r->sizes() == y.sizes() && r->device() == x.device(), "residual must have the result's shape");
+      r2 = rows_2d(*r);
+      if (M > 1 && r2.stride(0) < N && r2.stride(0) != 0) r2 = r2.contiguous();
+    }
+    if (act != 0 && keep) pre = torch::empty({M, (N + 7) / 8 * 8}, x.options());
+    check_rc(llmt_linear_act(x2.data_ptr(), w2.data_ptr(), y.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, bc.defined() && is_f32(bc),
+                             r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, int_of(M, "rows"),
+                             int_of(N, "features"), int_of(K, "features"), x2.stride(0), w2.stride(0), N, r2.defined() ? r2.stride(0) : 0,
+                             pre.defined() ? pre.stride(0) : 0, status_ptr(), cur_stream()),
+             "llmt_linear_act");
+    ctx->save_for_backward({x, w, b.has_value() ? *b : Tensor(), pre});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["residual"] = r.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list d) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &w = s[1], &b = s[2], &pre = s[3];
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = b.defined() && ctx->needs_input_grad(2);
+    variable_list out(6);
+    // needs_input_grad counts the tensors that were given
+    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(b.defined() ? 3 : 2)) out[3] = d[0];
+    if (!nx && !nw && !nb) return out;
+    bool python_side = false;
+    {
+      py::gil_scoped_acquire gil;
+      if (beyond_kernels(d)) {
+        auto r = through_statement("linear_act", {x, w, opt(b)}, py::make_tuple(act), {nx, nw, nb}, d);
+        out[0] = r[0];
+        out[1] = r[1];
+        out[2] = r[2];
+        return out;
+      }
+      try {
+        python_side = python_takes_backward({w});
+      } catch (py::error_already_set& e) {
+        e.restore();
+        throw python_error();
+      }
+    }
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t N = w.size(0), K = w.size(1);
+    Tensor x2 = tma_rows(rows_2d(x)), w2 = tma_rows(w.stride(1) == 1 ? w : w.contiguous()), dy = rows_2d(d[0]);
+    const int64_t M = x2.size(0);
+    if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
+    const bool tma_ok = dy.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
+    const bool write = (nx || nw) && (act != 0 || !tma_ok);
+    Tensor dz = write ? torch::empty({M, (N + 7) / 8 * 8}, dy.options()).narrow(1, 0, N) : dy;
+    if (write || nb) {
+      if (nb) out[2] = torch::empty(b.sizes(), b.options());
+      check_rc(llmt_linear_dz(dy.data_ptr(), M > 1 ? dy.stride(0) : (N + 7) / 8 * 8, act != 0 ? pre.data_ptr() : nullptr, act != 0 ? pre.stride(0) : 0,
+                              (int)act, write ? dz.data_ptr() : nullptr, write ? dz.stride(0) : 0, nb ? out[2].data_ptr() : nullptr,
+                              nb && is_f32(b), (int)M, (int)N, cur_stream()),
+               "llmt_linear_dz");
+    }
+    if (!nx && !nw) return out;
+    if (python_side) {                     // a pending collective rides on the products, or the weight's gradient goes to its owner's buffer
+      py::gil_scoped_acquire gil;
+      try {
+        py::object fn = py::reinterpret_borrow<py::object>(py_hooks().linears_backward);
+        auto r = fn(x2, variable_list{w}, variable_list{dz}, nx, std::vector<bool>{nw}).cast<std::vector<OptTensor>>();
+        if (r[0].has_value()) out[0] = r[0]->reshape(x.sizes());
+        if (r[1].has_value()) out[1] = *r[1];
+        return out;
+      } catch (py::error_already_set& e) {
+        e.restore();
+        throw python_error();
+      }
+    }
+    const int64_t lddz = dz.stride(0);
+    if (nx) {
+      out[0] = torch::empty(x.sizes(), x.options());
+      check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, status_ptr(), cur_stream()),
+               "llmt_linear_dx");
+    }
+    if (nw) {
+      out[1] = torch::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
+      check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, status_ptr(), cur_stream()),
+               "llmt_linear_dw");
+    }
+    return out;
+  }
+};
+Tensor linear_act_node(const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, int64_t act) {
+  // z is kept only for a backward that will read it
+  const bool keep = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b.has_value() && b->requires_grad()));
+  return NativeLinearAct::apply(x, w, b, r, act, keep);
+}
+
 // Reads the status word (synchronises the current stream) and clears it. Returns {code, site, block, extra}.
 std::vector<int64_t> read_status(bool clear) {
   Tensor h = status_word().cpu();
@@ -1074,6 +1487,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_node", &rmsnorm_node);
   m.def("add_rmsnorm_node", &add_rmsnorm_node);
   m.def("qk_norm_rope_node", &qk_norm_rope_node);
+  m.def("set_statement_hook", &set_statement_hook);
+  m.def("layer_norm_max_width", &layer_norm_max_width);
+  m.def("layer_norm_node", &layer_norm_node);
+  m.def("rope_node", &rope_node);
+  m.def("rope_pair_node", &rope_pair_node);
+  m.def("rope_tables", &rope_tables);
+  m.def("qk_norm_rope_part_max_dim", &qk_norm_rope_part_max_dim);
+  m.def("qk_norm_rope_part_node", &qk_norm_rope_part_node);
+  m.def("linear_act_node", &linear_act_node);
   m.def("router_topk", &router_topk);
   m.def("router_topk_bwd", &router_topk_bwd);
   m.def("moe_plan", &moe_plan);

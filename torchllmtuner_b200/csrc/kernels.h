@@ -30,6 +30,42 @@ int llmt_grouped_wgrad_bf16(const void* A, const void* B, void* C, const int* se
 // ---- memory-bound kernels (elementwise.cu) ----
 int llmt_rmsnorm_fwd(const void* x, const void* res, const void* w, void* y, void* sum_out, float* rstd, int T, int D,
                      float eps, cudaStream_t st);
+// ---- linear layers with bias, activation (activations.cuh) and residual (linear_act.cu) ----
+int llmt_linear_act(const void* x, const void* w, void* y, const void* bias, int bias_f32, const void* res, void* pre, int act, int M, int N, int K,
+                    int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, int* status, cudaStream_t stream);
+int llmt_linear_dx(const void* dz, const void* w, void* dx, int M, int N, int K, int64_t lddz, int64_t ldw, int64_t lddx, int* status, cudaStream_t stream);
+int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, int N, int K, int64_t lddz, int64_t ldx, int64_t lddw, int* status, cudaStream_t stream);
+int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, int M, int N,
+                   cudaStream_t stream);
+
+// ---- rotary positions (rope.cu), LayerNorm (layer_norm.cu) ----
+// One operand of a rotation: H heads per token; strides in elements. `w` and `dy` only where the entry point reads them.
+typedef struct {
+  const void *x, *w, *dy;
+  void* y;
+  int64_t x_tok, x_head, y_tok, y_head, dy_tok, dy_head;
+  int H;
+} LlmtHeads;
+// Channels [off, off + 2 P) of every head of `d` rotate by tables [T][P] of row stride ldt; sign -1 rotates back.
+typedef struct {
+  int T, d, off, P, interleaved;
+  const float *cosb, *sinb;
+  int64_t ldt;
+  float sign;
+} LlmtRopeShape;
+int llmt_rope(const LlmtRopeShape* s, const LlmtHeads* a, const LlmtHeads* b, int f32, cudaStream_t stream);
+int llmt_qk_norm_rope_part_max_dim();
+int llmt_qk_norm_rope_part_fwd(const LlmtRopeShape* s, const LlmtHeads* q, const LlmtHeads* k, float eps, float shift, int f32, cudaStream_t stream);
+int llmt_qk_norm_rope_part_partials(int T, int Hq, int Hk, int d);
+int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* s, const LlmtHeads* q, const LlmtHeads* k, float eps, float shift, float* partial, int P,
+                               void* dwq, void* dwk, int f32, cudaStream_t stream);
+int llmt_rope_tables(const int64_t* pos, const double* inv, int P, double factor, float* cosb, float* sinb, int64_t T, cudaStream_t stream);
+int llmt_layer_norm_max_width(int f32);
+int llmt_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean, float* rstd, int R, int D, float eps,
+                        int f32, cudaStream_t stream);
+int llmt_layer_norm_bwd_partials(int R, int D, int f32);
+int llmt_layer_norm_bwd(const void* dy, const void* x, int64_t ldx, const void* w, const float* mean, const float* rstd, void* dx, float* partial,
+                        int P, void* dw, void* db, int R, int D, int f32, cudaStream_t stream);
 int llmt_rmsnorm_bwd_partials(int T);
 int llmt_rmsnorm_bwd(const void* dy, const void* x, const void* w, const float* rstd, const void* dres, void* dx,
                      float* dw_partial, float* dw_f32, void* dw_bf16, int accumulate, int T, int D, cudaStream_t st);

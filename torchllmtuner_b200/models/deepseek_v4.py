@@ -28,11 +28,13 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
+from typing import ClassVar
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
 from .common import Embedding, GatedMLP, Linear, RMSNorm
 from .contracts import DecoderStructure
 from .moe import MoE
@@ -44,6 +46,7 @@ MLP_TYPES = ("hash_moe", "moe")
 
 @dataclass
 class DeepseekV4Config(Qwen3Config):
+    scales_rotary: ClassVar[bool] = False
     q_lora_rank: int = 32
     o_groups: int = 2
     o_lora_rank: int = 16
@@ -118,13 +121,7 @@ def rope_tables_interleaved(positions: torch.Tensor, dim: int, theta: float):
 def rotate_trailing_pairs(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
     """x [T, ..., d]; the last 2*cos.shape[-1] channels rotate as interleaved pairs (even, odd), in fp32; the leading
     channels pass through. Passing -sin undoes the rotation."""
-    w = 2 * cos.shape[-1]
-    lead, rot = x[..., :-w], x[..., -w:]
-    shape = [cos.shape[0]] + [1] * (x.dim() - 2) + [cos.shape[-1]]
-    c, s = cos.view(shape), sin.view(shape)
-    even, odd = rot[..., 0::2].float(), rot[..., 1::2].float()
-    out = torch.stack((even * c - odd * s, odd * c + even * s), dim=-1).flatten(-2).to(x.dtype)
-    return torch.cat((lead, out), dim=-1)
+    return ops.rope(x, cos, sin, layout="interleaved", offset=x.shape[-1] - 2 * cos.shape[-1])
 
 
 class GroupedLinear(nn.Module):
@@ -353,9 +350,10 @@ class V4Attention(nn.Module):
         T = x.shape[0]
         cos, sin = ctx.rope[self.rope_kind]
         q_res = self.q_a_norm(self.q_a_proj(x))
-        q = unweighted_rms_norm(self.q_b_proj(q_res).view(T, self.H, self.d), self.eps)
-        q = rotate_trailing_pairs(q, cos, sin)
-        kv = _whole(ctx, rotate_trailing_pairs(self.kv_norm(self.kv_proj(x)), cos, sin))
+        rotary = dict(layout="interleaved", offset=self.d - 2 * cos.shape[-1])
+        q, kv = ops.qk_norm_rope(self.q_b_proj(q_res).view(T, self.H, self.d), self.kv_proj(x).view(T, 1, self.d), None, self.kv_norm.weight,
+                                 cos, sin, self.eps, norm=True, **rotary)        # queries without a norm weight
+        kv = _whole(ctx, kv.view(T, self.d))
         comp = self.compressor(x, q_res, ctx) if self.compressor is not None else None
         docs = _docs(ctx)
         outs = []
@@ -367,7 +365,7 @@ class V4Attention(nn.Module):
             g0 = docs[doc][0]
             outs.append(self._attend(q[q0:q0 + L], kv[g0:g0 + first + L], e, b, first))
         o = torch.cat(outs, 0) if len(outs) > 1 else outs[0]
-        o = rotate_trailing_pairs(o, cos, -sin)            # values carried the rotation of their own position: undo the query's
+        o = ops.rope(o, cos, sin, inverse=True, **rotary)  # values carried the rotation of their own position: undo the query's
         g = self.o_a_proj(o.reshape(T, self.groups, -1)).reshape(T, -1)
         return self.o_b_proj(g)
 

@@ -261,20 +261,15 @@ class LatentAttention(nn.Module):
         self.o_proj = Linear(H * d, D, dtype, device)
         self.scale = 1.0 / math.sqrt(d)
 
-    def _rope(self, t, cos, sin):
-        half = t.shape[-1] // 2
-        c, s = cos[:, None, :half].to(t.dtype), sin[:, None, :half].to(t.dtype)
-        a, b = t[..., :half], t[..., half:]
-        return torch.cat((a * c - b * s, b * c + a * s), -1)
-
     def forward(self, x, ctx):
         T, H = x.shape[0], self.H
         q = self.q_proj(x).view(T, H, self.d)
         c = self.kv_norm(self.kv_down(x))
         kn = self.k_up(c).view(T, H, self.dn)
         v = self.v_up(c).view(T, H, self.d)
-        kr = self._rope(self.k_rope(x).view(T, 1, self.dr), ctx.cos, ctx.sin).expand(T, H, self.dr)
-        q = torch.cat((q[..., :self.dn], self._rope(q[..., self.dn:], ctx.cos, ctx.sin)), -1)
+        cos, sin = ctx.cos[:, :self.dr // 2], ctx.sin[:, :self.dr // 2]
+        kr = ops.rope(self.k_rope(x).view(T, 1, self.dr), cos, sin).expand(T, H, self.dr)
+        q = ops.rope(q, cos, sin, offset=self.dn)
         k = torch.cat((kn, kr), -1)
         attend = ctx.cp.attention if ctx.cp is not None else ops.attention
         o = attend(q.contiguous(), k.contiguous(), v.contiguous(), ctx.attn_meta, self.scale)

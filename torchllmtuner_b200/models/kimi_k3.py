@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
+from typing import ClassVar
 
 import torch
 import torch.nn as nn
@@ -39,6 +40,7 @@ from .qwen3 import ForwardContext, Qwen3Config, Qwen3ForCausalLM, Qwen3Model
 
 @dataclass
 class KimiConfig(Qwen3Config):
+    scales_rotary: ClassVar[bool] = False
     # linear attention (KDA)
     kda_layers: list[int] = field(default_factory=list)      # 1-based indices, as in the published configs; default: all but every 4th
     linear_heads: int = 4

@@ -10,8 +10,8 @@ Differences from the Qwen-style tower of `models/vision.py`:
   * clips are POOLED OVER TIME (mean over frames) before each `m x m` neighbourhood is folded into one row, so an item
     contributes (gh / m) * (gw / m) rows however many frames it has;
   * the projector is LayerNorm over the patch width -> Linear -> GELU -> Linear to the text width.
-Matrix products go through `ops.linear` (tcgen05 GEMM on the device), attention through the packed-row kernel with one
-non-causal piece per item.
+Projections are `ops.linear_act` (tcgen05 GEMM whose epilogue adds the bias, applies the GELU and adds the residual stream), norms
+`ops.layer_norm`, the rotation one pass over queries and keys, attention the packed-row kernel with one non-causal piece per item.
 """
 from __future__ import annotations
 
@@ -59,8 +59,8 @@ class BiasLinear(nn.Module):
         self.weight = nn.Parameter(torch.empty(out_features, in_features, dtype=dtype, device=device))
         self.bias = nn.Parameter(torch.zeros(out_features, dtype=dtype, device=device))
 
-    def forward(self, x):
-        return ops.linear(x, self.weight) + self.bias.to(x.dtype)
+    def forward(self, x, activation: str | None = None, residual=None):
+        return ops.linear_act(x, self.weight, self.bias, activation=activation, residual=residual)
 
 
 class LayerNorm(nn.Module):
@@ -71,7 +71,7 @@ class LayerNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(dim, dtype=dtype, device=device))
 
     def forward(self, x):
-        return F.layer_norm(x.float(), (x.shape[-1],), self.weight.float(), self.bias.float(), self.eps).to(x.dtype)
+        return ops.layer_norm(x, self.weight, self.bias, self.eps)
 
 
 def time_code(dim: int, frames: int) -> torch.Tensor:
@@ -97,9 +97,7 @@ def grid_pair_angles(grids, head_dim: int, theta: float, device=None) -> torch.T
 
 def rotate_pairs(x: torch.Tensor, ang: torch.Tensor) -> torch.Tensor:
     """x [N, H, d], interleaved pairs (2j, 2j+1) rotate by ang[:, j]."""
-    c, s = ang.cos()[:, None, :], ang.sin()[:, None, :]
-    a, b = x[..., 0::2].float(), x[..., 1::2].float()
-    return torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2).to(x.dtype)
+    return ops.rope(x, ang.cos(), ang.sin(), layout="interleaved")
 
 
 class MoonViTBlock(nn.Module):
@@ -112,13 +110,13 @@ class MoonViTBlock(nn.Module):
         self.fc0, self.fc1 = BiasLinear(D, cfg.intermediate_size, dtype, device), BiasLinear(cfg.intermediate_size, D, dtype, device)
         self.scale = 1.0 / math.sqrt(self.head_dim)
 
-    def forward(self, x, ang, meta: AttnMeta):
+    def forward(self, x, cos, sin, meta: AttnMeta):
         N = x.shape[0]
         q, k, v = self.wqkv(self.norm0(x)).view(N, 3, self.heads, self.head_dim).unbind(1)
-        q, k = rotate_pairs(q, ang), rotate_pairs(k, ang)
+        q, k = ops.qk_norm_rope(q, k, None, None, cos, sin, 0.0, layout="interleaved", norm=False)
         o = ops.attention(q.contiguous(), k.contiguous(), v.contiguous(), meta, self.scale)   # width 72 runs padded to 128
-        x = x + self.wo(o.reshape(N, -1))
-        return x + self.fc1(F.gelu(self.fc0(self.norm1(x))))
+        x = self.wo(o.reshape(N, -1), residual=x)
+        return self.fc1(self.fc0(self.norm1(x), "gelu"), residual=x)
 
 
 class MoonViTTower(nn.Module):
@@ -188,9 +186,10 @@ class MoonViTTower(nn.Module):
         x = self.patch_embed(F.pad(patches.to(w.dtype), (0, self.padded_patch_dim - cfg.patch_dim)))
         x = x + self.position_table(grids, x.dtype)
         ang = grid_pair_angles(grids, cfg.head_dim, cfg.rope_theta, device=x.device)
+        cos, sin = ang.cos(), ang.sin()
         cu = torch.tensor([0] + counts, dtype=torch.int64).cumsum(0)
         meta = AttnMeta.build(cu, causal=False, device=x.device)
         for blk in self.blocks:
-            x = blk(x, ang, meta)
+            x = blk(x, cos, sin, meta)
         x = self.merge(self.pre_norm(self.final_layernorm(x)), grids)
-        return self.proj1(F.gelu(self.proj0(x.flatten(1))))
+        return self.proj1(self.proj0(x.flatten(1), "gelu"))

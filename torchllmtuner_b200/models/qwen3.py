@@ -13,13 +13,16 @@ from __future__ import annotations
 import math
 import zlib
 from dataclasses import dataclass, field
+from typing import ClassVar
 
 import torch
 import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
 from .. import ops
+from ..errors import UnsupportedCombinationError
 from ..ops import AttnMeta
+from ..ops.validation import validate_rope_scaling
 from .common import Embedding, GatedMLP, Linear, RMSNorm, next_token_targets
 from .contracts import DecoderStructure
 from .moe import MoE
@@ -36,6 +39,7 @@ class Qwen3Config:
     head_dim: int | None = None
     rms_norm_eps: float = 1e-6
     rope_theta: float = 1_000_000.0
+    rope_scaling: dict | None = None           # longer contexts: rope_type linear | llama3 | yarn and its numbers (see ops.rope_tables)
     tie_word_embeddings: bool = False
     qk_norm: bool = True
     initializer_range: float = 0.02
@@ -64,6 +68,14 @@ class Qwen3Config:
             self.head_dim = self.hidden_size // self.num_attention_heads
         if self.num_attention_heads % self.num_key_value_heads:
             raise ValueError("num_attention_heads must be a multiple of num_key_value_heads")
+        if self.rope_scaling is not None:
+            if not self.scales_rotary:
+                raise UnsupportedCombinationError(f"{self.model_type}: scaled rotary frequencies are not built for this family")
+            scaling = dict(self.rope_scaling)
+            scaling.setdefault("rope_type", scaling.pop("type", None))
+            self.rope_scaling = None if scaling["rope_type"] in (None, "default") else validate_rope_scaling(scaling)
+
+    scales_rotary: ClassVar[bool] = True       # families that build their own tables say False
 
     def is_moe_layer(self, i: int) -> bool:
         return (self.num_experts > 0 and i not in self.mlp_only_layers and (i + 1) % max(1, self.decoder_sparse_step) == 0)
@@ -261,7 +273,7 @@ class Qwen3ForCausalLM(nn.Module):
         return out
 
     def build_context(self, positions: torch.Tensor, attn_meta: AttnMeta, cp=None) -> ForwardContext:
-        cos, sin = ops.rope_tables(positions, self.config.head_dim, self.config.rope_theta)
+        cos, sin = ops.rope_tables(positions, self.config.head_dim, self.config.rope_theta, scaling=self.config.rope_scaling)
         return ForwardContext(cos, sin, attn_meta, cp)
 
     # ------------------------------------------------------------------ forward

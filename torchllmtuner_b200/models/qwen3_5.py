@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
+from typing import ClassVar
 
 import torch
 import torch.nn as nn
@@ -34,6 +35,7 @@ from .qwen3 import ForwardContext, Qwen3Config, Qwen3ForCausalLM, Qwen3Model
 
 @dataclass
 class Qwen35Config(Qwen3Config):
+    scales_rotary: ClassVar[bool] = False
     layer_types: list[str] = field(default_factory=list)
     full_attention_interval: int = 4
     linear_num_value_heads: int = 4
@@ -121,16 +123,6 @@ def mrope_tables(positions: torch.Tensor, rotary_dim: int, theta: float, section
     return emb.cos(), emb.sin()
 
 
-def rotate_leading(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-    """x [T, H, d]; the first cos.shape[-1] channels rotate in the half-rotation layout, the rest pass through."""
-    r = cos.shape[-1]
-    xr, xp = x[..., :r], x[..., r:]
-    half = r // 2
-    rot = torch.cat((-xr[..., half:], xr[..., :half]), -1)
-    c, s = cos[:, None, :].to(x.dtype), sin[:, None, :].to(x.dtype)
-    return torch.cat((xr * c + rot * s, xp), -1)
-
-
 def attend(q, k, v, ctx, scale):
     if ctx.cp is not None:
         return ctx.cp.attention(q, k, v, ctx.attn_meta, scale)
@@ -209,8 +201,9 @@ class GatedFullAttention(nn.Module):
             q, gate = qg[..., :self.d], qg[..., self.d:].reshape(T, self.H * self.d)
         else:
             q, gate = qg.view(T, self.H, self.d), None
-        q = rotate_leading(self.q_norm(q), ctx.cos, ctx.sin)
-        k = rotate_leading(self.k_norm(self.k_proj(x).view(T, self.Hkv, self.d)), ctx.cos, ctx.sin)
+        half = ctx.cos.shape[-1] // 2                          # the tables hold both halves of the rotated channels, which turn alike
+        q, k = ops.qk_norm_rope(q, self.k_proj(x).view(T, self.Hkv, self.d), self.q_norm.weight, self.k_norm.weight, ctx.cos[:, :half],
+                                ctx.sin[:, :half], self.q_norm.eps, norm=True, zero_centered=True)
         v = self.v_proj(x).view(T, self.Hkv, self.d)
         o = attend(q.contiguous(), k.contiguous(), v.contiguous(), ctx, self.scale).reshape(T, self.H * self.d)
         if gate is not None:

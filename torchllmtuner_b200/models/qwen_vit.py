@@ -16,8 +16,9 @@ Inside the tower rows run in merge-block order (frame, block row, block column, 
 order Hugging Face processors emit; `patch_order="row_major"` (this framework's data pipeline) is permuted on entry. Either
 way one output row per merged cell comes out in (frame, block row, block column) order, the order of the placeholder tokens.
 
-Every projection is `ops.linear` (the sm_100a GEMM on the device), attention is `ops.attention` with one non-causal piece
-per frame (head width 72 of the published tower runs zero-padded to 128)."""
+Every projection is `ops.linear_act` (the sm_100a GEMM whose epilogue adds the bias, applies the GELU and adds the residual stream), the norms
+are `ops.layer_norm`, queries and keys rotate in one pass, attention is `ops.attention` with one non-causal piece per frame (head width 72 of the
+published tower runs zero-padded to 128)."""
 from __future__ import annotations
 
 import math
@@ -113,13 +114,6 @@ def interpolated_positions(table: torch.Tensor, grids, m: int) -> torch.Tensor:
     return torch.cat(out)
 
 
-def rotate_halves(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-    """x [N, H, d]; channel j pairs with channel j + d/2."""
-    xf = x.float()
-    a, b = xf[..., :x.shape[-1] // 2], xf[..., x.shape[-1] // 2:]
-    return (xf * cos[:, None, :] + torch.cat((-b, a), -1) * sin[:, None, :]).to(x.dtype)
-
-
 class _Weight(nn.Module):
     """A bare parameter under the name `<module>.weight` (the position table is an embedding in published files)."""
 
@@ -145,7 +139,7 @@ class PatchProjection(nn.Module):
         w = self.proj.weight.view(self.proj.weight.shape[0], -1)
         if self.pad:
             x, w = F.pad(x, (0, self.pad)), F.pad(w, (0, self.pad))
-        return ops.linear(x, w) + self.proj.bias.to(x.dtype)
+        return ops.linear_act(x, w, self.proj.bias)
 
 
 class QwenViTAttention(nn.Module):
@@ -155,12 +149,12 @@ class QwenViTAttention(nn.Module):
         self.heads, self.head_dim, self.scale = cfg.num_heads, cfg.head_dim, cfg.head_dim ** -0.5
         self.qkv, self.proj = BiasLinear(D, 3 * D, dtype, device), BiasLinear(D, D, dtype, device)
 
-    def forward(self, x, cos, sin, meta: AttnMeta):
-        N = x.shape[0]
+    def forward(self, x, cos, sin, meta: AttnMeta, residual=None):
+        N, half = x.shape[0], self.head_dim // 2               # the tables hold both halves of a head, which turn alike
         q, k, v = self.qkv(x).view(N, 3, self.heads, self.head_dim).unbind(1)
-        q, k = rotate_halves(q, cos, sin), rotate_halves(k, cos, sin)
+        q, k = ops.qk_norm_rope(q, k, None, None, cos[:, :half], sin[:, :half], 0.0, norm=False)
         o = ops.attention(q.contiguous(), k.contiguous(), v.contiguous(), meta, self.scale)
-        return self.proj(o.reshape(N, -1))
+        return self.proj(o.reshape(N, -1), residual=residual)
 
 
 class QwenViTMLP(nn.Module):
@@ -169,8 +163,8 @@ class QwenViTMLP(nn.Module):
         self.linear_fc1 = BiasLinear(cfg.hidden_size, cfg.intermediate_size, dtype, device)
         self.linear_fc2 = BiasLinear(cfg.intermediate_size, cfg.hidden_size, dtype, device)
 
-    def forward(self, x):
-        return self.linear_fc2(F.gelu(self.linear_fc1(x), approximate="tanh"))
+    def forward(self, x, residual=None):
+        return self.linear_fc2(self.linear_fc1(x, "gelu_tanh"), residual=residual)
 
 
 class QwenViTBlock(nn.Module):
@@ -181,8 +175,8 @@ class QwenViTBlock(nn.Module):
         self.attn, self.mlp = QwenViTAttention(cfg, dtype, device), QwenViTMLP(cfg, dtype, device)
 
     def forward(self, x, cos, sin, meta: AttnMeta):
-        x = x + self.attn(self.norm1(x), cos, sin, meta)
-        return x + self.mlp(self.norm2(x))
+        x = self.attn(self.norm1(x), cos, sin, meta, residual=x)
+        return self.mlp(self.norm2(x), residual=x)
 
 
 class QwenViTMerger(nn.Module):
@@ -193,7 +187,7 @@ class QwenViTMerger(nn.Module):
         self.linear_fc1, self.linear_fc2 = BiasLinear(self.wide, self.wide, dtype, device), BiasLinear(self.wide, cfg.out_hidden_size, dtype, device)
 
     def forward(self, x):                      # rows already in merge-block order: a block is m*m consecutive rows
-        return self.linear_fc2(F.gelu(self.linear_fc1(self.norm(x).view(-1, self.wide))))
+        return self.linear_fc2(self.linear_fc1(self.norm(x).view(-1, self.wide), "gelu"))
 
 
 class QwenViTTower(nn.Module):

@@ -9,6 +9,8 @@ from __future__ import annotations
 import re
 from dataclasses import dataclass
 
+from ..ops.validation import ROPE_SCALINGS
+
 
 @dataclass
 class HFPiece:
@@ -28,9 +30,9 @@ class RefPiece:
     n: int
 
 
-def refuse_unsupported_hf_settings(hf: dict, accepted: dict) -> None:
+def refuse_unsupported_hf_settings(hf: dict, accepted: dict, rope_types=("default",)) -> None:
     """A config.json may switch on something this framework's model of the family does not have (a bias on the attention
-    projections, a sliding window, a scaled rotary embedding). Building the model anyway would load the weights it knows
+    projections, a sliding window, a scaled rotary embedding of a kind not in `rope_types`). Building the model anyway would load the weights it knows
     and silently compute something else, so such a folder is refused, naming the setting."""
     from ..errors import UnsupportedCombinationError
     for key, ok in accepted.items():
@@ -38,8 +40,23 @@ def refuse_unsupported_hf_settings(hf: dict, accepted: dict) -> None:
             raise UnsupportedCombinationError(f"config.json sets {key}={hf[key]!r}; this framework's model supports {key} in {list(ok)}")
     rope = hf.get("rope_parameters") or hf.get("rope_scaling") or {}
     kind = rope.get("rope_type", rope.get("type", "default")) if isinstance(rope, dict) else "default"
-    if kind not in ("default", None):
-        raise UnsupportedCombinationError(f"config.json asks for a {kind!r} rotary embedding; only the default one is built")
+    if kind not in (*rope_types, None):
+        built = "only the default one is" if tuple(rope_types) == ("default",) else f"{list(rope_types)} are"
+        raise UnsupportedCombinationError(f"config.json asks for a {kind!r} rotary embedding; {built} built")
+
+
+def rope_scaling_from_hf(hf: dict) -> dict | None:
+    """The scaled rotary embedding a config.json asks for (`rope_parameters` of transformers 5, `rope_scaling` before), None for the default one.
+    It has to name the length the model was trained at: `max_position_embeddings`, which libraries fall back to, is that length in some files and
+    the extended one in others."""
+    from ..errors import UnsupportedCombinationError
+    rope = hf.get("rope_parameters") or hf.get("rope_scaling") or {}
+    kind = rope.get("rope_type", rope.get("type")) if isinstance(rope, dict) else None
+    if kind in ("default", None):
+        return None
+    if kind != "linear" and not rope.get("original_max_position_embeddings"):
+        raise UnsupportedCombinationError(f"config.json asks for a {kind!r} rotary embedding without original_max_position_embeddings")
+    return {"rope_type": kind, **{k: v for k, v in rope.items() if k not in ("rope_type", "type", "rope_theta")}}
 
 
 class ModelStateFormat:
@@ -104,7 +121,10 @@ class Qwen3StateFormat(ModelStateFormat):
         # a dense config.json has neither key; published files say `num_experts`, transformers 5 writes `num_local_experts`
         out["num_experts"] = hf.get("num_experts", hf.get("num_local_experts", 0)) or 0
         refuse_unsupported_hf_settings(hf, {"attention_bias": (False,), "use_sliding_window": (False,), "hidden_act": ("silu",),
-                                            "attention_dropout": (0, 0.0)})
+                                            "attention_dropout": (0, 0.0)}, ("default", *ROPE_SCALINGS))
+        scaling = rope_scaling_from_hf(hf)
+        if scaling is not None:
+            out["rope_scaling"] = scaling
         return out
     _EXP = re.compile(r"^(model\.layers\.\d+\.mlp)\.routed\.experts\.(w1_EFD|w3_EFD|w2_EDF)$")
     _ROUTER = re.compile(r"^(model\.layers\.\d+\.mlp)\.router\.gate\.weight$")
@@ -143,6 +163,8 @@ class Qwen3StateFormat(ModelStateFormat):
                "num_key_value_heads": arch.num_key_value_heads, "head_dim": arch.head_dim, "rms_norm_eps": arch.rms_norm_eps,
                "rope_theta": arch.rope_theta, "tie_word_embeddings": arch.tie_word_embeddings, "hidden_act": "silu",
                "max_position_embeddings": arch.max_position_embeddings, "torch_dtype": "bfloat16"}
+        if arch.rope_scaling is not None:
+            cfg["rope_scaling"] = dict(arch.rope_scaling)
         if moe:
             cfg.update(num_experts=arch.num_experts, num_experts_per_tok=arch.num_experts_per_tok,
                        moe_intermediate_size=arch.moe_intermediate_size, norm_topk_prob=arch.norm_topk_prob,

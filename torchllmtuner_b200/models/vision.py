@@ -26,7 +26,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
-from ..errors import ConfigError
+from ..errors import ConfigError, UnsupportedCombinationError
 from ..ops.attn_meta import AttnMeta
 from .common import GatedMLP, Linear, RMSNorm
 from .contracts import DecoderStructure
@@ -264,6 +264,8 @@ class VisionLanguageModel(nn.Module):
         if getattr(self.text, "positions_are_document_indices", False):      # no rotary in the text model: only restarts matter
             doc = torch.cat([torch.arange(int(p[1]), device=positions.device) for p in attn_meta.pieces])
             return self.text.build_context(doc, attn_meta, cp)
+        if getattr(self.config, "rope_scaling", None) is not None:
+            raise UnsupportedCombinationError("three-axis positions and scaled rotary frequencies are not built together")
         cos, sin = mrope_tables(positions, self.config.head_dim, self.config.rope_theta, self.mrope_sections)
         return ForwardContext(cos, sin, attn_meta, cp)
 

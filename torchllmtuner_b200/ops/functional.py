@@ -4,6 +4,7 @@ There is no library fallback on CUDA: if the extension cannot be loaded the call
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 
@@ -11,8 +12,9 @@ import torch
 from torch.autograd import forward_ad
 
 from . import reference as ref
-from ..errors import UnsupportedCombinationError
-from .validation import validate_attention_inputs, validate_rms_norm_inputs
+from ..errors import ConfigError, UnsupportedCombinationError
+from .validation import (validate_attention_inputs, validate_layer_norm_inputs, validate_linear_act_inputs, validate_qk_inputs, validate_rms_norm_inputs,
+                         validate_rope_scaling, validate_rotary_inputs)
 from .attn_meta import AttnMeta
 from .cuda_ext import load as _ext
 
@@ -45,8 +47,16 @@ def _native():
     if _nodes is None:
         ext = _ext()
         ext.set_autograd_hooks(_symm_module(), _linears_backward)
+        ext.set_statement_hook(_statement_grads)
         _nodes = ext
     return _nodes if _symm._ACTIVE is None and not torch.jit.is_tracing() else None
+
+
+def _node_ext():
+    """The extension with the hooks of its C++ autograd nodes set."""
+    if _nodes is None:
+        _native()
+    return _nodes
 
 
 class _PythonNode(torch.autograd.Function):
@@ -291,6 +301,33 @@ def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return ext.linears_node(x, (w,))[0] if ext is not None else _Linear.apply(x, w)
 
 
+_ACTIVATION_CODES = {None: 0, "gelu": 1, "gelu_tanh": 2, "silu": 3, "relu": 4}       # the kernels' numbers (csrc/activations.cuh)
+
+
+def linear_act(x, w, bias=None, *, activation: str | None = None, residual=None):
+    """act(x W^T + bias) + residual with everything behind the product in its epilogue: x [..., K], w [N, K], bias [N], residual broadcastable to
+    [..., N]; activation None, "gelu" (erf), "gelu_tanh", "silu" or "relu". bf16 on the device, any widths and strides. Elsewhere (other types,
+    per-op checkpointing and pending peer-memory collectives, which are kept per product, transforms and tracing) the same as tensor expressions."""
+    validate_linear_act_inputs(x, w, bias, activation, residual, _ACTIVATION_CODES)
+    given = [t for t in (x, w, bias, residual) if t is not None]
+    if (_SAC is None and _use_cuda(x) and x.dtype == w.dtype == torch.bfloat16 and x.numel() and w.numel()
+            and (bias is None or bias.dtype in _ROW_TYPES) and (residual is None or residual.dtype == x.dtype) and _has_rules(*given)):
+        shape = (*x.shape[:-1], w.shape[0])
+        if residual is None or torch.broadcast_shapes(residual.shape, shape) == shape:
+            ext = _native()
+            if ext is not None:
+                return ext.linear_act_node(x, w, bias, residual if residual is None or residual.shape == shape else residual.expand(shape),
+                                           _ACTIVATION_CODES[activation])
+    # the product of `linear` has no rule under functorch transforms, and none for a gradient over no rows
+    product = linear if x.numel() and w.numel() and (_NO_TRANSFORM is None or _NO_TRANSFORM()) else ref.linear
+    return ref.linear_act(x, w, bias, activation=activation, residual=residual, product=product)
+
+
+def _linear_act_statement(x, w, bias, act: int):
+    name = next(n for n, code in _ACTIVATION_CODES.items() if code == act)
+    return ref.linear_act(x, w, bias, activation=name)
+
+
 def _all_bf16(ws) -> bool:
     return all(w.dtype == torch.bfloat16 and w.is_cuda for w in ws)
 
@@ -311,15 +348,77 @@ def add_rms_norm(x, residual, weight, eps: float):
     return ref.add_rms_norm(x, residual, weight, eps)
 
 
-# ----------------------------------------------------------------------------------------------- QK-norm + RoPE
-rope_tables = ref.rope_tables
+# ----------------------------------------------------------------------------------------------- LayerNorm
+_ROW_TYPES = (torch.bfloat16, torch.float32)
 
 
-def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float):
-    """q [T,Hq,d], k [T,Hkv,d] (views with packed heads are fine); cos/sin fp32 [T,d/2]."""
-    if _use_cuda(q) and q.dtype == torch.bfloat16:
+def layer_norm(x, weight, bias, eps: float):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, statistics in fp32."""
+    validate_layer_norm_inputs(x, weight, bias)
+    if (_use_cuda(x) and x.dtype in _ROW_TYPES and weight.dtype == bias.dtype == x.dtype and 0 < x.shape[-1] <= _node_ext().layer_norm_max_width(x.dtype == torch.float32)
+            and _has_rules(x, weight, bias)):
+        return _node_ext().layer_norm_node(x, weight, bias, eps)
+    return ref.layer_norm(x, weight, bias, eps)
+
+
+# ----------------------------------------------------------------------------------------------- rotary positions, QK-norm + RoPE
+_frequencies = functools.lru_cache(maxsize=64)(lambda head_dim, theta, items: ref.scaled_frequencies(head_dim, theta, dict(items)))
+
+
+def rope_tables(positions, head_dim: int, theta: float, dtype=torch.float32, scaling=None):
+    """cos, sin [T, head_dim / 2] of `positions` [T]. `scaling` extends the context (see `reference.scaled_frequencies`): a dict with rope_type
+    "linear" (factor), "llama3" (factor, original_max_position_embeddings, low_freq_factor, high_freq_factor) or "yarn" (factor,
+    original_max_position_embeddings, optionally beta_fast, beta_slow, truncate, attention_factor, mscale, mscale_all_dim); its angles are taken in 64 bits."""
+    if scaling is None:
+        return ref.rope_tables(positions, head_dim, theta, dtype)
+    validate_rope_scaling(scaling)
+    if head_dim < 2 or head_dim % 2 or not theta > 1 or positions.dim() != 1:
+        raise ConfigError(f"rotary tables need positions [T], an even head width and theta > 1; got {tuple(positions.shape)}, {head_dim}, {theta}")
+    if not (_use_cuda(positions) and positions.dtype in (torch.int64, torch.int32) and head_dim <= 512 and _has_rules(positions)):
+        return ref.rope_tables(positions, head_dim, theta, dtype, scaling)
+    inv, factor = _frequencies(head_dim, float(theta), tuple(sorted((k, v) for k, v in scaling.items() if v is not None)))
+    cos, sin = _ext().rope_tables(positions.long(), inv, factor)
+    return (cos, sin) if dtype == torch.float32 else (cos.to(dtype), sin.to(dtype))
+
+
+def _rotary_kernel(cos, sin, *xs) -> bool:
+    return (all(_use_cuda(x) and x.dtype in _ROW_TYPES for x in xs) and cos.dtype == sin.dtype == torch.float32
+            and not (cos.requires_grad or sin.requires_grad) and _has_rules(cos, sin, *xs))
+
+
+def rope(x, cos, sin, *, layout: str = "half", offset: int = 0, inverse: bool = False):
+    """x [T, ..., d]: the channels [offset, offset + 2 P) rotate by cos/sin [T, P], the rest pass. `layout` "half" pairs channel j with channel
+    j + P of that range, "interleaved" the channels 2j and 2j + 1; `inverse` rotates back. Any strides."""
+    validate_rotary_inputs(x, cos, sin, layout, offset)
+    if not _rotary_kernel(cos, sin, x):
+        return ref.rope(x, cos, sin, layout=layout, offset=offset, inverse=inverse)
+    x3 = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
+    y = _node_ext().rope_node(x3, cos, sin, offset, layout == "interleaved", inverse)
+    return y if x.dim() == 3 else y.view(x.shape)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float, *, layout: str = "half", offset: int = 0, norm: bool | None = None,
+                 zero_centered: bool = False):
+    """Per-head RMSNorm and rotation of queries and keys in one pass. q [T,Hq,d], k [T,Hkv,d] (views are fine); cos/sin fp32 [T,P].
+
+    `norm` None: an operand without a weight is not normalised; True: it is, without a factor; False: neither is. `zero_centered`: the factor is
+    1 + weight. `layout` and `offset` say which channels rotate, see `rope`; the default rotates whole heads in halves (P = d / 2)."""
+    plain = norm is None and layout == "half" and offset == 0 and not zero_centered
+    if plain and _use_cuda(q) and q.dtype == torch.bfloat16 and q.dim() == 3 and 2 * cos.shape[-1] == q.shape[-1] and q.shape[-1] in (64, 128, 256):
         return tuple(_run_node(_ext().qk_norm_rope_node, q, k, q_weight, k_weight, cos, sin, eps))
-    return ref.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
+    validate_qk_inputs(q, k, q_weight, k_weight, cos, sin, layout, offset)
+    normed = [norm is not False and not (norm is None and w is None) for w in (q_weight, k_weight)]
+    weights = [w for w, n in zip((q_weight, k_weight), normed) if n and w is not None]
+    if ((plain and q.dtype == torch.float32) or not _rotary_kernel(cos, sin, q, k) or not _has_rules(*weights)
+            or any(w.dtype != q.dtype for w in weights) or (any(normed) and q.shape[-1] > _node_ext().qk_norm_rope_part_max_dim())):
+        return ref.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, layout=layout, offset=offset, norm=norm, zero_centered=zero_centered)
+    ext, inter = _node_ext(), layout == "interleaved"
+    if all(normed):
+        return tuple(ext.qk_norm_rope_part_node(q, k, q_weight, k_weight, cos, sin, eps, offset, inter, 1.0 if zero_centered else 0.0))
+    if not any(normed):
+        return tuple(ext.rope_pair_node(q, k, cos, sin, offset, inter))
+    return tuple(qk_norm_rope(x, x[:, :0], w, None, cos, sin, eps, layout=layout, offset=offset, norm=n, zero_centered=zero_centered)[0]
+                 for x, w, n in zip((q, k), (q_weight, k_weight), normed))
 
 
 # ----------------------------------------------------------------------------------------------- SwiGLU
@@ -378,6 +477,24 @@ def _through_statement(ctx, inputs, grads):
     need = ctx.needs_input_grad[:len(inputs)]
     got = iter(torch.autograd.grad(outs, [t for t, n in zip(inputs, need) if n], grads, create_graph=graph, allow_unused=True))
     return tuple(next(got) if n else None for n in need) + (None,) * (len(ctx.needs_input_grad) - len(inputs))
+
+
+_STATEMENTS = {"layer_norm": ref.layer_norm, "head_norm_rope": ref.head_norm_rope, "linear_act": _linear_act_statement}
+
+
+def _statement_grads(name, inputs, config, need, grads):
+    """Called by a C++ node whose backward needs tensor expressions (see `_beyond_kernels`): gradients of the inputs that `need` marks, with a
+    graph of their own where one is being built. "rope" is linear: its one input is the upstream gradient itself."""
+    if name == "rope":
+        x, cos, sin = inputs
+        offset, interleaved, sign = config
+        return [ref.rope(x, cos, sin, layout="interleaved" if interleaved else "half", offset=offset, inverse=sign < 0)]
+    graph = torch.is_grad_enabled()
+    with torch.enable_grad():
+        inputs = [None if t is None else t.view_as(t) for t in inputs]      # distinct graph nodes, also where two inputs are one tensor
+        out = _STATEMENTS[name](*inputs, *config)
+    got = iter(torch.autograd.grad(out, [t for t, n in zip(inputs, need) if n], grads[0], create_graph=graph, allow_unused=True))
+    return [next(got) if n else None for n in need]
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

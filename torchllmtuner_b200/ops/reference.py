@@ -31,11 +31,49 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     return rms_norm(s, weight, eps), s
 
 
-def rope_tables(positions: torch.Tensor, head_dim: int, theta: float, dtype=torch.float32):
-    """cos/sin of shape [T, head_dim/2] for half-rotation RoPE."""
+def rope_tables(positions: torch.Tensor, head_dim: int, theta: float, dtype=torch.float32, scaling=None):
+    """cos/sin of shape [T, head_dim/2] for half-rotation RoPE. `scaling` (a dict, see `scaled_frequencies`): frequencies scaled for contexts
+    longer than the trained one, angles in 64 bits."""
+    if scaling is not None:
+        inv, factor = scaled_frequencies(head_dim, theta, scaling)
+        ang = positions.double()[:, None] * torch.tensor(inv, dtype=torch.float64, device=positions.device)
+        return (ang.cos() * factor).to(dtype), (ang.sin() * factor).to(dtype)
     inv = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32, device=positions.device) / head_dim))
     ang = positions.float()[:, None] * inv[None, :]
     return ang.cos().to(dtype), ang.sin().to(dtype)
+
+
+def scaled_frequencies(head_dim: int, theta: float, scaling: dict):
+    """Inverse frequencies (a tuple of head_dim/2 numbers) of a rotary embedding scaled by `scaling["factor"]`, and the factor on cos and sin.
+
+    rope_type "linear": every frequency divided by `factor` (positions interpolated).
+    "llama3": a frequency that turns less than `low_freq_factor` times within `original_max_position_embeddings` is divided, one that turns more
+    than `high_freq_factor` times is kept, between them the two are mixed linearly in the number of turns.
+    "yarn": mixed linearly in the channel between the channels that turn `beta_fast` (32) and `beta_slow` (1) times within
+    `original_max_position_embeddings` (`truncate`: rounded outwards to whole channels); cos and sin times `attention_factor`
+    (0.1 ln factor + 1; with `mscale` and `mscale_all_dim` the ratio of 0.1 m ln factor + 1 of the two)."""
+    kind, s = scaling["rope_type"], float(scaling["factor"])
+    inv = [float(theta) ** (-2.0 * j / head_dim) for j in range(head_dim // 2)]
+    if kind == "linear":
+        return tuple(v / s for v in inv), 1.0
+    L = float(scaling["original_max_position_embeddings"])
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        keep = [min(1.0, max(0.0, (L * v / (2.0 * math.pi) - low) / (high - low))) for v in inv]
+        return tuple(v * k + v / s * (1.0 - k) for v, k in zip(inv, keep)), 1.0
+    channel = lambda turns: head_dim * math.log(L / (turns * 2.0 * math.pi)) / (2.0 * math.log(theta))  # noqa: E731
+    low, high = channel(float(scaling.get("beta_fast") or 32.0)), channel(float(scaling.get("beta_slow") or 1.0))
+    if scaling.get("truncate", True):
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, head_dim - 1)
+    width = (high - low) or 0.001
+    ramp = [min(1.0, max(0.0, (j - low) / width)) for j in range(head_dim // 2)]
+    factor = scaling.get("attention_factor")
+    if factor is None:
+        gain = lambda m: 0.1 * m * math.log(s) + 1.0 if s > 1.0 else 1.0  # noqa: E731
+        m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        factor = gain(float(m)) / gain(float(m_all)) if m and m_all else gain(1.0)
+    return tuple(v * (1.0 - r) + v / s * r for v, r in zip(inv, ramp)), float(factor)
 
 
 def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
@@ -46,15 +84,59 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
     return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
 
 
-def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float):
-    """Per-head RMSNorm over head_dim (skipped when the weight is None) followed by half-rotation RoPE.
-    q [T, Hq, d], k [T, Hkv, d]."""
+def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, layout: str = "half", offset: int = 0, inverse: bool = False) -> torch.Tensor:
+    """x [T, ..., d]: the channels [offset, offset + 2 P) rotate by cos/sin [T, P], the rest pass; arithmetic in fp32. `layout` "half" pairs
+    channel j with channel j + P of that range, "interleaved" the channels 2j and 2j + 1. `inverse` rotates back."""
+    r = 2 * cos.shape[-1]
+    shape = [cos.shape[0]] + [1] * (x.dim() - 2) + [cos.shape[-1]]
+    c, s = cos.float().reshape(shape), sin.float().reshape(shape)
+    if inverse:
+        s = -s
+    t = x[..., offset:offset + r].float()
+    if layout == "half":
+        x1, x2 = t[..., :r // 2], t[..., r // 2:]
+        t = torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
+    else:
+        x1, x2 = t[..., 0::2], t[..., 1::2]
+        t = torch.stack((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1).flatten(-2)
+    t = t.to(x.dtype)
+    return t if r == x.shape[-1] else torch.cat((x[..., :offset], t, x[..., offset + r:]), dim=-1)
+
+
+def head_norm_rope(x, weight, cos, sin, offset: int, interleaved: bool, eps: float, shift: float):
+    """x [T, H, d]: RMSNorm of every head (times weight + shift where there is a weight), then the rotation of `rope`; one rounding."""
+    xf = x.float()
+    xf = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        xf = xf * (shift + weight.float() if shift else weight.float())
+    return rope(xf, cos, sin, layout="interleaved" if interleaved else "half", offset=offset).to(x.dtype)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float, *, layout: str = "half", offset: int = 0, norm: bool | None = None,
+                 zero_centered: bool = False):
+    """Per-head RMSNorm over head_dim followed by RoPE. q [T, Hq, d], k [T, Hkv, d]. `norm` None: an operand without a weight is not
+    normalised; True: it is, without a factor; False: neither is. `zero_centered`: the factor is 1 + weight. `layout`, `offset`: see `rope`."""
     def one(x, w):
-        xf = x.float()
-        if w is not None:
-            xf = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
-        return _rope(xf, cos, sin).to(x.dtype)
+        if norm is False or (norm is None and w is None):
+            return rope(x, cos, sin, layout=layout, offset=offset)
+        return head_norm_rope(x, w, cos, sin, offset, layout == "interleaved", eps, 1.0 if zero_centered else 0.0)
     return one(q, q_weight), one(k, k_weight)
+
+
+def layer_norm(x, weight, bias, eps: float):
+    return F.layer_norm(x.float(), (x.shape[-1],), weight.float(), bias.float(), eps).to(x.dtype)
+
+
+ACTIVATIONS = {None: lambda z: z, "gelu": F.gelu, "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"), "silu": F.silu, "relu": F.relu}
+
+
+def linear_act(x, w, bias=None, *, activation: str | None = None, residual=None, product=linear):
+    """act(x W^T + bias) + residual; `product` is the linear map."""
+    y = product(x, w)
+    if bias is not None:
+        y = y + bias.to(x.dtype)
+    y = ACTIVATIONS[activation](y)
+    return y if residual is None else residual + y
 
 
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

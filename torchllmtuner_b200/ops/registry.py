@@ -31,7 +31,7 @@ def _register_builtins():
     from . import functional as F
     from . import reference as R
     for n in ("linear", "rms_norm", "add_rms_norm", "qk_norm_rope", "swiglu", "attention", "cross_entropy_sum",
-              "linear_cross_entropy_sum"):
+              "linear_cross_entropy_sum", "linear_act", "layer_norm", "rope"):
         register_kernel(n, "cuda", getattr(F, n))
         register_kernel(n, "cpu", getattr(R, n) if hasattr(R, n) else getattr(F, n))
 
