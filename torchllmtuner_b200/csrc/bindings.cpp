@@ -1281,12 +1281,12 @@ struct NativeHeadNormRope : public torch::autograd::Function<NativeHeadNormRope>
     h.dy = dy.data_ptr(); h.dy_tok = dy.stride(0); h.dy_head = dy.stride(1);
     int P = 0;
     if (need_w) {
-      P = llmt_qk_norm_rope_part_partials((int)x.size(0), h.H, 0, (int)x.size(2));
-      part = torch::empty({P, 2, x.size(2)}, x.options().dtype(at::kFloat));
+      P = llmt_qk_norm_rope_part_partials((int)x.size(0), h.H, (int)x.size(2));
+      part = torch::empty({P, x.size(2)}, x.options().dtype(at::kFloat));
     }
     const LlmtRopeShape rs = rope_shape(x, cosb, sinb, c, 1.f);
-    check_rc(llmt_qk_norm_rope_part_bwd(&rs, &h, nullptr, (float)eps, (float)shift, need_w ? part.data_ptr<float>() : nullptr, P,
-                                        need_w ? dw.data_ptr() : nullptr, nullptr, is_f32(x), cur_stream()),
+    check_rc(llmt_qk_norm_rope_part_bwd(&rs, &h, (float)eps, (float)shift, need_w ? part.data_ptr<float>() : nullptr, P,
+                                        need_w ? dw.data_ptr() : nullptr, is_f32(x), cur_stream()),
              "llmt_qk_norm_rope_part_bwd", need_w ? 2 : 1);
     return out;
   }
@@ -1341,6 +1341,13 @@ Tensor tma_rows(const Tensor& t) {
   r.copy_(t);
   return r;
 }
+// Partial sums of a product that is cut along its depth; of this call alone, so graphs and streams share nothing.
+Tensor linear_workspace(int64_t M, int64_t N, int64_t K, bool gradient, const Tensor& like) {
+  const int64_t n = llmt_linear_ws_floats((int)M, (int)N, (int)K, gradient);
+  return n > 0 ? torch::empty({n}, like.options().dtype(at::kFloat)) : Tensor();
+}
+inline float* ws_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+inline int64_t ws_size(const Tensor& t) { return t.defined() ? t.numel() : 0; }
 struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, int64_t act, bool keep) {
     c10::cuda::CUDAGuard guard(x.device());
@@ -1363,11 +1370,12 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
       if (M > 1 && r2.stride(0) < N && r2.stride(0) != 0) r2 = r2.contiguous();
     }
     if (act != 0 && keep) pre = torch::empty({M, (N + 7) / 8 * 8}, x.options());
+    const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), false, x);
     check_rc(llmt_linear_act(x2.data_ptr(), w2.data_ptr(), y.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, bc.defined() && is_f32(bc),
-                             r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, int_of(M, "rows"),
-                             int_of(N, "features"), int_of(K, "features"), x2.stride(0), w2.stride(0), N, r2.defined() ? r2.stride(0) : 0,
-                             pre.defined() ? pre.stride(0) : 0, status_ptr(), cur_stream()),
-             "llmt_linear_act");
+                             r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, (int)M,
+                             (int)N, (int)K, x2.stride(0), w2.stride(0), N, r2.defined() ? r2.stride(0) : 0, pre.defined() ? pre.stride(0) : 0,
+                             ws_ptr(ws), ws_size(ws), status_ptr(), cur_stream()),
+             "llmt_linear_act", ws.defined() ? 2 : 1);
     ctx->save_for_backward({x, w, b.has_value() ? *b : Tensor(), pre});
     ctx->saved_data["act"] = act;
     ctx->saved_data["residual"] = r.has_value();
@@ -1431,13 +1439,17 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     const int64_t lddz = dz.stride(0);
     if (nx) {
       out[0] = torch::empty(x.sizes(), x.options());
-      check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, status_ptr(), cur_stream()),
-               "llmt_linear_dx");
+      const Tensor ws = linear_workspace(M, K, N, true, dz);
+      check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, ws_ptr(ws), ws_size(ws),
+                              status_ptr(), cur_stream()),
+               "llmt_linear_dx", ws.defined() ? 2 : 1);
     }
     if (nw) {
       out[1] = torch::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
-      check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, status_ptr(), cur_stream()),
-               "llmt_linear_dw");
+      const Tensor ws = linear_workspace(N, K, M, true, dz);
+      check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, ws_ptr(ws), ws_size(ws),
+                              status_ptr(), cur_stream()),
+               "llmt_linear_dw", ws.defined() ? 2 : 1);
     }
     return out;
   }

@@ -31,10 +31,14 @@ int llmt_grouped_wgrad_bf16(const void* A, const void* B, void* C, const int* se
 int llmt_rmsnorm_fwd(const void* x, const void* res, const void* w, void* y, void* sum_out, float* rstd, int T, int D,
                      float eps, cudaStream_t st);
 // ---- linear layers with bias, activation (activations.cuh) and residual (linear_act.cu) ----
+int64_t llmt_linear_ws_floats(int M, int N, int K, int gradient);
 int llmt_linear_act(const void* x, const void* w, void* y, const void* bias, int bias_f32, const void* res, void* pre, int act, int M, int N, int K,
-                    int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, int* status, cudaStream_t stream);
-int llmt_linear_dx(const void* dz, const void* w, void* dx, int M, int N, int K, int64_t lddz, int64_t ldw, int64_t lddx, int* status, cudaStream_t stream);
-int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, int N, int K, int64_t lddz, int64_t ldx, int64_t lddw, int* status, cudaStream_t stream);
+                    int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, float* ws, int64_t ws_floats, int* status,
+                    cudaStream_t stream);
+int llmt_linear_dx(const void* dz, const void* w, void* dx, int M, int N, int K, int64_t lddz, int64_t ldw, int64_t lddx, float* ws, int64_t ws_floats,
+                   int* status, cudaStream_t stream);
+int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, int N, int K, int64_t lddz, int64_t ldx, int64_t lddw, float* ws, int64_t ws_floats,
+                   int* status, cudaStream_t stream);
 int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, int M, int N,
                    cudaStream_t stream);
 
@@ -56,9 +60,9 @@ typedef struct {
 int llmt_rope(const LlmtRopeShape* s, const LlmtHeads* a, const LlmtHeads* b, int f32, cudaStream_t stream);
 int llmt_qk_norm_rope_part_max_dim();
 int llmt_qk_norm_rope_part_fwd(const LlmtRopeShape* s, const LlmtHeads* q, const LlmtHeads* k, float eps, float shift, int f32, cudaStream_t stream);
-int llmt_qk_norm_rope_part_partials(int T, int Hq, int Hk, int d);
-int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* s, const LlmtHeads* q, const LlmtHeads* k, float eps, float shift, float* partial, int P,
-                               void* dwq, void* dwk, int f32, cudaStream_t stream);
+int llmt_qk_norm_rope_part_partials(int T, int H, int d);
+int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* s, const LlmtHeads* x, float eps, float shift, float* partial, int P, void* dw, int f32,
+                               cudaStream_t stream);
 int llmt_rope_tables(const int64_t* pos, const double* inv, int P, double factor, float* cosb, float* sinb, int64_t T, cudaStream_t stream);
 int llmt_layer_norm_max_width(int f32);
 int llmt_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean, float* rstd, int R, int D, float eps,

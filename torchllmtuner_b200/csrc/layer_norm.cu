@@ -158,19 +158,21 @@ layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict_
   }
 }
 
-// partial [grid][2][D]: sums of dy h and of dy over the block's rows.
-template <typename T, int NV, bool ALIGNED>
-__global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, int64_t ldx,
-                                                                              const T* __restrict__ w, const float* __restrict__ mean,
-                                                                              const float* __restrict__ rstd, T* __restrict__ dx,
-                                                                              float* __restrict__ partial, int R, int D, int tr) {
+// partial [grid][2][D]: sums of dy h and of dy over the block's rows. WARP: one warp per row, eight rows per block; otherwise the block is one
+// group. The sums of a column stay in registers over all rows (2 V NV of them, so an SM holds 256 threads); the next row is fetched before this
+// one is reduced.
+template <typename T, int NV, bool WARP, bool ALIGNED, int THREADS>
+__global__ void __launch_bounds__(THREADS, NV <= 2 ? 2 : 1) layer_norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, int64_t ldx,
+                                                                                 const T* __restrict__ w, const float* __restrict__ mean,
+                                                                                 const float* __restrict__ rstd, T* __restrict__ dx,
+                                                                                 float* __restrict__ partial, int R, int D, int tr) {
   constexpr int V = Granule<T>::V;
   __shared__ float2 red[2 * 32];
-  extern __shared__ float sums[];                       // [2][D], only with several groups
-  const int grp = threadIdx.x / tr, groups = blockDim.x / tr;
+  extern __shared__ __align__(16) float sums[];         // only with several groups
+  const int grp = WARP ? threadIdx.x >> 5 : 0, groups = WARP ? THREADS / 32 : 1;
   const int64_t step = (int64_t)gridDim.x * groups;
   int64_t row = (int64_t)blockIdx.x * groups + grp;
-  const RowPlace<V, ALIGNED> p{row < R ? shift_of(x + row * ldx) : 0, D, tr, (int)threadIdx.x - grp * tr};
+  const RowPlace<V, ALIGNED> p{row < R ? shift_of(x + row * ldx) : 0, D, tr, WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x};
   int buf = 0;
   float dw[NV][V], db[NV][V];
   Raw<T, V> wr[NV], xr[NV], gr[NV];
@@ -195,49 +197,59 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) layer_norm_bwd_kernel(co
   }
   const float inv_d = 1.f / (float)D;
   for (; row < R; row += step) {
-    float h[NV][V], g[NV][V];
     float2 s = make_float2(0.f, 0.f);
+    const float rr = r, mr = -m * r;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float wv[V];
-      xr[i].get(h[i]);
-      gr[i].get(g[i]);
-      mask_cols(p, i, h[i]);
-      mask_cols(p, i, g[i]);                            // a zero gradient keeps a foreign column out of every sum
+      float h[V], g[V], wv[V];
+      xr[i].get(h);
+      gr[i].get(g);
       if constexpr (ALIGNED) load_weights(w, p, i, wr[i]);
       wr[i].get(wv);
+      mask_cols(p, i, h);
+      mask_cols(p, i, g);                               // a zero gradient keeps a foreign column out of every sum
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        h[i][j] = (h[i][j] - m) * r;
-        dw[i][j] += g[i][j] * h[i][j];
-        db[i][j] += g[i][j];
-        g[i][j] *= wv[j];
-        s.x += g[i][j];
-        s.y += g[i][j] * h[i][j];
+        h[j] = h[j] * rr + mr;
+        dw[i][j] += g[j] * h[j];
+        db[i][j] += g[j];
+        g[j] *= wv[j];
+        s.x += g[j];
+        s.y += g[j] * h[j];
       }
     }
-    const float rr = r;
+    Raw<T, V> xn[NV], gn[NV];
     if (row + step < R) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        load_cols(x + (row + step) * ldx, p, i, xr[i]);
-        load_cols(dy + (row + step) * (int64_t)D, p, i, gr[i]);
+        load_cols(x + (row + step) * ldx, p, i, xn[i]);
+        load_cols(dy + (row + step) * (int64_t)D, p, i, gn[i]);
       }
       m = mean[row + step];
       r = rstd[row + step];
     }
-    s = group_sum2<false>(s, tr, red, buf);
-    s.x *= inv_d;
-    s.y *= inv_d;
+    s = group_sum2<WARP>(s, tr, red, buf);
+    // r (g w - mean - h k) with h = x r + mr, as one polynomial in x: fewer live registers than keeping h and g
+    const float k = s.y * inv_d, c0 = rr * (s.x * inv_d + mr * k), c1 = rr * rr * k;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      float h[V], g[V], wv[V];
+      xr[i].get(h);
+      gr[i].get(g);
+      if constexpr (ALIGNED) load_weights(w, p, i, wr[i]);
+      wr[i].get(wv);
 #pragma unroll
-      for (int j = 0; j < V; ++j) g[i][j] = rr * (g[i][j] - s.x - h[i][j] * s.y);
-      store_cols(dx + row * (int64_t)D, p, i, g[i]);
+      for (int j = 0; j < V; ++j) g[j] = rr * (g[j] * wv[j]) - (c1 * h[j] + c0);
+      store_cols(dx + row * (int64_t)D, p, i, g);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      xr[i] = xn[i];
+      gr[i] = gn[i];
     }
   }
   float* out = partial + (int64_t)blockIdx.x * 2 * D;
-  if (groups == 1) {
+  if constexpr (!WARP) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -248,6 +260,41 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) layer_norm_bwd_kernel(co
           out[D + c] = db[i][j];
         }
       }
+    return;
+  }
+  // the sums of the eight warps meet in a tree; a thread's columns are the same in every warp where rows are aligned, else they are shifted by
+  // the row: then the warps are added one after another
+  if constexpr (ALIGNED) {
+    float4* box = reinterpret_cast<float4*>(sums);      // [4 warps][2 NV V / 4][32 lanes]
+    constexpr int Q = 2 * NV * V / 4;
+#pragma unroll
+    for (int half = 4; half > 0; half >>= 1) {
+      if (grp >= half && grp < 2 * half) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const float* f = q < Q / 2 ? &dw[q * 4 / V][q * 4 % V] : &db[(q - Q / 2) * 4 / V][(q - Q / 2) * 4 % V];
+          box[((grp - half) * Q + q) * 32 + p.t] = make_float4(f[0], f[1], f[2], f[3]);
+        }
+      }
+      __syncthreads();
+      if (grp < half) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          float* f = q < Q / 2 ? &dw[q * 4 / V][q * 4 % V] : &db[(q - Q / 2) * 4 / V][(q - Q / 2) * 4 % V];
+          const float4 o = box[(grp * Q + q) * 32 + p.t];
+          f[0] += o.x; f[1] += o.y; f[2] += o.z; f[3] += o.w;
+        }
+      }
+      __syncthreads();
+    }
+    if (grp == 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (p.any(i)) {
+          store_vec<float, V>(out + p.col(i), dw[i]);
+          store_vec<float, V>(out + D + p.col(i), db[i]);
+        }
+    }
     return;
   }
   for (int k = 0; k < groups; ++k) {                    // the groups of a block are added in their order
@@ -265,7 +312,7 @@ __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1) layer_norm_bwd_kernel(co
     }
     __syncthreads();
   }
-  for (int c = threadIdx.x; c < 2 * D; c += blockDim.x) out[c] = sums[c];
+  for (int c = threadIdx.x; c < 2 * D; c += THREADS) out[c] = sums[c];
 }
 
 // dw | db [2 D] in T = column sums of partial [P][2 D]: 32 columns per block, its 32 warps take every 32nd row, fixed order.
@@ -289,16 +336,15 @@ __global__ void __launch_bounds__(1024) layer_norm_colsum_kernel(const float* __
 int sm_count();
 
 // Threads per row and vectors per thread. Forward: a warp per row while that is at most 8 vectors a thread (no barrier); beyond, 4 vectors.
-// Backward: two sums per column stay in registers, so 1 vector up to 512 threads, then 2 and 4.
+// Backward: a warp per row up to 5 vectors (what registers hold beside two sums per column), beyond 4 vectors and one group per block.
 struct LnShape { int tr, nv, groups; };
 static LnShape ln_fwd_shape(int vecs) {
   if (vecs <= 256) return {32, vecs <= 192 ? (vecs + 31) / 32 : 8, 8};
   return {(vecs + 127) / 128 * 32, 4, 1};
 }
 static LnShape ln_bwd_shape(int vecs) {
-  const int nv = vecs <= 512 ? 1 : vecs <= 1024 ? 2 : 4;
-  const int tr = (vecs + 32 * nv - 1) / (32 * nv) * 32;
-  return {tr, nv, tr >= 192 ? 1 : 384 / tr < 8 ? 384 / tr : 8};
+  if (vecs <= 160) return {32, (vecs + 31) / 32, 8};
+  return {(vecs + 127) / 128 * 32, 4, 1};
 }
 constexpr int kLnMaxVecs = 2048;
 
@@ -312,11 +358,11 @@ static bool ln_aligned(const void* x, int64_t ldx, int D) {
 
 template <typename T>
 static int ln_bwd_grid(int R, const LnShape& s) {
-  const int threads = s.tr * s.groups, V = Granule<T>::V;
-  const int most = sm_count() * ((s.nv == 1 ? 1024 : 512) / threads > 0 ? (s.nv == 1 ? 1024 : 512) / threads : 1);
+  const int V = Granule<T>::V;
+  const int most = sm_count() * (s.tr == 32 ? (s.nv <= 2 ? 2 : 1) : s.tr >= 256 ? 1 : 256 / s.tr);
   const int need = (R + s.groups - 1) / s.groups;
-  const int g = need < most ? need : most;
-  return (g + V - 1) / V * V;
+  if (need >= most) return most / V * V;                 // not beyond what the machine holds at once
+  return (need + V - 1) / V * V;
 }
 
 // All rows of an operand lie at row * ld; every operand has the same granule shift in the same row.
@@ -366,14 +412,16 @@ static int ln_bwd(const void* dy, const void* x, int64_t ldx, const void* w, con
   const LnShape s = ln_bwd_shape(vecs);
   const int grid = ln_bwd_grid<T>(R, s), threads = s.tr * s.groups;
   if (grid > P) return -10;
-  const size_t smem = s.groups > 1 ? (size_t)2 * D * sizeof(float) : 0;                  // several groups: at most 384 granules, 24 KB
+  constexpr int V = Granule<T>::V;
+  const size_t smem = s.groups == 1 ? 0 : aligned ? (size_t)4 * 2 * s.nv * V * 32 * sizeof(float) : (size_t)2 * D * sizeof(float);   // at most 40 KB
   const T *gp = reinterpret_cast<const T*>(dy), *xp = reinterpret_cast<const T*>(x), *wp = reinterpret_cast<const T*>(w);
-#define LLMT_LN(N)                                                                                                                             \
-  if (s.nv == N) {                                                                                                                             \
-    if (aligned) layer_norm_bwd_kernel<T, N, true><<<grid, threads, smem, stream>>>(gp, xp, ldx, wp, mean, rstd, reinterpret_cast<T*>(dx), partial, R, D, s.tr); \
-    else layer_norm_bwd_kernel<T, N, false><<<grid, threads, smem, stream>>>(gp, xp, ldx, wp, mean, rstd, reinterpret_cast<T*>(dx), partial, R, D, s.tr);        \
+#define LLMT_LN(N, W, TH)                                                                                                                      \
+  if (s.nv == N && (s.tr == 32) == W && threads <= TH && (TH == 256 || threads > 256)) {                                                       \
+    if (aligned) layer_norm_bwd_kernel<T, N, W, true, TH><<<grid, threads, smem, stream>>>(gp, xp, ldx, wp, mean, rstd, reinterpret_cast<T*>(dx), partial, R, D, s.tr); \
+    else layer_norm_bwd_kernel<T, N, W, false, TH><<<grid, threads, smem, stream>>>(gp, xp, ldx, wp, mean, rstd, reinterpret_cast<T*>(dx), partial, R, D, s.tr);        \
   }
-  LLMT_LN(1) LLMT_LN(2) LLMT_LN(4)
+  LLMT_LN(1, true, 256) LLMT_LN(2, true, 256) LLMT_LN(3, true, 256) LLMT_LN(4, true, 256) LLMT_LN(5, true, 256)
+  LLMT_LN(4, false, 256) LLMT_LN(4, false, 512)
 #undef LLMT_LN
   if (cudaGetLastError() != cudaSuccess) return -3;
   layer_norm_colsum_kernel<T><<<(2 * D + 31) / 32, 1024, 0, stream>>>(partial, reinterpret_cast<T*>(dw), reinterpret_cast<T*>(db), grid, D);

@@ -24,22 +24,36 @@ constexpr int kLMaxStages = 8;
 constexpr int kLStageA = kLM * kLK * 2;
 constexpr int kLSmem = 227 * 1024;
 constexpr int kLSmemFixed = kLEpiWarps * 4096 + 1024 /*alignment*/ + 512 /*barriers*/;
+constexpr int kMaxWorkers = 160;
 
-struct LinArgs {
-  int M, N, K;
-  int bn;                                // tile width over the whole worker, a multiple of 32, at most 256
-  int num_m, full_n, tiles;              // tile rows; whole tile columns; tiles (a narrower last column comes last)
-  int kb, stages, stage_bytes;
+// What becomes of a product: stored as it is, or (`fwd`) with bias, activation and residual.
+struct LinOut {
+  int M, N;
   __nv_bfloat16* C;
   int64_t ldc;
-  // forward epilogue
   const void* bias;
-  int bias_f32, act;
+  int bias_f32;
   const __nv_bfloat16* res;
   int64_t ldres;
   __nv_bfloat16* pre;
   int64_t ldpre;
   int vec;                               // every row of C, res and pre starts on 16 bytes and N is a multiple of 8
+};
+// The tiles of a product and who computes them. A tile is kLM * CG rows by `bn` columns (a multiple of 32, at most 512): up to 256 columns by one
+// MMA per 16 deep slice, and the accumulator is double buffered in TMEM, so that a tile is drained under the next one's products; the columns
+// beyond 256 by a second MMA, and then there is one accumulator. The last column of tiles may be narrower (its products
+// are issued with fewer columns and take that much less time). The k-blocks of a tile are cut into `splits` parts, each a unit of work. Units of
+// whole tiles go to the workers in turn, part by part, so that the workers read the same k-blocks at a time; the units of narrow tiles follow,
+// worker w taking narrow_begin[w] .. narrow_begin[w + 1].
+struct LinPlan {
+  int bn, num_m, full_n, splits, kb;
+  int stages, stage_bytes, b2_offset, workers;      // b2_offset: of the second MMA's columns of B in a stage
+  float* ws;                             // splits > 1: [splits][tiles][rows / 32][bn / 4][32][4] partial sums
+  uint16_t narrow_begin[kMaxWorkers + 1];
+};
+struct LinArgs {
+  LinOut out;
+  LinPlan plan;
   int* status;
 };
 
@@ -47,26 +61,165 @@ __device__ __forceinline__ uint32_t lin_idesc(int m, int n, bool a_mn, bool b_mn
   return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-struct LinTile { int m, n0, width; };    // tile row, first column, columns computed (a multiple of 32)
-__device__ __forceinline__ LinTile lin_tile(const LinArgs& a, int t, int group) {
-  const int whole = a.num_m * a.full_n;
-  if (t >= whole) {
-    const int n0 = a.full_n * a.bn;
-    return {t - whole, n0, (a.N - n0 + 31) & ~31};
+// One unit: tile row, first column, columns computed (a multiple of 32), index of the tile, k-blocks [kb0, kb1).
+struct LinUnit { int m, n0, width, tile, part, kb0, kb1; };
+// The units of worker `w` one after another; false when there are no more.
+struct LinWalk {
+  int next, narrow, narrow_end;
+  __device__ __forceinline__ LinWalk(const LinPlan& p, int w) : next(w), narrow(p.narrow_begin[w]), narrow_end(p.narrow_begin[w + 1]) {}
+  __device__ __forceinline__ bool step(const LinPlan& p, int N, int group, LinUnit& u) {
+    const int whole = p.num_m * p.full_n;
+    if (next < whole * p.splits) {
+      u.part = next / whole;
+      u.tile = next - u.part * whole;
+      // super-rows of `group` tile rows are swept column by column, so concurrent tiles cover a near-square patch and share operands in L2
+      const int per = group * p.full_n, g = u.tile / per, first = g * group;
+      const int gm = p.num_m - first < group ? p.num_m - first : group;
+      const int r = u.tile - g * per;
+      u.m = first + r % gm;
+      u.n0 = (r / gm) * p.bn;
+      u.width = p.bn;
+      next += p.workers;
+    } else if (narrow < narrow_end) {
+      u.part = narrow / p.num_m;
+      u.m = narrow - u.part * p.num_m;
+      u.tile = whole + u.m;
+      u.n0 = p.full_n * p.bn;
+      u.width = (N - u.n0 + 31) & ~31;
+      ++narrow;
+    } else {
+      return false;
+    }
+    u.kb0 = (int)((int64_t)p.kb * u.part / p.splits);
+    u.kb1 = (int)((int64_t)p.kb * (u.part + 1) / p.splits);
+    return true;
   }
-  // super-rows of `group` tile rows are swept column by column, so concurrent tiles cover a near-square patch and share operands in L2
-  const int per = group * a.full_n, g = t / per, first = g * group;
-  const int gm = a.num_m - first < group ? a.num_m - first : group;
-  const int r = t - g * per;
-  return {first + r % gm, (r / gm) * a.bn, a.bn};
+};
+
+__device__ __forceinline__ void load_bias8(const LinOut& o, int col, float* f) {
+  if (o.bias_f32) load_vec<float, 8>(reinterpret_cast<const float*>(o.bias) + col, f);
+  else load_vec<__nv_bfloat16, 8>(reinterpret_cast<const __nv_bfloat16*>(o.bias) + col, f);
+}
+// 32 rows x 64 columns of an operand of the epilogue, as 16 bytes per lane: row it * 4 + lane / 8, columns 8 (lane % 8) on. Clamped instead of
+// skipped, so that the eight loads are in flight together.
+__device__ __forceinline__ void load_patch(const __nv_bfloat16* p, int64_t ld, int row0, int col, int M, int end, int lane, uint4* v) {
+  const int c = col + (lane & 7) * 8 < end ? col + (lane & 7) * 8 : 0;
+#pragma unroll
+  for (int it = 0; it < 8; ++it)
+    v[it] = *reinterpret_cast<const uint4*>(p + (int64_t)min(row0 + it * 4 + (lane >> 3), M - 1) * ld + c);
+}
+// The staging rows (64 bf16 each) of a warp, to global memory in whole 128-byte lines. Chunks of 16 bytes are XORed with the row: no bank conflicts.
+__device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p, int64_t ld, int row0, int col, int M, int end, int lane) {
+  const int cc = lane & 7;
+  if (col + cc * 8 >= end) return;
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int rr = it * 4 + (lane >> 3);
+    const uint4 v = *reinterpret_cast<const uint4*>(stg + rr * 128 + ((cc ^ (rr & 7)) << 4));
+    if (row0 + rr < M) *reinterpret_cast<uint4*>(p + (int64_t)(row0 + rr) * ld + col + cc * 8) = v;
+  }
+}
+__device__ __forceinline__ void stage_row(uint8_t* stg, int lane, const uint32_t* packed) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
 }
 
-template <int CG, bool A_MN, bool B_MN, bool EPI>
+// A warp's 32 rows x 64 columns of sums (`acc`: 64 columns of row row0 + lane) become results: z = sum + bias, act(z) + residual in fp32, one
+// rounding. Columns from `end` on belong to another tile or to none. `res`: this patch of the residual (load_patch), used where RES. The bf16 rows are turned around in the warp's staging buffer, so
+// that global accesses run along rows.
+template <bool FWD, int ACT, bool RES>
+__device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int lane, int row0, int col0, int end, float* acc, const uint4* res) {
+  if (o.vec) {
+    if (FWD && o.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (col0 + 8 * j < end) {
+          float b[8];
+          load_bias8(o, col0 + 8 * j, b);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[8 * j + i] += b[i];
+        }
+      }
+    }
+    uint32_t packed[32];
+    if (FWD && ACT != kActNone && o.pre != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) packed[j] = pack_bf16x2(acc[2 * j], acc[2 * j + 1]);
+      __syncwarp();
+      stage_row(stg, lane, packed);
+      __syncwarp();
+      store_patch(stg, o.pre, o.ldpre, row0, col0, o.M, end, lane);
+    }
+    if (FWD) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = activate<ACT>(acc[j]);
+    }
+    if (FWD && RES) {
+      __syncwarp();
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int rr = it * 4 + (lane >> 3);
+        *reinterpret_cast<uint4*>(stg + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = res[it];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint4 v = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4));
+        float q[8];
+        unpack_bf16x2(v.x, q); unpack_bf16x2(v.y, q + 2); unpack_bf16x2(v.z, q + 4); unpack_bf16x2(v.w, q + 6);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[8 * j + i] += q[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) packed[j] = pack_bf16x2(acc[2 * j], acc[2 * j + 1]);
+    __syncwarp();
+    stage_row(stg, lane, packed);
+    __syncwarp();
+    store_patch(stg, o.C, o.ldc, row0, col0, o.M, end, lane);
+    return;
+  }
+  // rows off a 16-byte boundary: fp32 sums turned around 32 columns at a time, then a lane per column, one row after another
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float* turn = reinterpret_cast<float*>(stg);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) turn[lane * 32 + ((j + lane) & 31)] = acc[32 * half + j];
+    __syncwarp();
+    const int col = col0 + 32 * half + lane;
+    if (col >= end) continue;
+    float bias = 0.f;
+    if (FWD && o.bias != nullptr) {
+      if (o.bias_f32) bias = reinterpret_cast<const float*>(o.bias)[col];
+      else bias = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(o.bias)[col]);
+    }
+#pragma unroll 4
+    for (int rr = 0; rr < 32; ++rr) {
+      const int row = row0 + rr;
+      if (row >= o.M) break;
+      float v = turn[rr * 32 + ((lane + rr) & 31)];
+      if (FWD) {
+        v += bias;
+        if (ACT != kActNone && o.pre != nullptr) o.pre[(int64_t)row * o.ldpre + col] = __float2bfloat16_rn(v);
+        v = activate<ACT>(v);
+        if (RES) v += __bfloat162float(o.res[(int64_t)row * o.ldres + col]);
+      }
+      o.C[(int64_t)row * o.ldc + col] = __float2bfloat16_rn(v);
+    }
+  }
+}
+
+// WIDE: tiles of more than 256 columns (CTA pairs only).
+template <int CG, bool WIDE, bool A_MN, bool B_MN, bool SPLIT, bool FWD, int ACT, bool RES>
 __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                                                              const __grid_constant__ LinArgs a) {
+                                                              const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ LinArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi = smem + a.stages * a.stage_bytes;
+  const LinPlan& plan = a.plan;
+  const int stages = plan.stages, stage_bytes = plan.stage_bytes;
+  uint8_t* epi = smem + stages * stage_bytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(epi + kLEpiWarps * 4096);
   uint64_t* empty = full + kLMaxStages;
   uint64_t* tfull = empty + kLMaxStages;
@@ -74,13 +227,13 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // known to be the same in the whole warp
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0u;
-  const int unit = blockIdx.x / CG, units = gridDim.x / CG;
+  const int worker = blockIdx.x / CG;
   constexpr int kGroup = 16 / CG;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -100,50 +253,69 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  LinWalk walk(plan, worker);
+  LinUnit u;
+  constexpr int accs = WIDE ? 1 : 2;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      tma_prefetch_desc(&tmA);
-      tma_prefetch_desc(&tmB);
+    // The whole warp walks the loop with uniform control flow and one lane issues: inside a branch of one lane every TMA instruction took about 75
+    // clocks and every MMA about 115, and a k-block 440 to 800 clocks whatever the tile's width (its products of 256 columns occupy the tensor
+    // pipe for 512).
+    {
+      const bool leader = elect_one();
+      if (leader) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+      }
       int stage = 0;
       uint32_t phase = 0, armed = 0, armed_parity = 0;
       bool ok = true;
-      const int b_rows = a.bn / CG;                     // rows of B per load (a narrow tile loads as many and uses fewer)
-      for (int t = unit; t < a.tiles && ok; t += units) {
-        const LinTile tile = lin_tile(a, t, kGroup);
-        const int m0 = (tile.m * CG + (int)rank) * kLM, nb = tile.n0 + (int)rank * (tile.width / CG);
-        for (int kb = 0; kb < a.kb; ++kb) {
+      // rows of B per load and MMA (a narrow tile loads as many and uses fewer)
+      const int b_rows = (WIDE ? 256 : plan.bn) / CG, b2_rows = WIDE ? (plan.bn - 256) / CG : 0;
+      // the transaction bytes of both CTAs' loads are counted by the leader's barrier
+      const uint32_t full0 = CG == 2 ? cluster_map_u32(smem_u32(full), 0) : smem_u32(full);
+      while (ok && walk.step(plan, a.out.N, kGroup, u)) {
+        const int m0 = (u.m * CG + (int)rank) * kLM, w1 = WIDE ? min(u.width, 256) : u.width, nb = u.n0 + (int)rank * (w1 / CG),
+                  nb2 = u.n0 + w1 + (int)rank * ((u.width - w1) / CG);
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1, abort_flag, a.status, 500 + stage)) {
             ok = false;
             break;
           }
-          uint8_t* sa = smem + stage * a.stage_bytes;
-          uint8_t* sb = sa + kLStageA;
           if (rank == 0) {
-            mbar_arrive_expect_tx(&full[stage], CG * a.stage_bytes);
             armed |= 1u << stage;
             armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
           }
-          const int k0 = kb * kLK;
-          const uint32_t bar = CG == 2 ? cluster_map_u32(smem_u32(&full[stage]), 0) : 0u;
-          auto load = [&](void* dst, const CUtensorMap* m, int c0, int c1) {
-            if constexpr (CG == 2) tma_load_2d_pair(dst, m, bar, c0, c1);
-            else tma_load_2d(dst, m, &full[stage], c0, c1);
-          };
-          if constexpr (!A_MN) load(sa, &tmA, k0, m0);
-          else {
+          if (leader) {
+            uint8_t* sa = smem + stage * stage_bytes;
+            uint8_t* sb = sa + kLStageA;
+            if (rank == 0) mbar_arrive_expect_tx(&full[stage], CG * stage_bytes);
+            const int k0 = kb * kLK;
+            auto load = [&](void* dst, const CUtensorMap* m, int c0, int c1) {
+              if constexpr (CG == 2) tma_load_2d_pair(dst, m, full0 + 8 * stage, c0, c1);
+              else tma_load_2d(dst, m, &full[stage], c0, c1);
+            };
+            if constexpr (!A_MN) load(sa, &tmA, k0, m0);
+            else {
 #pragma unroll
-            for (int j = 0; j < kLM / 64; ++j) load(sa + j * (kLK * 128), &tmA, m0 + 64 * j, k0);
+              for (int j = 0; j < kLM / 64; ++j) load(sa + j * (kLK * 128), &tmA, m0 + 64 * j, k0);
+            }
+            if constexpr (!B_MN) {
+              load(sb, &tmB, k0, nb);
+              if (WIDE) load(sa + plan.b2_offset, &tmB2, k0, nb2);
+            } else {
+              for (int j = 0; j * 64 < b_rows; ++j) load(sb + j * (kLK * 128), &tmB, nb + 64 * j, k0);
+              if (WIDE)
+                for (int j = 0; j * 64 < b2_rows; ++j) load(sa + plan.b2_offset + j * (kLK * 128), &tmB, nb2 + 64 * j, k0);
+            }
           }
-          if constexpr (!B_MN) load(sb, &tmB, k0, nb);
-          else
-            for (int j = 0; j * 64 < b_rows; ++j) load(sb + j * (kLK * 128), &tmB, nb + 64 * j, k0);
-          if (++stage == a.stages) { stage = 0; phase ^= 1; }
+          __syncwarp();
+          if (++stage == stages) { stage = 0; phase ^= 1; }
         }
       }
       if (*abort_flag) {                                // copies in flight land before this CTA's shared memory is released
-        for (int s = 0; s < a.stages; ++s) {
+        for (int s = 0; s < stages; ++s) {
           if (!(armed & (1u << s))) continue;
           const uint32_t par = (armed_parity >> s) & 1u;
           for (uint32_t i = 0; i < (1u << 16); ++i)
@@ -154,143 +326,95 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool leader = elect_one();
+      // lower words of the operand descriptors at stage 0; a stage further on is lstep (16-byte units), the second MMA's columns b2step
+      const uint32_t la0 = desc_lo(smem_u32(smem), A_MN ? kLK * 128 : 16), lb0 = desc_lo(smem_u32(smem) + kLStageA, B_MN ? kLK * 128 : 16);
+      const uint32_t lstep = stage_bytes >> 4, b2step = (plan.b2_offset - kLStageA) >> 4;
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = unit; t < a.tiles && ok; t += units) {
-        const uint32_t idesc = lin_idesc(kLM * CG, lin_tile(a, t, kGroup).width, A_MN, B_MN);
+      while (ok && walk.step(plan, a.out.N, kGroup, u)) {
+        const uint32_t idesc = lin_idesc(kLM * CG, WIDE ? min(u.width, 256) : u.width, A_MN, B_MN);
+        const uint32_t idesc2 = WIDE ? lin_idesc(kLM * CG, u.width - 256, A_MN, B_MN) : 0u;
+        const bool second = WIDE && u.width > 256;
         if (!mbar_wait_bounded<CG == 2>(&tempty[acc], acc_phase ^ 1, abort_flag, a.status, 600 + acc)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256;
-        for (int kb = 0; kb < a.kb; ++kb) {
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait_bounded(&full[stage], phase, abort_flag, a.status, 700 + stage)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * a.stage_bytes), sb = sa + kLStageA;
-          const uint32_t la = desc_lo(sa, A_MN ? kLK * 128 : 16), lb = desc_lo(sb, B_MN ? kLK * 128 : 16);
-          const uint32_t acc0 = kb ? 1u : 0u;
+          if (leader) {
+            const uint32_t la = la0 + stage * lstep, lb = lb0 + stage * lstep, acc0 = kb > u.kb0 ? 1u : 0u;
+            auto slices = [&](uint32_t d, uint32_t b, uint32_t id) {
 #pragma unroll
-          for (int k = 0; k < kLK / 16; ++k) {
-            const uint64_t da = desc_pack(la + (A_MN ? k * 128 : k * 2));
-            const uint64_t db = desc_pack(lb + (B_MN ? k * 128 : k * 2));
-            if constexpr (CG == 2) umma_bf16_ss_pair(d_tmem, da, db, idesc, k ? 1u : acc0);
-            else umma_bf16_ss(d_tmem, da, db, idesc, k ? 1u : acc0);
+              for (int k = 0; k < kLK / 16; ++k) {
+                const uint64_t da = desc_pack(la + (A_MN ? k * 128 : k * 2)), db = desc_pack(b + (B_MN ? k * 128 : k * 2));
+                if constexpr (CG == 2) umma_bf16_ss_pair(d, da, db, id, k ? 1u : acc0);
+                else umma_bf16_ss(d, da, db, id, k ? 1u : acc0);
+              }
+            };
+            slices(d_tmem, lb, idesc);
+            if (WIDE && second) slices(d_tmem + 256, lb + b2step, idesc2);
+            if constexpr (CG == 2) umma_commit_pair(&empty[stage]);
+            else umma_commit(&empty[stage]);
           }
-          if constexpr (CG == 2) umma_commit_pair(&empty[stage]);
-          else umma_commit(&empty[stage]);
-          if (++stage == a.stages) { stage = 0; phase ^= 1; }
+          __syncwarp();
+          if (++stage == stages) { stage = 0; phase ^= 1; }
         }
         if (!ok) break;
-        if constexpr (CG == 2) umma_commit_pair(&tfull[acc]);
-        else umma_commit(&tfull[acc]);
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        if (leader) {
+          if constexpr (CG == 2) umma_commit_pair(&tfull[acc]);
+          else umma_commit(&tfull[acc]);
+        }
+        __syncwarp();
+        if (++acc == accs) { acc = 0; acc_phase ^= 1; }
       }
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ epilogue
-    // A warp turns 32 rows x 32 columns (fp32) around in shared memory, so that global accesses run along rows. Two warps share a quarter of
-    // the rows and take alternate chunks of columns.
+    // Two warps share a quarter of the rows (the TMEM lanes a warp may read) and take alternate patches of 64 columns.
     const int quarter = warp & 3, side = (warp - 2) >> 2;
     uint8_t* stg = epi + (warp - 2) * 4096;
-    const int rr0 = lane >> 3, cc = lane & 7;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = unit; t < a.tiles; t += units) {
-      const LinTile tile = lin_tile(a, t, kGroup);
-      const int row0 = (tile.m * CG + (int)rank) * kLM + quarter * 32;
-      const int cols = min(tile.width, a.N - tile.n0);
-      if (EPI && a.res != nullptr) {                    // the residual's rows come into L2 while the product is computed
-        const int pr = min(row0 + lane, a.M - 1);
-        const uint8_t* line = reinterpret_cast<const uint8_t*>(a.res + (int64_t)pr * a.ldres + tile.n0);
+    while (walk.step(plan, a.out.N, kGroup, u)) {
+      const int row0 = (u.m * CG + (int)rank) * kLM + quarter * 32;
+      const int cols = min(u.width, a.out.N - u.n0);
+      if (RES) {                                        // the residual's rows come into L2 while the product is computed
+        const uint8_t* line = reinterpret_cast<const uint8_t*>(a.out.res + (int64_t)min(row0 + lane, a.out.M - 1) * a.out.ldres + u.n0);
         for (int o = side * 128; o < cols * 2; o += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + o));
       }
       if (!mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, a.status, 800 + acc)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
 #pragma unroll 1
-      for (int c = side * 32; c < cols; c += 64) {
-        uint32_t r[32];
+      for (int c = side * 64; c < cols; c += 128) {
+        uint32_t r[64];
         tmem_ld_32x32(t_row + c, r);
-        const int col0 = tile.n0 + c;
-        if (a.vec) {
-          const int col = col0 + cc * 4;
-          const bool col_ok = col < a.N;
-          uint2 old[8];
-          float bias[4] = {0.f, 0.f, 0.f, 0.f};
-          if constexpr (EPI) {
-            if (a.bias != nullptr && col_ok) {
-              if (a.bias_f32) load_vec<float, 4>(reinterpret_cast<const float*>(a.bias) + col, bias);
-              else load_vec<__nv_bfloat16, 4>(reinterpret_cast<const __nv_bfloat16*>(a.bias) + col, bias);
-            }
-            if (a.res != nullptr) {                     // clamped instead of skipped: eight loads in flight together
-              const int64_t at = col_ok ? col : tile.n0;
+        tmem_ld_32x32(t_row + c + 32, r + 32);
+        uint4 res[RES ? 8 : 1];
+        if (RES && a.out.vec) load_patch(a.out.res, a.out.ldres, row0, u.n0 + c, a.out.M, u.n0 + cols, lane, res);
+        tmem_wait_ld();
+        if constexpr (SPLIT) {
+          const int64_t tiles = (int64_t)plan.num_m * plan.full_n + (a.out.N % plan.bn ? plan.num_m : 0);
+          float4* w = reinterpret_cast<float4*>(plan.ws) + (((u.part * tiles + u.tile) * (CG * 4) + rank * 4 + quarter) * (plan.bn / 4) + c / 4) * 32 + lane;
 #pragma unroll
-              for (int it = 0; it < 8; ++it)
-                old[it] = *reinterpret_cast<const uint2*>(a.res + (int64_t)min(row0 + rr0 + it * 4, a.M - 1) * a.ldres + at);
-            }
-          }
-          tmem_wait_ld();
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int rr = it * 4 + rr0, row = row0 + rr;
-            const uint4 v = *reinterpret_cast<const uint4*>(stg + rr * 128 + ((cc ^ (rr & 7)) << 4));
-            float o[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
-            if constexpr (EPI) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) o[j] += bias[j];
-              if (a.pre != nullptr && col_ok && row < a.M) store_vec<__nv_bfloat16, 4>(a.pre + (int64_t)row * a.ldpre + col, o);
-              activate<4>(a.act, o);
-              if (a.res != nullptr) {
-                float q[4];
-                unpack_bf16x2(old[it].x, q);
-                unpack_bf16x2(old[it].y, q + 2);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] += q[j];
-              }
-            }
-            if (col_ok && row < a.M) store_vec<__nv_bfloat16, 4>(a.C + (int64_t)row * a.ldc + col, o);
-          }
-        } else {                                        // rows off a 16-byte boundary: a lane per column, one row after another
-          tmem_wait_ld();
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) reinterpret_cast<uint32_t*>(stg)[lane * 32 + ((j + lane) & 31)] = r[j];
-          __syncwarp();
-          const int col = col0 + lane;
-          if (col < a.N) {
-            float bias = 0.f;
-            if constexpr (EPI) {
-              if (a.bias != nullptr) bias = a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[col] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.bias)[col]);
-            }
-#pragma unroll 4
-            for (int rr = 0; rr < 32; ++rr) {
-              const int row = row0 + rr;
-              if (row >= a.M) break;
-              float o[1] = {__uint_as_float(reinterpret_cast<uint32_t*>(stg)[rr * 32 + ((lane + rr) & 31)])};
-              if constexpr (EPI) {
-                o[0] += bias;
-                if (a.pre != nullptr) a.pre[(int64_t)row * a.ldpre + col] = __float2bfloat16_rn(o[0]);
-                activate<1>(a.act, o);
-                if (a.res != nullptr) o[0] += __bfloat162float(a.res[(int64_t)row * a.ldres + col]);
-              }
-              a.C[(int64_t)row * a.ldc + col] = __float2bfloat16_rn(o[0]);
-            }
-          }
+          for (int j = 0; j < 16; ++j)
+            if (c + 4 * j < u.width)
+              w[j * 32] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+        } else {
+          finish_patch<FWD, ACT, RES>(a.out, stg, lane, row0, u.n0 + c, u.n0 + cols, reinterpret_cast<float*>(r), res);
         }
       }
       tc_fence_before();
       if constexpr (CG == 2) mbar_arrive_cluster(cluster_map_u32(smem_u32(&tempty[acc]), 0));
       else mbar_arrive(&tempty[acc]);
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      if (++acc == accs) { acc = 0; acc_phase ^= 1; }
     }
   }
 
@@ -304,16 +428,54 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
   }
 }
 
+// The parts of every tile added in their order, and the epilogue: a warp per 32 rows x 64 columns.
+constexpr int kJoinWarps = 4;
+template <bool FWD, int ACT, bool RES>
+__global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __grid_constant__ LinArgs a, int cg, int patches) {
+  __shared__ __align__(16) uint8_t stage[kJoinWarps][4096];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int id = blockIdx.x * kJoinWarps + wid;
+  if (id >= patches) return;
+  const LinPlan& p = a.plan;
+  const int blocks = cg * 4, per_tile_row = (a.out.N + 63) / 64;
+  const int mb = id / per_tile_row, col0 = (id - mb * per_tile_row) * 64;      // 32-row block, first column
+  const int row0 = mb * 32, m = mb / blocks, block = mb - m * blocks;
+  const int n = col0 / p.bn, c = col0 - n * p.bn, whole = p.num_m * p.full_n;
+  int tile;
+  if (n >= p.full_n) tile = whole + m;
+  else {
+    const int group = 16 / cg, g = m / group, first = g * group, gm = p.num_m - first < group ? p.num_m - first : group;
+    tile = g * group * p.full_n + n * gm + (m - first);
+  }
+  const int width = n >= p.full_n ? (a.out.N - n * p.bn + 31) & ~31 : p.bn;
+  const int64_t tiles = (int64_t)whole + (a.out.N % p.bn ? p.num_m : 0), part = tiles * blocks * (p.bn / 4) * 32;
+  const float4* w = reinterpret_cast<const float4*>(p.ws) + (((int64_t)tile * blocks + block) * (p.bn / 4) + c / 4) * 32 + lane;
+  uint4 res[8];
+  if (RES && a.out.vec) load_patch(a.out.res, a.out.ldres, row0, col0, a.out.M, a.out.N, lane, res);
+  float acc[64];
+#pragma unroll
+  for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c + 4 * j < width) {
+        const float4 v = w[s * part + j * 32];
+        acc[4 * j] += v.x; acc[4 * j + 1] += v.y; acc[4 * j + 2] += v.z; acc[4 * j + 3] += v.w;
+      }
+  }
+  finish_patch<FWD, ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N, acc, res);
+}
+
 // ------------------------------------------------------------------------------------------ dz and db
 // A block owns a strip of columns and every eighth group of rows; the eight blocks of a cluster add their column sums through distributed
 // shared memory in rank order, so db needs neither a second launch nor a workspace nor atomics.
 constexpr int kStripBlocks = 8;
-template <int V, int THREADS>
-__global__ void __launch_bounds__(THREADS) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy, const __nv_bfloat16* __restrict__ z,
-                                                            int64_t ldz, int act, __nv_bfloat16* __restrict__ dz, int64_t lddz, void* __restrict__ db,
+template <int V, int THREADS, int ACT>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy, const __nv_bfloat16* __restrict__ z,
+                                                            int64_t ldz, __nv_bfloat16* __restrict__ dz, int64_t lddz, void* __restrict__ db,
                                                             int db_f32, int M, int N) {
   constexpr int LANES = V == 8 ? 8 : 32, COLS = LANES * V, ROWS = THREADS / LANES;
-  __shared__ float part[ROWS][COLS + 1];
+  __shared__ float part[ROWS / (THREADS / 256)][COLS + 1];
   __shared__ float total[COLS];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const int col = blockIdx.x * COLS + lane * V;
@@ -322,28 +484,45 @@ __global__ void __launch_bounds__(THREADS) linear_dz_kernel(const __nv_bfloat16*
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   if (col < N) {
-#pragma unroll 4
-    for (int64_t row = (int64_t)rank * ROWS + sub; row < M; row += ROWS * kStripBlocks) {
-      float g[V];
-      load_vec<__nv_bfloat16, V>(dy + row * ldy + col, g);
-      if (z != nullptr) {
-        float p[V];
-        load_vec<__nv_bfloat16, V>(z + row * ldz + col, p);
-        activate_grad<V>(act, p, g);
-      }
+    constexpr int U = 4;                                 // rows in flight per thread
+    const int64_t step = (int64_t)ROWS * kStripBlocks;
+    for (int64_t row = (int64_t)rank * ROWS + sub; row < M; row += U * step) {
+      Raw<__nv_bfloat16, V> rg[U], rz[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += g[j];
-      if (dz != nullptr) store_vec<__nv_bfloat16, V>(dz + row * lddz + col, g);
+      for (int u = 0; u < U; ++u)
+        if (row + u * step < M) {
+          rg[u].load(dy + (row + u * step) * ldy + col);
+          if (ACT != kActNone) rz[u].load(z + (row + u * step) * ldz + col);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (row + u * step >= M) break;
+        float g[V], p[V];
+        rg[u].get(g);
+        if (ACT != kActNone) {
+          rz[u].get(p);
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] = activate_grad<ACT>(p[j], g[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += g[j];
+        if (dz != nullptr) store_vec<__nv_bfloat16, V>(dz + (row + u * step) * lddz + col, g);
+      }
     }
   }
   if (db == nullptr) return;
+  constexpr int HELD = ROWS / (THREADS / 256);          // rows of sums in shared memory; the groups of HELD threads' rows follow one another
 #pragma unroll
-  for (int j = 0; j < V; ++j) part[sub][lane * V + j] = acc[j];
-  __syncthreads();
+  for (int k = 0; k < THREADS / 256; ++k) {
+    if (sub / HELD == k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) part[sub % HELD][lane * V + j] = k ? part[sub % HELD][lane * V + j] + acc[j] : acc[j];
+    __syncthreads();
+  }
   if (threadIdx.x < COLS) {
     float s = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < ROWS; ++i) s += part[i][threadIdx.x];
+    for (int i = 0; i < HELD; ++i) s += part[i][threadIdx.x];
     total[threadIdx.x] = s;
   }
   cluster_sync();
@@ -373,62 +552,187 @@ static bool allow_smem(F kern, int bytes, uint64_t& done) {
   return true;
 }
 
-template <int CG, bool A_MN, bool B_MN, bool EPI>
-static int lin_launch(const CUtensorMap& ta, const CUtensorMap& tb, const LinArgs& a, cudaStream_t stream) {
-  static uint64_t done = 0;
-  auto kern = linear_kernel<CG, A_MN, B_MN, EPI>;
+template <typename K>
+static int lin_run(K kern, uint64_t& done, int cg, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LinArgs& a, cudaStream_t stream) {
   if (!allow_smem(kern, kLSmem, done)) return -2;
-  const int most = sm_count() / CG;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((a.tiles < most ? a.tiles : most) * CG);
+  cfg.gridDim = dim3(a.plan.workers * cg);
   cfg.blockDim = dim3(kLThreads);
-  cfg.dynamicSmemBytes = a.stages * a.stage_bytes + kLSmemFixed;
+  cfg.dynamicSmemBytes = a.plan.stages * a.plan.stage_bytes + kLSmemFixed;
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = CG; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  at.val.clusterDim.x = cg; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, ta, tb, a) == cudaSuccess ? 0 : -3;
+  cfg.numAttrs = cg == 2 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, ta, tb, tb2, a) == cudaSuccess ? 0 : -3;
+}
+template <bool A_MN, bool B_MN, bool SPLIT, bool FWD, int ACT, bool RES>
+static int lin_launch(int cg, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LinArgs& a, cudaStream_t stream) {
+  static uint64_t single = 0, pair = 0, wide = 0;
+  if (cg == 1) return lin_run(linear_kernel<1, false, A_MN, B_MN, SPLIT, FWD, ACT, RES>, single, 1, ta, tb, tb2, a, stream);
+  if (a.plan.bn <= 256) return lin_run(linear_kernel<2, false, A_MN, B_MN, SPLIT, FWD, ACT, RES>, pair, 2, ta, tb, tb2, a, stream);
+  return lin_run(linear_kernel<2, true, A_MN, B_MN, SPLIT, FWD, ACT, RES>, wide, 2, ta, tb, tb2, a, stream);
+}
+template <bool FWD, int ACT, bool RES>
+static int lin_join(int cg, const LinArgs& a, cudaStream_t stream) {
+  const int patches = a.plan.num_m * cg * 4 * ((a.out.N + 63) / 64);
+  linear_join_kernel<FWD, ACT, RES><<<(patches + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, stream>>>(a, cg, patches);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-// C[M, N] = op(A) op(B) as in llmt_gemm_bf16 (tn, nn and tt layouts); e: the forward's epilogue, or nullptr.
-static int lin_gemm(const void* A, const void* B, LinArgs a, int64_t lda, int64_t ldb, bool a_mn, bool b_mn, bool epi, cudaStream_t stream) {
-  if (a.M <= 0 || a.N <= 0) return 0;
-  if (a.K <= 0 || (lda & 7) || (ldb & 7) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return -10;
-  if ((epi && (a_mn || b_mn)) || (a_mn && !b_mn)) return -4;
-  const int cg = a.M > kLM ? 2 : 1;
-  a.bn = a.N > 128 ? 256 : 128;
-  a.num_m = (a.M + kLM * cg - 1) / (kLM * cg);
-  a.full_n = a.N / a.bn;
-  a.tiles = a.num_m * (a.full_n + (a.N % a.bn ? 1 : 0));
-  a.kb = (a.K + kLK - 1) / kLK;
-  const int b_rows = a.bn / cg;
-  a.stage_bytes = kLStageA + (b_mn ? (b_rows + 63) / 64 * 64 : b_rows) * kLK * 2;
-  a.stages = (kLSmem - kLSmemFixed) / a.stage_bytes;
-  if (a.stages > kLMaxStages) a.stages = kLMaxStages;
-  CUtensorMap ta, tb;
+struct LinCut { int cg, bn, splits; };
+static int64_t lin_ws_floats(int M, int N, const LinCut& c) {
+  if (c.splits < 2) return 0;
+  const int64_t num_m = (M + kLM * c.cg - 1) / (kLM * c.cg), num_n = (N + c.bn - 1) / c.bn;
+  return c.splits * num_m * num_n * kLM * c.cg * c.bn;
+}
+
+// Time of one k-block of a tile, in ns. Alone the products bound it (256 columns 302, 192 230, 128 and fewer about 200 with the loop around them);
+// with every SM at it the operands, which come from L2 at 10 to 13 TB/s: 256 columns 420, 192 360, 128 260 (16384 x 4608 x 1152). `loaded`: columns
+// that the TMA boxes fetch, more than `bn` where B is stored [K][N] and half a tile is no multiple of 64.
+static double lin_kb_ns(int bn, int loaded, double busy) {
+  const double alone = bn * 1.18 > 200 ? bn * 1.18 : 200, crowded = 90 + 0.65 * (bn + loaded);
+  return crowded > alone ? alone + (crowded - alone) * busy : alone;
+}
+// Units of whole tiles go round the workers; those of narrow tiles go one by one to the worker that is free first.
+static void lin_plan(LinPlan& p, int N, int num_tiles_m, int most) {
+  p.full_n = N / p.bn;
+  p.num_m = num_tiles_m;
+  const int rest = N - p.full_n * p.bn, whole = p.num_m * p.full_n * p.splits, narrow = rest ? p.num_m * p.splits : 0;
+  p.workers = whole + narrow < most ? whole + narrow : most;
+  const int ahead = whole % p.workers;                   // workers [0, ahead) have one whole unit more
+  const int behind = ahead ? p.workers - ahead : 0;
+  const int fit = rest ? (int)(lin_kb_ns(p.bn, p.bn, 0) / lin_kb_ns((rest + 31) / 32 * 32, 0, 0) + 0.1) : 0;       // narrow units in the time of a whole one
+  const int catch_up = narrow < behind * fit ? narrow : behind * fit, left = narrow - catch_up;
+  int at = 0;
+  for (int w = 0; w < p.workers; ++w) {
+    p.narrow_begin[w] = (uint16_t)at;
+    if (w >= ahead && behind) at += catch_up / behind + (w - ahead < catch_up % behind ? 1 : 0);
+    at += left / p.workers + (w < left % p.workers ? 1 : 0);
+  }
+  p.narrow_begin[p.workers] = (uint16_t)at;
+}
+// The longest worker's units, in us (kb deep, `splits` parts).
+static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb, bool b_mn) {
+  const int most = sm_count() / cg, full_n = N / bn, rest = N - full_n * bn, whole = num_m * full_n * splits, narrow = rest ? num_m * splits : 0;
+  const int workers = whole + narrow < most ? whole + narrow : most;
+  const double depth = (double)((kb + splits - 1) / splits);
+  const int loaded = b_mn ? (bn + 64 * cg - 1) / (64 * cg) * 64 * cg : bn;
+  // a tile is not done before its sums are drained: about 0.9 us per 128 columns, hidden under the next tile's products where there are two
+  // accumulators
+  auto unit = [&](int w, int running) {
+    const double drain = 0.9 * w / 128, mma = depth * lin_kb_ns(w, loaded, (double)running * cg / sm_count()) * 1e-3;
+    return bn > 256 ? mma + drain : mma > drain ? mma : drain;
+  };
+  const int rounds = whole / workers, ahead = whole % workers, behind = ahead ? workers - ahead : 0;
+  double t = rounds * unit(bn, workers) + (ahead ? unit(bn, ahead + (narrow < behind ? narrow : behind)) : 0);
+  if (narrow) {
+    const double tn = unit((rest + 31) / 32 * 32, workers);
+    const int fit = full_n ? (int)(unit(bn, workers) / tn + 0.1) : 0, left = narrow - (narrow < behind * fit ? narrow : behind * fit);
+    t += tn * ((left + workers - 1) / workers);
+  }
+  return t + (bn > 256 ? 0 : 0.9 * (full_n ? bn : rest) / 128);
+}
+
+// How a product is cut: CTAs per tile, tile width and parts along K. The shortest of the candidates by the estimate: tile widths that divide N
+// evenly into 1, 2, ... columns of tiles, one CTA or a pair, and parts along K where the tiles leave workers idle. The parts cost a second
+// launch and their sums in memory: 5.5 us and 4 bytes per sum and part at 4 TB/s (1152 x 1152 in 3 parts: 8.0 us).
+static LinCut lin_find_cut(int M, int N, int K, bool b_mn) {
+  const int kb = (K + kLK - 1) / kLK;
+  LinCut best{1, 128, 1};
+  double least = 1e30;
+  for (int cg = 1; cg <= (M > kLM ? 2 : 1); ++cg) {
+    const int num_m = (M + kLM * cg - 1) / (kLM * cg), most = sm_count() / cg;
+    const int widest = cg == 2 ? 512 : 256;              // at least four stages of operands fit shared memory
+    int last = 0;
+    if (num_m > 65535) continue;
+    for (int n = (N + widest - 1) / widest; n <= (N + 127) / 128; ++n) {
+      const int bn = ((N + n - 1) / n + 31) / 32 * 32;
+      if (bn == last) continue;
+      last = bn;
+      const int tiles = num_m * ((N + bn - 1) / bn);
+      for (int splits = 1; splits == 1 || (splits <= 8 && splits * 2 <= kb); ++splits) {
+        if (splits > 1 && (bn % 64 || tiles * (splits - 1) >= 2 * most || (int64_t)num_m * splits > 65535)) break;
+        double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, b_mn);
+        if (cg == 1) t *= 1.04;                          // a single CTA reads 1.5 times the operands per product
+        if (splits > 1) t += 5.5 + 4e-6 * splits * (double)M * N / 4.0;
+        if (t < least) {
+          least = t;
+          best = {cg, bn, splits};
+        }
+      }
+    }
+  }
+  return best;
+}
+// The cut of a size is found once per thread and place in a small table (it takes the host some 10 us).
+static LinCut lin_cut(int M, int N, int K, bool b_mn) {
+  struct Found { int M, N, K, b_mn; LinCut cut; };
+  static thread_local Found table[64];
+  Found& f = table[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 9176u ^ (unsigned)b_mn) >> 7 & 63];
+  if (f.M != M || f.N != N || f.K != K || f.b_mn != (int)b_mn) f = Found{M, N, K, b_mn, lin_find_cut(M, N, K, b_mn)};
+  return f.cut;
+}
+
+// out [M, N] = op(A) op(B), K deep: A stored [M][K] or (a_mn) [K][M], B stored [N][K] or (b_mn) [K][N]. ws: lin_ws_floats of the same sizes.
+static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda, int64_t ldb, bool a_mn, bool b_mn, bool fwd, int act, float* ws,
+                    int64_t ws_floats, cudaStream_t stream) {
+  LinOut& o = a.out;
+  if (o.M <= 0 || o.N <= 0) return 0;
+  if (K <= 0 || (lda & 7) || (ldb & 7) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return -10;
+  const LinCut cut = lin_cut(o.M, o.N, K, b_mn);
+  if (lin_ws_floats(o.M, o.N, cut) > (ws == nullptr ? 0 : ws_floats) || sm_count() / cut.cg > kMaxWorkers) return -10;
+  LinPlan& p = a.plan;
+  p.bn = cut.bn;
+  p.splits = cut.splits;
+  p.ws = ws;
+  p.kb = (K + kLK - 1) / kLK;
+  if (p.splits > p.kb || (int64_t)((o.M + kLM * cut.cg - 1) / (kLM * cut.cg)) * p.splits > 65535) return -10;
+  lin_plan(p, o.N, (o.M + kLM * cut.cg - 1) / (kLM * cut.cg), sm_count() / cut.cg);
+  const int first = p.bn < 256 ? p.bn : 256, b_rows = first / cut.cg, b2_rows = (p.bn - first) / cut.cg;
+  auto rows = [&](int r) { return (b_mn ? (r + 63) / 64 * 64 : r) * kLK * 2; };        // column blocks of 64 where B is stored [K][N]
+  p.b2_offset = kLStageA + rows(b_rows);
+  p.stage_bytes = p.b2_offset + rows(b2_rows);
+  p.stages = (kLSmem - kLSmemFixed) / p.stage_bytes;
+  if (p.stages > kLMaxStages) p.stages = kLMaxStages;
+  CUtensorMap ta, tb, tb2;
   uint64_t dims[2], str[1] = {(uint64_t)lda * 2};
   uint32_t box[2];
-  if (!a_mn) { dims[0] = a.K; dims[1] = a.M; box[0] = kLK; box[1] = kLM; }
-  else       { dims[0] = a.M; dims[1] = a.K; box[0] = 64; box[1] = kLK; }
+  if (!a_mn) { dims[0] = K; dims[1] = o.M; box[0] = kLK; box[1] = kLM; }
+  else       { dims[0] = o.M; dims[1] = K; box[0] = 64; box[1] = kLK; }
   if (make_tmap_bf16(&ta, A, 2, dims, str, box)) return -11;
   str[0] = (uint64_t)ldb * 2;
-  if (!b_mn) { dims[0] = a.K; dims[1] = a.N; box[0] = kLK; box[1] = b_rows; }
-  else       { dims[0] = a.N; dims[1] = a.K; box[0] = 64; box[1] = kLK; }
+  if (!b_mn) { dims[0] = K; dims[1] = o.N; box[0] = kLK; box[1] = b_rows; }
+  else       { dims[0] = o.N; dims[1] = K; box[0] = 64; box[1] = kLK; }
   if (make_tmap_bf16(&tb, B, 2, dims, str, box)) return -12;
-  auto at16 = [](const void* p, int64_t ld) { return p == nullptr || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % 8 == 0); };
-  a.vec = a.N % 8 == 0 && at16(a.C, a.ldc) && at16(a.res, a.ldres) && at16(a.pre, a.ldpre) && !(reinterpret_cast<uintptr_t>(a.bias) & 15);
-#define LLMT_LIN(AM, BMN, E) \
-  if (a_mn == AM && b_mn == BMN && epi == E) \
-    return cg == 2 ? lin_launch<2, AM, BMN, E>(ta, tb, a, stream) : lin_launch<1, AM, BMN, E>(ta, tb, a, stream);
-  LLMT_LIN(false, false, true) LLMT_LIN(false, true, false) LLMT_LIN(true, true, false)
+  tb2 = tb;
+  if (!b_mn && b2_rows > 0) {
+    box[1] = b2_rows;
+    if (make_tmap_bf16(&tb2, B, 2, dims, str, box)) return -12;
+  }
+  auto at16 = [](const void* q, int64_t ld) { return q == nullptr || (!(reinterpret_cast<uintptr_t>(q) & 15) && ld % 8 == 0); };
+  o.vec = o.N % 8 == 0 && at16(o.C, o.ldc) && at16(o.res, o.ldres) && at16(o.pre, o.ldpre) && !(reinterpret_cast<uintptr_t>(o.bias) & 15);
+  const bool split = p.splits > 1;
+  if (!fwd) {
+    int rc;
+    if (a_mn) rc = split ? lin_launch<true, true, true, false, 0, false>(cut.cg, ta, tb, tb2, a, stream) : lin_launch<true, true, false, false, 0, false>(cut.cg, ta, tb, tb2, a, stream);
+    else rc = split ? lin_launch<false, true, true, false, 0, false>(cut.cg, ta, tb, tb2, a, stream) : lin_launch<false, true, false, false, 0, false>(cut.cg, ta, tb, tb2, a, stream);
+    return rc || !split ? rc : lin_join<false, 0, false>(cut.cg, a, stream);
+  }
+  if (split)
+    if (int rc = lin_launch<false, false, true, false, 0, false>(cut.cg, ta, tb, tb2, a, stream)) return rc;
+#define LLMT_LIN(ACT, RES)                                                                              \
+  if (act == ACT && (o.res != nullptr) == RES)                                                          \
+    return split ? lin_join<true, ACT, RES>(cut.cg, a, stream) : lin_launch<false, false, false, true, ACT, RES>(cut.cg, ta, tb, tb2, a, stream);
+  LLMT_LIN(0, false) LLMT_LIN(1, false) LLMT_LIN(2, false) LLMT_LIN(3, false) LLMT_LIN(4, false)
+  LLMT_LIN(0, true) LLMT_LIN(1, true) LLMT_LIN(2, true) LLMT_LIN(3, true) LLMT_LIN(4, true)
 #undef LLMT_LIN
   return -4;
 }
 
-template <int V, int THREADS>
-static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, int M, int N,
+template <int V, int THREADS, int ACT>
+static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int db_f32, int M, int N,
                      cudaStream_t stream) {
   constexpr int COLS = V == 8 ? 64 : 32;
   cudaLaunchConfig_t cfg{};
@@ -441,7 +745,7 @@ static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, in
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   using B = __nv_bfloat16;
-  return cudaLaunchKernelEx(&cfg, linear_dz_kernel<V, THREADS>, reinterpret_cast<const B*>(dy), ldy, reinterpret_cast<const B*>(z), ldz, act,
+  return cudaLaunchKernelEx(&cfg, linear_dz_kernel<V, THREADS, ACT>, reinterpret_cast<const B*>(dy), ldy, reinterpret_cast<const B*>(z), ldz,
                             reinterpret_cast<B*>(dz), lddz, db, db_f32, M, N) == cudaSuccess ? 0 : -3;
 }
 
@@ -449,43 +753,56 @@ static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, in
 
 using namespace llmt;
 
-// y [M, N] = act(x [M, K] W [N, K]^T + bias) + res; pre (optional) receives x W^T + bias.
+// Workspace of a product out [M, N] of depth K, in floats (0: none is needed). `gradient`: of llmt_linear_dx or llmt_linear_dw.
+extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int gradient) { return lin_ws_floats(M, N, lin_cut(M, N, K, gradient != 0)); }
+
+// y [M, N] = act(x [M, K] W [N, K]^T + bias) + res; pre (optional, read by llmt_linear_dz) receives x W^T + bias where there is an activation.
 extern "C" int llmt_linear_act(const void* x, const void* w, void* y, const void* bias, int bias_f32, const void* res, void* pre, int act, int M, int N,
-                               int K, int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, int* status, cudaStream_t stream) {
+                               int K, int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, float* ws, int64_t ws_floats, int* status,
+                               cudaStream_t stream) {
   if (act < 0 || act >= kActKinds) return -10;
   LinArgs a{};
-  a.M = M; a.N = N; a.K = K;
-  a.C = reinterpret_cast<__nv_bfloat16*>(y); a.ldc = ldy;
-  a.bias = bias; a.bias_f32 = bias_f32; a.act = act;
-  a.res = reinterpret_cast<const __nv_bfloat16*>(res); a.ldres = ldres;
-  a.pre = reinterpret_cast<__nv_bfloat16*>(pre); a.ldpre = ldpre;
+  LinOut& o = a.out;
+  o.M = M; o.N = N;
+  o.C = reinterpret_cast<__nv_bfloat16*>(y); o.ldc = ldy;
+  o.bias = bias; o.bias_f32 = bias_f32;
+  o.res = reinterpret_cast<const __nv_bfloat16*>(res); o.ldres = ldres;
+  o.pre = reinterpret_cast<__nv_bfloat16*>(pre); o.ldpre = ldpre;
   a.status = status;
-  return lin_gemm(x, w, a, ldx, ldw, false, false, true, stream);
+  return lin_gemm(x, w, a, K, ldx, ldw, false, false, true, act, ws, ws_floats, stream);
 }
 // dx [M, K] = dz [M, N] W [N, K]
-extern "C" int llmt_linear_dx(const void* dz, const void* w, void* dx, int M, int N, int K, int64_t lddz, int64_t ldw, int64_t lddx, int* status,
-                              cudaStream_t stream) {
+extern "C" int llmt_linear_dx(const void* dz, const void* w, void* dx, int M, int N, int K, int64_t lddz, int64_t ldw, int64_t lddx, float* ws,
+                              int64_t ws_floats, int* status, cudaStream_t stream) {
   LinArgs a{};
-  a.M = M; a.N = K; a.K = N;
-  a.C = reinterpret_cast<__nv_bfloat16*>(dx); a.ldc = lddx;
+  a.out.M = M; a.out.N = K;
+  a.out.C = reinterpret_cast<__nv_bfloat16*>(dx); a.out.ldc = lddx;
   a.status = status;
-  return lin_gemm(dz, w, a, lddz, ldw, false, true, false, stream);
+  return lin_gemm(dz, w, a, N, lddz, ldw, false, true, false, 0, ws, ws_floats, stream);
 }
 // dW [N, K] = dz [M, N]^T x [M, K]
-extern "C" int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, int N, int K, int64_t lddz, int64_t ldx, int64_t lddw, int* status,
-                              cudaStream_t stream) {
+extern "C" int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, int N, int K, int64_t lddz, int64_t ldx, int64_t lddw, float* ws,
+                              int64_t ws_floats, int* status, cudaStream_t stream) {
   LinArgs a{};
-  a.M = N; a.N = K; a.K = M;
-  a.C = reinterpret_cast<__nv_bfloat16*>(dw); a.ldc = lddw;
+  a.out.M = N; a.out.N = K;
+  a.out.C = reinterpret_cast<__nv_bfloat16*>(dw); a.out.ldc = lddw;
   a.status = status;
-  return lin_gemm(dz, x, a, lddz, ldx, true, true, false, stream);
+  return lin_gemm(dz, x, a, M, lddz, ldx, true, true, false, 0, ws, ws_floats, stream);
 }
-// dz = dy act'(z) (z nullptr: dz = dy; dz nullptr: not written), db = column sums of dz in fp32 before rounding (nullptr: not computed).
+// dz = dy act'(z) (act 0: dz = dy; dz nullptr: not written), db = column sums of dz in fp32 before rounding (nullptr: not computed).
 extern "C" int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, int M,
                               int N, cudaStream_t stream) {
-  if (M < 0 || N <= 0 || act < 0 || act >= kActKinds) return -10;
+  if (M < 0 || N <= 0 || act < 0 || act >= kActKinds || (act != 0 && z == nullptr)) return -10;
   auto at16 = [](const void* p, int64_t ld) { return p == nullptr || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % 8 == 0); };
-  const bool vec = N % 8 == 0 && at16(dy, ldy) && at16(z, ldz) && at16(dz, lddz);
-  return vec ? dz_launch<8, 512>(dy, ldy, z, ldz, act, dz, lddz, db, db_f32, M, N, stream)
-             : dz_launch<1, 512>(dy, ldy, z, ldz, act, dz, lddz, db, db_f32, M, N, stream);
+  const bool vec = N % 8 == 0 && at16(dy, ldy) && at16(act ? z : nullptr, ldz) && at16(dz, lddz);
+  // few strips of columns and many rows: larger blocks, so that an SM has enough loads in flight (16384 x 1152: 18 strips, 144 blocks)
+  const bool few = (int64_t)((N + 63) / 64) * kStripBlocks < 3 * sm_count() && M > 2048;
+#define LLMT_DZ(ACT)                                                                                              \
+  if (act == ACT)                                                                                                 \
+    return !vec ? dz_launch<1, 256, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, M, N, stream)                     \
+           : few ? dz_launch<8, 1024, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, M, N, stream)                   \
+                 : dz_launch<8, 256, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, M, N, stream);
+  LLMT_DZ(0) LLMT_DZ(1) LLMT_DZ(2) LLMT_DZ(3) LLMT_DZ(4)
+#undef LLMT_DZ
+  return -4;
 }

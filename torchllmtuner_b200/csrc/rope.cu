@@ -42,72 +42,81 @@ __device__ __forceinline__ void load_table(const float* t, int j, bool wide, flo
 }
 
 // ------------------------------------------------------------------------------------------ rotation
-// A thread owns one unit of one token and walks over the heads of a share of them, so its cos and sin are read once: a pair of vectors (half
-// layout), a vector that holds whole pairs (interleaved), or a vector that passes. Neighbouring threads own neighbouring units, then
-// neighbouring heads, so a warp touches one run of memory. V values per vector by divisibility and alignment (rope_vec); at V = 1 an
-// interleaved unit is the two halves of a pair. Bound by memory.
+// A thread owns one unit of one token in up to four heads, so its cos and sin are read once: a pair of vectors (half layout), a vector that
+// holds whole pairs (interleaved), or a vector that passes. Neighbouring threads own neighbouring units, then neighbouring heads, so a warp
+// touches one run of memory; the heads of a thread are `shares` apart and all their loads are issued before the first is used. V values per
+// vector by divisibility and alignment (rope_vec); at V = 1 an interleaved unit is the two halves of a pair. Bound by memory.
+constexpr int kRopeHeads = 4;
+struct RopeWork {
+  RopeOperand o;
+  int shares, tokens;            // threads of one token and unit; tokens of a block
+};
 template <typename T, int V, bool PAIRS>
-__global__ void __launch_bounds__(256) rope_kernel(RopeShape s, RopeOperand a, RopeOperand b, int units, int shares, int tokens_per_block) {
-  constexpr bool SCALAR_PAIRS = PAIRS && V == 1;
-  constexpr int N = PAIRS ? V / 2 : V;                  // table values of a unit
-  const int per_token = units * shares;
-  const int lt = threadIdx.x / per_token, r = threadIdx.x - lt * per_token;
-  const int64_t t = (int64_t)blockIdx.x * tokens_per_block + lt;
-  if (lt >= tokens_per_block || t >= s.T) return;
+__global__ void __launch_bounds__(256) rope_kernel(RopeShape s, RopeWork wa, RopeWork wb, int units) {
+  constexpr bool SCALAR_PAIRS = PAIRS && V == 1, TWO = !PAIRS || SCALAR_PAIRS;       // TWO: the pair's members are in two vectors
+  constexpr int N = SCALAR_PAIRS ? 1 : PAIRS ? V / 2 : V;                              // table values of a unit
+  const RopeWork& k = blockIdx.y ? wb : wa;
+  const int per_token = units * k.shares;
+  const int lt = per_token >= 256 ? 0 : threadIdx.x / per_token;
+  const int64_t t = (int64_t)blockIdx.x * k.tokens + lt;
+  if (lt >= k.tokens || t >= s.T) return;
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
-  // blocks may have fewer threads than a token has units and shares: then a thread takes several (the loop runs once otherwise)
-  for (int w = r; w < per_token; w += tokens_per_block == 1 ? blockDim.x : per_token) {
+  const int rot_units = PAIRS ? (SCALAR_PAIRS ? s.P : 2 * s.P / V) : s.P / V;
+  const int64_t x_step = k.o.x_head * k.shares, y_step = k.o.y_head * k.shares;
+  // one round unless a token has more than 256 threads' work
+  for (int w = threadIdx.x - lt * per_token; w < per_token; w += 256) {
     const int share = w / units, u = w - share * units;
-    const int rot_units = PAIRS ? (SCALAR_PAIRS ? s.P : 2 * s.P / V) : s.P / V;
     const bool rot = u < rot_units;
-    int c0, c1 = 0;                                     // columns of the unit's vector(s)
+    int c0, gap = 0;                                    // first column, distance to the partner's vector
     if (rot) {
-      c0 = PAIRS ? s.off + u * (SCALAR_PAIRS ? 2 : V) : s.off + u * V;
-      c1 = SCALAR_PAIRS ? c0 + 1 : c0 + s.P;
+      c0 = s.off + u * (SCALAR_PAIRS ? 2 : V);
+      gap = SCALAR_PAIRS ? 1 : s.P;
     } else {
       c0 = (u - rot_units) * V;
       if (c0 >= s.off) c0 += 2 * s.P;
     }
-    float c[SCALAR_PAIRS ? 1 : N > 0 ? N : 1], n[SCALAR_PAIRS ? 1 : N > 0 ? N : 1];
-    if (rot) {
-      const int j = PAIRS ? (SCALAR_PAIRS ? u : u * N) : u * V;
-      load_table<SCALAR_PAIRS ? 1 : (N > 0 ? N : 1)>(s.cosb + t * s.ldt, j, wide, c);
-      load_table<SCALAR_PAIRS ? 1 : (N > 0 ? N : 1)>(s.sinb + t * s.ldt, j, wide, n);
+    const T* px = reinterpret_cast<const T*>(k.o.x) + t * k.o.x_tok + share * k.o.x_head + c0;
+    T* py = reinterpret_cast<T*>(k.o.y) + t * k.o.y_tok + share * k.o.y_head + c0;
+    Raw<T, V> r1[kRopeHeads], r2[TWO ? kRopeHeads : 1];
 #pragma unroll
-      for (int i = 0; i < (SCALAR_PAIRS ? 1 : N > 0 ? N : 1); ++i) n[i] *= s.sign;
-    }
-    const int heads = a.H + b.H;
-#pragma unroll 4
-    for (int h = share; h < heads; h += shares) {
-      const bool first = h < a.H;
-      const int hh = first ? h : h - a.H;
-      const T* px = first ? reinterpret_cast<const T*>(a.x) + t * a.x_tok + hh * a.x_head : reinterpret_cast<const T*>(b.x) + t * b.x_tok + hh * b.x_head;
-      T* py = first ? reinterpret_cast<T*>(a.y) + t * a.y_tok + hh * a.y_head : reinterpret_cast<T*>(b.y) + t * b.y_tok + hh * b.y_head;
-      if (!rot) {
-        Raw<T, V> raw;
-        raw.load(px + c0);
-        raw.store(py + c0);
-        continue;
+    for (int i = 0; i < kRopeHeads; ++i)
+      if (share + i * k.shares < k.o.H) {
+        r1[i].load(px + i * x_step);
+        if (TWO && rot) r2[TWO ? i : 0].load(px + i * x_step + gap);
       }
+    if (!rot) {
+#pragma unroll
+      for (int i = 0; i < kRopeHeads; ++i)
+        if (share + i * k.shares < k.o.H) r1[i].store(py + i * y_step);
+      continue;
+    }
+    float c[N], n[N];
+    load_table<N>(s.cosb + t * s.ldt, u * N, wide, c);
+    load_table<N>(s.sinb + t * s.ldt, u * N, wide, n);
+#pragma unroll
+    for (int i = 0; i < N; ++i) n[i] *= s.sign;
+#pragma unroll
+    for (int i = 0; i < kRopeHeads; ++i) {
+      if (share + i * k.shares >= k.o.H) continue;
       float x1[V], y1[V];
-      load_vec<T, V>(px + c0, x1);
-      if constexpr (PAIRS && !SCALAR_PAIRS) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          y1[2 * i] = x1[2 * i] * c[i] - x1[2 * i + 1] * n[i];
-          y1[2 * i + 1] = x1[2 * i + 1] * c[i] + x1[2 * i] * n[i];
-        }
-        store_vec<T, V>(py + c0, y1);
-      } else {
+      r1[i].get(x1);
+      if constexpr (TWO) {
         float x2[V], y2[V];
-        load_vec<T, V>(px + c1, x2);
+        r2[i].get(x2);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          y1[i] = x1[i] * c[i] - x2[i] * n[i];
-          y2[i] = x2[i] * c[i] + x1[i] * n[i];
+        for (int j = 0; j < V; ++j) {
+          y1[j] = x1[j] * c[j] - x2[j] * n[j];
+          y2[j] = x2[j] * c[j] + x1[j] * n[j];
         }
-        store_vec<T, V>(py + c0, y1);
-        store_vec<T, V>(py + c1, y2);
+        store_vec<T, V>(py + i * y_step, y1);
+        store_vec<T, V>(py + i * y_step + gap, y2);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          y1[2 * j] = x1[2 * j] * c[j] - x1[2 * j + 1] * n[j];
+          y1[2 * j + 1] = x1[2 * j + 1] * c[j] + x1[2 * j] * n[j];
+        }
+        store_vec<T, V>(py + i * y_step, y1);
       }
     }
   }
@@ -134,15 +143,22 @@ static int rope_vec(const RopeShape& s, const RopeOperand& a, const RopeOperand&
 
 template <typename T, int V, bool PAIRS>
 static int rope_launch(const RopeShape& s, const RopeOperand& a, const RopeOperand& b, cudaStream_t stream) {
-  const int rot = PAIRS ? (V == 1 ? s.P : 2 * s.P / V) : s.P / V;
-  const int units = rot + (s.d - 2 * s.P) / V, heads = a.H + b.H;
-  const int shares = heads >= 16 ? heads / 4 : heads >= 2 ? (heads + 1) / 2 : 1;        // up to four heads per thread
-  const int per_token = units * shares;
-  const int tokens = per_token >= 256 ? 1 : 256 / per_token;
-  const int threads = per_token >= 256 ? 256 : tokens * per_token;
-  const int64_t blocks = ((int64_t)s.T + tokens - 1) / tokens;
+  const int units = (PAIRS ? (V == 1 ? s.P : 2 * s.P / V) : s.P / V) + (s.d - 2 * s.P) / V;
+  int64_t blocks = 0;
+  auto work = [&](const RopeOperand& o) {
+    RopeWork w{o, (o.H + kRopeHeads - 1) / kRopeHeads, 1};
+    if (o.H == 0) return w;
+    // few tokens: one head per thread, so that the machine is filled first
+    if ((int64_t)s.T * units * w.shares < (int64_t)sm_count() * 1024) w.shares = o.H;
+    if (units * w.shares < 256) w.tokens = 256 / (units * w.shares);
+    const int64_t need = ((int64_t)s.T + w.tokens - 1) / w.tokens;
+    if (need > blocks) blocks = need;
+    return w;
+  };
+  const RopeWork wa = work(a), wb = work(b);
   if (blocks > 0x7fffffff) return -10;
-  rope_kernel<T, V, PAIRS><<<(int)blocks, threads, 0, stream>>>(s, a, b, units, shares, tokens);
+  if (a.H == 0) rope_kernel<T, V, PAIRS><<<(int)blocks, 256, 0, stream>>>(s, wb, wb, units);
+  else rope_kernel<T, V, PAIRS><<<dim3((int)blocks, b.H ? 2 : 1), 256, 0, stream>>>(s, wa, wb, units);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 template <typename T>
@@ -159,9 +175,11 @@ static int rope_dispatch(const RopeShape& s, const RopeOperand& a, const RopeOpe
 // ------------------------------------------------------------------------------------------ per-head norm + rotation
 // n = x * rsqrt(mean x^2 + eps) * (w + shift) (no weight: factor 1), then the rotation. The gradient: g = rotation back of dy,
 //   dx = r (g w' - x r^2 mean(g w' x)),  dw = sum over tokens and heads of g x r;  r is computed again from x, which is read anyway.
-// Wide form: a group of G lanes per head, 8 channels per lane (16 bytes of bf16); the partner of a lane's channels is in the lane P / 8 away
-// (half layout) and comes by shuffle, or in the lane itself (interleaved). A group walks over a share of one token's heads, so tables and
-// weights are loaded once per token and operand. Needs d, off and P (interleaved: 2 P) divisible by 8, d <= 256 and 16-byte addresses.
+// Wide form: a group of G lanes per head, 8 channels per lane (16 bytes of bf16). The rotation is linear, so with the weights folded into the
+// tables a channel is r (x cw + x' nw), x' its partner: in the lane itself (interleaved), or in the lane P / 8 away (half layout), from where the
+// lane's raw 16 bytes come by shuffle. A channel that passes has cw = w, nw = 0. A group walks over a share of one token's heads, several heads
+// at a time, so tables and weights are loaded once per token and operand and several loads are in flight. Needs d, off and P (interleaved: 2 P)
+// divisible by 8, d <= 256 and 16-byte addresses. Bound by memory where there are thousands of tokens.
 // General form: a warp per head, the normalised head in shared memory, any d <= 1024.
 struct NormOperand {
   const void *x, *w;
@@ -172,61 +190,42 @@ struct NormOperand {
 };
 struct NormArgs {
   RopeShape s;
-  NormOperand q, k;
+  NormOperand q, k;              // backward: q alone
   float eps, shift;
-  float* partial;                // backward: [grid][2][d]
+  float* partial;                // backward: [grid][d]
 };
 
-template <int G>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Rotation of a lane's 8 channels: `mine` in, out in place. rot: 0 passes, 1 first half, 2 second half, 3 interleaved.
-template <int G>
-__device__ __forceinline__ void rotate_lane(float* v, int rot, int partner, const float* c, const float* n) {
-  float o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, v[i], partner, G);
-  if (rot == 3) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = v[2 * i], b = v[2 * i + 1];
-      v[2 * i] = a * c[i] - b * n[i];
-      v[2 * i + 1] = b * c[i] + a * n[i];
-    }
-  } else if (rot == 1) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] * c[i] - o[i] * n[i];
-  } else if (rot == 2) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = v[i] * c[i] + o[i] * n[i];
-  }
-}
-
-// Where lane `g` of a group stands: its kind of rotation, partner and first table column.
+// Where lane `g` of a group stands: its kind of rotation (0 passes, 1 first half, 2 second half, 3 interleaved), partner and first table column.
 struct LanePlace { int rot, partner, col; };
 __device__ __forceinline__ LanePlace lane_place(const RopeShape& s, int g) {
   const int c = g * 8;
-  LanePlace p{0, g, 0};
-  if (c < s.off || c >= s.off + 2 * s.P) return p;
+  if (c < s.off || c >= s.off + 2 * s.P) return {0, g, 0};
   if (s.interleaved) return {3, g, (c - s.off) / 2};
   const int step = s.P / 8;
   if (c < s.off + s.P) return {1, g + step, c - s.off};
   return {2, g - step, c - s.off - s.P};
 }
-__device__ __forceinline__ void lane_tables(const RopeShape& s, const LanePlace& p, int64_t t, bool wide, float* c, float* n) {
+// The factor of each of the lane's channels and of its partner, rotating forwards (sign 1) or back (-1).
+__device__ __forceinline__ void lane_tables(const RopeShape& s, const LanePlace& p, int64_t t, bool wide, float sign, float* c, float* n) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) { c[i] = 1.f; n[i] = 0.f; }
   if (p.rot == 0) return;
   if (p.rot == 3) {
-    load_table<4>(s.cosb + t * s.ldt, p.col, wide, c);
-    load_table<4>(s.sinb + t * s.ldt, p.col, wide, n);
+    float c4[4], n4[4];
+    load_table<4>(s.cosb + t * s.ldt, p.col, wide, c4);
+    load_table<4>(s.sinb + t * s.ldt, p.col, wide, n4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[2 * i] = c[2 * i + 1] = c4[i];
+      n[2 * i] = -sign * n4[i];
+      n[2 * i + 1] = sign * n4[i];
+    }
   } else {
     load_table<8>(s.cosb + t * s.ldt, p.col, wide, c);
     load_table<8>(s.sinb + t * s.ldt, p.col, wide, n);
+    const float f = p.rot == 1 ? -sign : sign;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] *= f;
   }
 }
 template <typename T>
@@ -238,8 +237,61 @@ __device__ __forceinline__ void lane_weight(const void* w, int c, int d, float s
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] += shift;
 }
+// The partners of the lane's 8 channels.
+template <typename T, int G, bool PAIRS>
+__device__ __forceinline__ void partners(const Raw<T, 8>& raw, const float* x, int partner, float* o) {
+  if constexpr (PAIRS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
+  } else {
+    Raw<T, 8> q;
+#pragma unroll
+    for (int i = 0; i < Raw<T, 8>::kWords; ++i) q.w[i] = __shfl_sync(0xffffffffu, raw.w[i], partner, G);
+    q.get(o);
+  }
+}
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 
-template <typename T, int G>
+template <typename T, int G, bool PAIRS, int HB>
+__device__ __forceinline__ void norm_heads_fwd(const NormOperand& o, const T* px, T* py, int h, int shares, bool on, const LanePlace& p, float inv_d,
+                                               float eps, const float* cw, const float* nw) {
+  Raw<T, 8> raw[HB];
+  float sq[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    raw[i].zero();
+    if (on && h + i * shares < o.H) raw[i].load(px + (int64_t)(h + i * shares) * o.x_head);
+  }
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    float x[8];
+    raw[i].get(x);
+    sq[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sq[i] += x[j] * x[j];
+  }
+#pragma unroll
+  for (int m = G / 2; m > 0; m >>= 1)
+#pragma unroll
+    for (int i = 0; i < HB; ++i) sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    float x[8], q[8];
+    raw[i].get(x);
+    partners<T, G, PAIRS>(raw[i], x, p.partner, q);
+    const float r = rsqrtf(sq[i] * inv_d + eps);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = r * (x[j] * cw[j] + q[j] * nw[j]);
+    if (on && h + i * shares < o.H) store_vec<T, 8>(py + (int64_t)(h + i * shares) * o.y_head, x);
+  }
+}
+
+template <typename T, int G, bool PAIRS>
 __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid_constant__ NormArgs a, int shares) {
   const RopeShape& s = a.s;
   constexpr int GPB = 256 / G;
@@ -249,115 +301,137 @@ __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid
   const int share = (int)(item - t * shares);
   const bool live = t < s.T;
   if (!live) t = s.T - 1;                               // the whole warp stays in the shuffles
-  const bool in = g * 8 < s.d;
+  const bool on = live && g * 8 < s.d;
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
   const LanePlace p = lane_place(s, g);
-  float c[8], n[8], w[8];
-  lane_tables(s, p, t, wide, c, n);
+  float c[8], n[8];
+  lane_tables(s, p, t, wide, 1.f, c, n);
   const float inv_d = 1.f / (float)s.d;
-#pragma unroll
+#pragma unroll 1
   for (int op = 0; op < 2; ++op) {
     const NormOperand& o = op ? a.k : a.q;
-    lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
-    const int rounds = (o.H + shares - 1) / shares;     // equal for all groups of a warp
-#pragma unroll 2
-    for (int i = 0; i < rounds; ++i) {
-      const int h = i * shares + share;
-      const bool on = in && h < o.H;
-      float x[8];
-      Raw<T, 8> raw;
-      raw.zero();
-      if (on) raw.load(reinterpret_cast<const T*>(o.x) + t * o.x_tok + h * o.x_head + g * 8);
-      raw.get(x);
-      float sq = 0.f;
+    if (o.H == 0) continue;
+    float cw[8], nw[8];
+    {
+      float w[8], wp[8];
+      lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
+      lane_weight<T>(o.w, p.partner * 8, s.d, a.shift, wp);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sq += x[j] * x[j];
-      const float r = rsqrtf(lanes_sum<G>(sq) * inv_d + a.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= r * w[j];
-      rotate_lane<G>(x, p.rot, p.partner, c, n);
-      if (on && live) store_vec<T, 8>(reinterpret_cast<T*>(o.y) + t * o.y_tok + h * o.y_head + g * 8, x);
+      for (int j = 0; j < 8; ++j) {
+        cw[j] = c[j] * w[j];
+        nw[j] = n[j] * (PAIRS ? wp[j ^ 1] : wp[j]);
+      }
     }
+    const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + g * 8;
+    T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
+    const int rounds = (o.H + shares - 1) / shares;     // equal for all groups of a warp
+    int i = 0;
+    for (; i + 4 <= rounds; i += 4) norm_heads_fwd<T, G, PAIRS, 4>(o, px, py, i * shares + share, shares, on, p, inv_d, a.eps, cw, nw);
+    if (rounds - i >= 2) {
+      norm_heads_fwd<T, G, PAIRS, 2>(o, px, py, i * shares + share, shares, on, p, inv_d, a.eps, cw, nw);
+      i += 2;
+    }
+    if (rounds > i) norm_heads_fwd<T, G, PAIRS, 1>(o, px, py, i * shares + share, shares, on, p, inv_d, a.eps, cw, nw);
   }
 }
 
-template <typename T, int G>
-__global__ void __launch_bounds__(256, 3) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares) {
+template <typename T, int G, bool PAIRS, int HB>
+__device__ __forceinline__ void norm_heads_bwd(const NormOperand& o, const T* px, const T* pd, T* py, int h, int shares, bool on, const LanePlace& p,
+                                               float inv_d, float eps, const float* c, const float* n, const float* w, float* dw) {
+  Raw<T, 8> rx[HB], rd[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    rx[i].zero();
+    rd[i].zero();
+    if (on && h + i * shares < o.H) {
+      rx[i].load(px + (int64_t)(h + i * shares) * o.x_head);
+      rd[i].load(pd + (int64_t)(h + i * shares) * o.dy_head);
+    }
+  }
+  float d[HB][8], sq[HB], dot[HB];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    float x[8], q[8];
+    rd[i].get(d[i]);
+    partners<T, G, PAIRS>(rd[i], d[i], p.partner, q);
+    rx[i].get(x);
+    sq[i] = dot[i] = 0.f;
+    float e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = d[i][j] * c[j] + q[j] * n[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      d[i][j] = e[j];
+      sq[i] += x[j] * x[j];
+      dot[i] += e[j] * w[j] * x[j];
+    }
+  }
+#pragma unroll
+  for (int m = G / 2; m > 0; m >>= 1)
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
+      dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], m);
+    }
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    if (!(on && h + i * shares < o.H)) continue;         // a dead head's r may be infinite (eps 0)
+    const float r = rsqrtf(sq[i] * inv_d + eps), k = r * r * r * dot[i] * inv_d;
+    float x[8], out[8];
+    rx[i].get(x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float dr = d[i][j] * r;
+      dw[j] += dr * x[j];
+      out[j] = dr * w[j] - x[j] * k;
+    }
+    store_vec<T, 8>(py + (int64_t)(h + i * shares) * o.y_head, out);
+  }
+}
+
+template <typename T, int G, bool PAIRS>
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares) {
   const RopeShape& s = a.s;
+  const NormOperand& o = a.q;
   constexpr int GPB = 256 / G;
-  __shared__ float sums[2][G * 8];
+  __shared__ float sums[GPB][G * 8 + 4];
   const int g = threadIdx.x % G, grp = threadIdx.x / G;
   const bool in = g * 8 < s.d;
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
   const LanePlace p = lane_place(s, g);
   const float inv_d = 1.f / (float)s.d;
-  float dw[2][8];
+  const int rounds = (o.H + shares - 1) / shares;
+  float dw[8], w[8];
+  lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dw[0][i] = dw[1][i] = 0.f;
+  for (int i = 0; i < 8; ++i) dw[i] = 0.f;
   const int64_t items = (int64_t)s.T * shares, step = (int64_t)gridDim.x * GPB;
-  const int64_t base = (int64_t)blockIdx.x * GPB;
-  for (int64_t b0 = base; b0 < items; b0 += step) {     // uniform in the block
-    const int64_t item = b0 + grp;
-    const bool live = item < items;
-    const int64_t t = (live ? item : items - 1) / shares;
-    const int share = (int)((live ? item : items - 1) - t * shares);
-    float c[8], n[8], w[8];
-    lane_tables(s, p, t, wide, c, n);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] = -n[i];
-#pragma unroll
-    for (int op = 0; op < 2; ++op) {
-      const NormOperand& o = op ? a.k : a.q;
-      lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
-      const int rounds = (o.H + shares - 1) / shares;
-#pragma unroll 2
-      for (int i = 0; i < rounds; ++i) {
-        const int h = i * shares + share;
-        const bool on = in && live && h < o.H;
-        float x[8], d[8];
-        Raw<T, 8> rx, rd;
-        rx.zero();
-        rd.zero();
-        if (on) {
-          rx.load(reinterpret_cast<const T*>(o.x) + t * o.x_tok + h * o.x_head + g * 8);
-          rd.load(reinterpret_cast<const T*>(o.dy) + t * o.dy_tok + h * o.dy_head + g * 8);
-        }
-        rx.get(x);
-        rd.get(d);
-        rotate_lane<G>(d, p.rot, p.partner, c, n);
-        float sq = 0.f, dot = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sq += x[j] * x[j];
-          dot += d[j] * w[j] * x[j];
-        }
-#pragma unroll
-        for (int m = G / 2; m > 0; m >>= 1) {
-          sq += __shfl_xor_sync(0xffffffffu, sq, m);
-          dot += __shfl_xor_sync(0xffffffffu, dot, m);
-        }
-        const float r = rsqrtf(sq * inv_d + a.eps), k = r * r * r * dot * inv_d;
-        float out[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          out[j] = r * d[j] * w[j] - x[j] * k;
-          if (on) dw[op][j] += d[j] * x[j] * r;          // a masked lane's r may be infinite (eps 0)
-        }
-        if (on) store_vec<T, 8>(reinterpret_cast<T*>(o.y) + t * o.y_tok + h * o.y_head + g * 8, out);
-      }
-    }
+  for (int64_t b0 = (int64_t)blockIdx.x * GPB; b0 < items; b0 += step) {     // uniform in the block
+    const int64_t item = b0 + grp < items ? b0 + grp : items - 1;
+    const bool on = in && b0 + grp < items;
+    const int64_t t = item / shares;
+    const int share = (int)(item - t * shares);
+    float c[8], n[8];
+    lane_tables(s, p, t, wide, -1.f, c, n);
+    const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + g * 8;
+    const T* pd = reinterpret_cast<const T*>(o.dy) + t * o.dy_tok + g * 8;
+    T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
+    int i = 0;
+    for (; i + 2 <= rounds; i += 2) norm_heads_bwd<T, G, PAIRS, 2>(o, px, pd, py, i * shares + share, shares, on, p, inv_d, a.eps, c, n, w, dw);
+    if (rounds > i) norm_heads_bwd<T, G, PAIRS, 1>(o, px, pd, py, i * shares + share, shares, on, p, inv_d, a.eps, c, n, w, dw);
   }
   if (a.partial == nullptr) return;
-  for (int k = 0; k < GPB; ++k) {                       // the groups of a block in their order
-    if (grp == k && in) {
+  if (in) {
 #pragma unroll
-      for (int op = 0; op < 2; ++op)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sums[op][g * 8 + j] = k == 0 ? dw[op][j] : sums[op][g * 8 + j] + dw[op][j];
-    }
-    __syncthreads();
+    for (int j = 0; j < 8; ++j) sums[grp][g * 8 + j] = dw[j];
   }
-  for (int i = threadIdx.x; i < 2 * s.d; i += 256) a.partial[(int64_t)blockIdx.x * 2 * s.d + i] = i < s.d ? sums[0][i] : sums[1][i - s.d];
+  __syncthreads();
+  for (int i = threadIdx.x; i < s.d; i += 256) {        // the groups of a block in their order
+    float v = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < GPB; ++k) v += sums[k][i];
+    a.partial[(int64_t)blockIdx.x * s.d + i] = v;
+  }
 }
 
 // General form. Four warps per block, each with one head at a time; buf: the head before the rotation.
@@ -377,17 +451,17 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_norm_rope_any_kernel(const 
   extern __shared__ float smem[];
   const RopeShape& s = a.s;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, d = s.d;
-  float* buf = smem + wid * (BWD ? 3 * d : d);          // BWD: dy | sums of dwq | sums of dwk
+  float* buf = smem + wid * (BWD ? 2 * d : d);          // BWD: dy | sums of dw
   if (BWD)
-    for (int c = lane; c < 2 * d; c += 32) buf[d + c] = 0.f;
+    for (int c = lane; c < d; c += 32) buf[d + c] = 0.f;
   const int heads = a.q.H + a.k.H;
   const int64_t items = (int64_t)s.T * heads;
   for (int64_t item = (int64_t)blockIdx.x * kAnyWarps + wid; item < items; item += (int64_t)gridDim.x * kAnyWarps) {
     const int64_t t = item / heads;
     int h = (int)(item - t * heads);
-    const int op = h >= a.q.H;
-    const NormOperand& o = op ? a.k : a.q;
-    if (op) h -= a.q.H;
+    const bool key = h >= a.q.H;
+    const NormOperand& o = key ? a.k : a.q;
+    if (key) h -= a.q.H;
     const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + h * o.x_head;
     T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + h * o.y_head;
     const T* pw = reinterpret_cast<const T*>(o.w);
@@ -417,7 +491,7 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_norm_rope_any_kernel(const 
         load_vec<T, 1>(px + c, &x);
         const float g = rotated(s, buf, c, t, -1.f);
         dot += g * weight(c) * x;
-        buf[d + op * d + c] += g * x * r;
+        buf[d + c] += g * x * r;
       }
       const float k = r * r * r * warp_sum(dot) / (float)d;
       for (int c = lane; c < d; c += 32) {
@@ -430,31 +504,29 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_norm_rope_any_kernel(const 
   }
   if (!BWD || a.partial == nullptr) return;
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * d; i += blockDim.x) {
+  for (int i = threadIdx.x; i < d; i += blockDim.x) {
     float v = 0.f;
-    for (int w = 0; w < kAnyWarps; ++w) v += smem[w * 3 * d + d + i];
-    a.partial[(int64_t)blockIdx.x * 2 * d + i] = v;
+    for (int w = 0; w < kAnyWarps; ++w) v += smem[w * 2 * d + d + i];
+    a.partial[(int64_t)blockIdx.x * d + i] = v;
   }
 }
 
-// dwq | dwk in T from partial [P][2 d], in a fixed order; either may be absent.
+// dw [d] in T from partial [P][d], in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* __restrict__ partial, T* __restrict__ dwq, T* __restrict__ dwk, int P, int d) {
+__global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* __restrict__ partial, T* __restrict__ dw, int P, int d) {
   __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (c < 2 * d) {
+  if (c < d) {
 #pragma unroll 4
-    for (int q = wid; q < P; q += 32) v += partial[(int64_t)q * 2 * d + c];
+    for (int q = wid; q < P; q += 32) v += partial[(int64_t)q * d + c];
   }
   part[wid][lane] = v;
   __syncthreads();
   v = warp_sum(part[lane][wid]);
   const int oc = blockIdx.x * 32 + wid;
-  if (lane != 0 || oc >= 2 * d) return;
-  T* out = oc < d ? dwq : dwk;
-  if (out != nullptr) store_vec<T, 1>(out + (oc < d ? oc : oc - d), &v);
+  if (lane == 0 && oc < d) store_vec<T, 1>(dw + oc, &v);
 }
 
 static bool norm_wide(const NormArgs& a, int size, bool bwd) {
@@ -472,28 +544,29 @@ static bool norm_wide(const NormArgs& a, int size, bool bwd) {
   }
   return true;
 }
-// Groups that share a token's heads: two to four heads per group and operand keep loads in flight without reading the tables too often.
+// Groups that share a token's heads: four heads per group (loads in flight, tables read seldom), one where there are too few tokens to fill the
+// machine that way.
+static int norm_lanes(int d) { return d > 128 ? 32 : d > 64 ? 16 : 8; }
 static int norm_shares(const NormArgs& a) {
-  const int h = a.q.H > a.k.H ? a.q.H : a.k.H;
-  return h >= 8 ? h / 4 : h >= 2 ? h / 2 : 1;
+  const int h = a.q.H > a.k.H ? a.q.H : a.k.H, few = (h + 3) / 4;
+  return (int64_t)a.s.T * few * norm_lanes(a.s.d) < (int64_t)sm_count() * 1024 ? h : few;
 }
 static int norm_bwd_grid(const NormArgs& a, bool wide) {
-  const int64_t items = wide ? (int64_t)a.s.T * norm_shares(a) : (int64_t)a.s.T * (a.q.H + a.k.H);
-  const int G = a.s.d > 128 ? 32 : a.s.d > 64 ? 16 : 8;
-  const int64_t need = wide ? (items + 256 / G - 1) / (256 / G) : (items + kAnyWarps - 1) / kAnyWarps;
-  const int64_t most = (int64_t)sm_count() * (wide ? 3 : a.s.d <= 512 ? 8 : 4);
+  const int64_t items = (int64_t)a.s.T * (wide ? norm_shares(a) : a.q.H);
+  const int per = wide ? 256 / norm_lanes(a.s.d) : kAnyWarps;
+  const int64_t need = (items + per - 1) / per, most = (int64_t)sm_count() * (wide ? 2 : 4);
   return (int)(need < most ? need : most);
 }
 
 template <typename T>
 static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
   if (norm_wide(a, sizeof(T), false)) {
-    const int G = a.s.d > 128 ? 32 : a.s.d > 64 ? 16 : 8, shares = norm_shares(a);
+    const int G = norm_lanes(a.s.d), shares = norm_shares(a);
     const int64_t blocks = ((int64_t)a.s.T * shares + 256 / G - 1) / (256 / G);
     if (blocks > 0x7fffffff) return -10;
-    if (G == 32) qk_norm_rope_part_fwd_kernel<T, 32><<<(int)blocks, 256, 0, stream>>>(a, shares);
-    else if (G == 16) qk_norm_rope_part_fwd_kernel<T, 16><<<(int)blocks, 256, 0, stream>>>(a, shares);
-    else qk_norm_rope_part_fwd_kernel<T, 8><<<(int)blocks, 256, 0, stream>>>(a, shares);
+#define LLMT_QK(L, I) if (G == L && a.s.interleaved == I) qk_norm_rope_part_fwd_kernel<T, L, I><<<(int)blocks, 256, 0, stream>>>(a, shares);
+    LLMT_QK(32, true) LLMT_QK(32, false) LLMT_QK(16, true) LLMT_QK(16, false) LLMT_QK(8, true) LLMT_QK(8, false)
+#undef LLMT_QK
   } else {
     const int64_t items = (int64_t)a.s.T * (a.q.H + a.k.H), need = (items + kAnyWarps - 1) / kAnyWarps;
     const int64_t most = (int64_t)sm_count() * 64;
@@ -502,47 +575,71 @@ static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 template <typename T>
-static int norm_bwd(const NormArgs& a, int P, void* dwq, void* dwk, cudaStream_t stream) {
+static int norm_bwd(const NormArgs& a, int P, void* dw, cudaStream_t stream) {
   const bool wide = norm_wide(a, sizeof(T), true);
   const int grid = norm_bwd_grid(a, wide);
   if (a.partial != nullptr && grid > P) return -10;
   if (wide) {
-    const int shares = norm_shares(a);
-    if (a.s.d > 128) qk_norm_rope_part_bwd_kernel<T, 32><<<grid, 256, 0, stream>>>(a, shares);
-    else if (a.s.d > 64) qk_norm_rope_part_bwd_kernel<T, 16><<<grid, 256, 0, stream>>>(a, shares);
-    else qk_norm_rope_part_bwd_kernel<T, 8><<<grid, 256, 0, stream>>>(a, shares);
+    const int G = norm_lanes(a.s.d), shares = norm_shares(a);
+#define LLMT_QK(L, I) if (G == L && a.s.interleaved == I) qk_norm_rope_part_bwd_kernel<T, L, I><<<grid, 256, 0, stream>>>(a, shares);
+    LLMT_QK(32, true) LLMT_QK(32, false) LLMT_QK(16, true) LLMT_QK(16, false) LLMT_QK(8, true) LLMT_QK(8, false)
+#undef LLMT_QK
   } else {
-    qk_norm_rope_any_kernel<T, true><<<grid, 32 * kAnyWarps, kAnyWarps * 3 * a.s.d * sizeof(float), stream>>>(a);
+    qk_norm_rope_any_kernel<T, true><<<grid, 32 * kAnyWarps, kAnyWarps * 2 * a.s.d * sizeof(float), stream>>>(a);
   }
   if (cudaGetLastError() != cudaSuccess) return -3;
-  if (a.partial != nullptr)
-    qk_weight_sum_kernel<T><<<(2 * a.s.d + 31) / 32, 1024, 0, stream>>>(a.partial, reinterpret_cast<T*>(dwq), reinterpret_cast<T*>(dwk), grid, a.s.d);
+  if (a.partial != nullptr) qk_weight_sum_kernel<T><<<(a.s.d + 31) / 32, 1024, 0, stream>>>(a.partial, reinterpret_cast<T*>(dw), grid, a.s.d);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 // ------------------------------------------------------------------------------------------ tables
-// cos, sin [T][P] of factor-scaled angles position * inv_j. The product is taken in 64 bits, in units of pi, and brought into [-1, 1] there:
-// at position 131072 an fp32 angle is off by up to 2^-8 rad. What remains is exact enough in fp32, where sincospif takes over.
+// cos, sin [T][P] of factor-scaled angles position * inv_j. The product is taken in 64 bits in quarter turns, a = position inv_j 2 / pi, and split
+// there into the nearest whole number q and the rest f in [-1/2, 1/2]: at position 131072 an fp32 angle is off by up to 2^-8 rad. Then
+// cos and sin of x = f pi / 2, |x| <= pi / 4, are Taylor sums (the terms left out are below 2^-29) and q mod 4 says which of them, with which
+// sign, is the angle's. Rounding by adding and taking away 1.5 2^52 leaves q in the low bits of the sum; double-to-integer and rounding
+// instructions, which run at a quarter of the rate, bounded the first form of this kernel (sincospif of a rounded difference: 37 us for 131072 x 64
+// against the 10 us that the writes take).
 constexpr int kMaxFreqs = 256;
-struct Freqs { double inv_pi[kMaxFreqs]; };            // inv_j / pi
+struct Freqs { double quarter[kMaxFreqs]; };           // inv_j * 2 / pi
+__device__ __forceinline__ void angle_tables(double p, double quarter, float factor, float& c, float& n) {
+  const double a = p * quarter, magic = 6755399441055744.0;                            // 1.5 * 2^52
+  const double t = a + magic;
+  const int q = __double2loint(t);
+  const float x = (float)(a - (t - magic)) * 1.57079632679489662f, z = x * x;
+  float si = 1.f / 362880.f, co = -1.f / 3628800.f;
+  si = si * z - 1.f / 5040.f;
+  si = si * z + 1.f / 120.f;
+  si = si * z - 1.f / 6.f;
+  si = si * z * x + x;
+  co = co * z + 1.f / 40320.f;
+  co = co * z - 1.f / 720.f;
+  co = co * z + 1.f / 24.f;
+  co = co * z - 0.5f;
+  co = co * z + 1.f;
+  c = (q & 1) ? si : co;
+  n = (q & 1) ? co : si;
+  c *= ((q + 1) & 2) ? -factor : factor;
+  n *= (q & 2) ? -factor : factor;
+}
+// A thread keeps the frequencies of its V columns and walks over rows.
 template <bool VEC>
 __global__ void __launch_bounds__(256) rope_tables_kernel(const int64_t* __restrict__ pos, const __grid_constant__ Freqs f, float factor,
                                                           float* __restrict__ cosb, float* __restrict__ sinb, int64_t T, int P) {
   constexpr int V = VEC ? 4 : 1;
-  const int per_row = P / V;
-  const int64_t total = T * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / per_row;
-    const int j = (int)(i - t * per_row) * V;
-    const double p = (double)pos[t];
+  const int per_row = P / V, rows = 256 / per_row;      // at most 256 columns: a row fits a block
+  const int sub = threadIdx.x / per_row, j = (threadIdx.x - sub * per_row) * V;
+  if (sub >= rows) return;
+  double quarter[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) quarter[v] = f.quarter[j + v];
+  const int64_t step = (int64_t)gridDim.x * rows;
+  int64_t t = (int64_t)blockIdx.x * rows + sub, next = t < T ? pos[t] : 0;
+  for (; t < T; t += step) {
+    const double p = (double)next;
+    if (t + step < T) next = pos[t + step];              // a row ahead
     float c[V], n[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const double a = p * f.inv_pi[j + v];
-      sincospif((float)(a - 2.0 * rint(0.5 * a)), n + v, c + v);
-      c[v] *= factor;
-      n[v] *= factor;
-    }
+    for (int v = 0; v < V; ++v) angle_tables(p, quarter[v], factor, c[v], n[v]);
     if constexpr (VEC) {
       *reinterpret_cast<float4*>(cosb + t * P + j) = make_float4(c[0], c[1], c[2], c[3]);
       *reinterpret_cast<float4*>(sinb + t * P + j) = make_float4(n[0], n[1], n[2], n[3]);
@@ -591,27 +688,28 @@ extern "C" int llmt_qk_norm_rope_part_fwd(const LlmtRopeShape* sh, const LlmtHea
   if (a.s.T == 0 || a.q.H + a.k.H == 0) return 0;
   return f32 ? norm_fwd<float>(a, stream) : norm_fwd<__nv_bfloat16>(a, stream);
 }
-// Rows of `partial` ([rows][2][d]) that the backward writes for any alignment of its operands.
-extern "C" int llmt_qk_norm_rope_part_partials(int T, int Hq, int Hk, int d) {
+// Rows of `partial` ([rows][d]) that the backward of H heads writes for any alignment of its operands.
+extern "C" int llmt_qk_norm_rope_part_partials(int T, int H, int d) {
   NormArgs a{};
-  a.s.T = T; a.s.d = d; a.q.H = Hq; a.k.H = Hk;
+  a.s.T = T; a.s.d = d; a.q.H = H;
   const int w = norm_bwd_grid(a, true), n = norm_bwd_grid(a, false);
   return w > n ? w : n;
 }
-extern "C" int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* sh, const LlmtHeads* q, const LlmtHeads* k, float eps, float shift, float* partial, int P,
-                                          void* dwq, void* dwk, int f32, cudaStream_t stream) {
-  const NormArgs a = norm_args(sh, q, k, eps, shift, partial);
-  if (!rope_shape_ok(a.s) || a.s.d > 1024 || a.s.T == 0 || a.q.H + a.k.H == 0) return -10;
-  return f32 ? norm_bwd<float>(a, P, dwq, dwk, stream) : norm_bwd<__nv_bfloat16>(a, P, dwq, dwk, stream);
+extern "C" int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* sh, const LlmtHeads* x, float eps, float shift, float* partial, int P, void* dw, int f32,
+                                          cudaStream_t stream) {
+  const NormArgs a = norm_args(sh, x, nullptr, eps, shift, partial);
+  if (!rope_shape_ok(a.s) || a.s.d > 1024 || a.s.T == 0 || a.q.H == 0) return -10;
+  return f32 ? norm_bwd<float>(a, P, dw, stream) : norm_bwd<__nv_bfloat16>(a, P, dw, stream);
 }
 
 extern "C" int llmt_rope_tables(const int64_t* pos, const double* inv, int P, double factor, float* cosb, float* sinb, int64_t T, cudaStream_t stream) {
   if (P <= 0 || P > kMaxFreqs || T < 0) return -10;
   if (T == 0) return 0;
   Freqs f{};
-  for (int j = 0; j < P; ++j) f.inv_pi[j] = inv[j] / 3.14159265358979323846;
+  for (int j = 0; j < P; ++j) f.quarter[j] = inv[j] * 2.0 / 3.14159265358979323846;
   const bool vec = P % 4 == 0 && !((reinterpret_cast<uintptr_t>(cosb) | reinterpret_cast<uintptr_t>(sinb)) & 15);
-  const int64_t need = (T * (vec ? P / 4 : P) + 255) / 256, most = (int64_t)sm_count() * 32;
+  const int rows = 256 / (vec ? P / 4 : P);
+  const int64_t need = (T + rows - 1) / rows, most = (int64_t)sm_count() * 8;
   const int grid = (int)(need < most ? need : most);
   if (vec) rope_tables_kernel<true><<<grid, 256, 0, stream>>>(pos, f, (float)factor, cosb, sinb, T, P);
   else rope_tables_kernel<false><<<grid, 256, 0, stream>>>(pos, f, (float)factor, cosb, sinb, T, P);
