@@ -516,3 +516,45 @@ def test_repeated_calls_give_the_same_bits():
     want = step()
     for _ in range(4):
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def test_refusals_name_the_argument():
+    """What the kernels cannot take is refused on the host, before a launch, with the argument's name."""
+    from torchllmtuner_b200 import ops
+    from torchllmtuner_b200.errors import ConfigError
+    x, w, b = _rand(6, 64), _rand(8, 64), _rand(8)
+    for bad in (lambda: ops.linear_act(x, _rand(8, 63)), lambda: ops.linear_act(x, w, _rand(7)), lambda: ops.linear_act(x, w, activation="tanh"),
+                lambda: ops.linear_act(x, w.cpu()), lambda: ops.linear_act(x, w, b.cpu()), lambda: ops.linear_act(x, _rand(8, 64, 1)), lambda: ops.linear_act(x, None),
+                lambda: ops.linear_act(x, w, residual=_rand(6, 8).cpu())):
+        with pytest.raises(ConfigError):
+            bad()
+    n = _rand(64)
+    for bad in (lambda: ops.layer_norm(x, n[:63], n, 1e-6), lambda: ops.layer_norm(x, n, n[:, None], 1e-6), lambda: ops.layer_norm(x, n.cpu(), n, 1e-6),
+                lambda: ops.layer_norm(x, n, None, 1e-6)):
+        with pytest.raises(ConfigError):
+            bad()
+    cos, sin = _tables(6, 8)
+    h = _rand(6, 2, 32)
+    for bad in (lambda: ops.rope(h, cos, sin, offset=17), lambda: ops.rope(h, cos, sin, offset=-1), lambda: ops.rope(h, cos[:5], sin[:5]),
+                lambda: ops.rope(h, cos, sin[:, :4]), lambda: ops.rope(h, cos, sin, layout="pairs"), lambda: ops.rope(h, cos.cpu(), sin.cpu()),
+                lambda: ops.qk_norm_rope(h, h[..., :16], None, None, cos, sin, 1e-6, norm=True),
+                lambda: ops.qk_norm_rope(h, h, n, None, cos, sin, 1e-6, norm=True), lambda: ops.qk_norm_rope(h, h.float(), None, None, cos, sin, 1e-6, norm=True),
+                lambda: ops.qk_norm_rope(h, h, None, None, cos, sin, 1e-6, norm=True, offset=17)):
+        with pytest.raises(ConfigError):
+            bad()
+    pos = torch.arange(4, device=DEV)
+    for bad in ({"rope_type": "dynamic", "factor": 2.0}, {"rope_type": "yarn", "factor": 2.0}, {"rope_type": "linear", "factor": [2.0]}):
+        with pytest.raises(ConfigError):
+            ops.rope_tables(pos, 8, 1e4, scaling=bad)
+
+
+def test_residual_broadcast_over_columns():
+    from torchllmtuner_b200 import ops
+    x, w, r = _rand(40, 64, seed=1), _rand(24, 64, seed=2, std=0.1), _rand(40, 1, seed=3).requires_grad_()
+    y = ops.linear_act(x, w, residual=r)
+    ref = x.double() @ w.double().t() + r.detach().double()
+    _near(y.detach(), ref, _u(torch.bfloat16) * ref.abs() + 80 * E32 * (x.double().abs() @ w.double().abs().t() + r.detach().double().abs()), "y")
+    dy = _rand(40, 24, seed=4)
+    g, = torch.autograd.grad(y, r, dy)
+    ref = dy.double().sum(1, keepdim=True)
+    _near(g, ref, _u(torch.bfloat16) * ref.abs() + 32 * E32 * dy.double().abs().sum(1, keepdim=True), "dr")

@@ -1,6 +1,7 @@
 // Python bindings: thin tensor -> pointer adapters over the C entry points in kernels.h. All checks that can be
 // done on the host (dtype, device, contiguity, alignment) are done here so the kernels can assume them.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -1072,6 +1073,12 @@ variable_list through_statement(const char* name, const std::vector<OptTensor>& 
     throw python_error();
   }
 }
+// An uninitialised tensor beside `like`, without the dispatcher's detour. Under torch's deterministic mode, which fills such tensors, with it.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  if (at::globalContext().deterministicFillUninitializedMemory() && at::globalContext().deterministicAlgorithms())
+    return torch::empty(sizes, like.options().dtype(type));
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
@@ -1103,8 +1110,7 @@ struct NativeLayerNorm : public torch::autograd::Function<NativeLayerNorm> {
     TORCH_CHECK(D > 0 && w.dim() == 1 && b.dim() == 1 && w.size(0) == D && b.size(0) == D, "weight and bias must have x's last size");
     Tensor xr = norm_rows(x), wc = w.contiguous(), bc = b.contiguous();
     const int R = int_of(xr.size(0), "rows");
-    Tensor y = torch::empty(x.sizes(), x.options());
-    Tensor stats = torch::empty({2, R}, x.options().dtype(at::kFloat));
+    Tensor y = fresh(x.sizes(), x.scalar_type(), x), stats = fresh({2, R}, at::kFloat, x);
     check_rc(llmt_layer_norm_fwd(xr.data_ptr(), R > 1 ? xr.stride(0) : D, wc.data_ptr(), bc.data_ptr(), y.data_ptr(), stats.data_ptr<float>(),
                                  stats.data_ptr<float>() + R, R, int_of(D, "width"), (float)eps, is_f32(x), cur_stream()),
              "llmt_layer_norm_fwd", R > 0);
@@ -1127,11 +1133,11 @@ struct NativeLayerNorm : public torch::autograd::Function<NativeLayerNorm> {
     Tensor dy = d[0].to(x.scalar_type());
     if (!dy.is_contiguous() || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone(at::MemoryFormat::Contiguous);
     const int R = (int)xr.size(0);
-    Tensor dx = torch::empty(x.sizes(), x.options());
+    Tensor dx = fresh(x.sizes(), x.scalar_type(), x);
     if (R == 0) return {dx, torch::zeros_like(w), torch::zeros_like(b), Tensor()};
-    Tensor dw = torch::empty({D}, w.options()), db = torch::empty({D}, b.options());
+    Tensor dw = fresh({D}, w.scalar_type(), x), db = fresh({D}, b.scalar_type(), x);
     const int P = llmt_layer_norm_bwd_partials(R, (int)D, is_f32(x));
-    Tensor part = torch::empty({P, 2, D}, stats.options());
+    Tensor part = fresh({P, 2, D}, at::kFloat, x);
     check_rc(llmt_layer_norm_bwd(dy.data_ptr(), xr.data_ptr(), R > 1 ? xr.stride(0) : D, wc.data_ptr(), stats.data_ptr<float>(),
                                  stats.data_ptr<float>() + R, dx.data_ptr(), part.data_ptr<float>(), P, dw.data_ptr(), db.data_ptr(), R, (int)D,
                                  is_f32(x), cur_stream()),
@@ -1182,13 +1188,13 @@ std::vector<Tensor> rope_run(const Tensor& a, const OptTensor& b, Tensor cosb, T
   c10::cuda::CUDAGuard guard(a.device());
   check_rotary(a, cosb, sinb, c, "x");
   same_tables(cosb, sinb);
-  Tensor xa = unit_inner(a), ya = torch::empty(a.sizes(), a.options()), xb, yb;
+  Tensor xa = unit_inner(a), ya = fresh(a.sizes(), a.scalar_type(), a), xb, yb;
   LlmtHeads ha = heads_of(xa, ya), hb{};
   if (b.has_value()) {
     check_rotary(*b, cosb, sinb, c, "k");
     TORCH_CHECK(b->scalar_type() == a.scalar_type() && b->size(2) == a.size(2), "both operands must have one type and head width");
     xb = unit_inner(*b);
-    yb = torch::empty(b->sizes(), b->options());
+    yb = fresh(b->sizes(), b->scalar_type(), a);
     hb = heads_of(xb, yb);
   }
   const LlmtRopeShape s = rope_shape(a, cosb, sinb, c, sign);
@@ -1270,8 +1276,8 @@ struct NativeHeadNormRope : public torch::autograd::Function<NativeHeadNormRope>
     c10::cuda::CUDAGuard guard(x.device());
     same_tables(cosb, sinb);
     const bool need_w = w.defined() && ctx->needs_input_grad(1);
-    Tensor xi = unit_inner(x), dy = unit_inner(d[0]), dx = torch::empty(x.sizes(), x.options()), dw, part;
-    if (need_w) dw = x.numel() > 0 ? torch::empty(w.sizes(), w.options()) : torch::zeros(w.sizes(), w.options());
+    Tensor xi = unit_inner(x), dy = unit_inner(d[0]), dx = fresh(x.sizes(), x.scalar_type(), x), dw, part;
+    if (need_w) dw = x.numel() > 0 ? fresh(w.sizes(), w.scalar_type(), x) : torch::zeros(w.sizes(), w.options());
     out[0] = dx;
     out[1] = dw;
     if (x.numel() == 0) return out;
@@ -1282,7 +1288,7 @@ struct NativeHeadNormRope : public torch::autograd::Function<NativeHeadNormRope>
     int P = 0;
     if (need_w) {
       P = llmt_qk_norm_rope_part_partials((int)x.size(0), h.H, (int)x.size(2));
-      part = torch::empty({P, x.size(2)}, x.options().dtype(at::kFloat));
+      part = fresh({P, x.size(2)}, at::kFloat, x);
     }
     const LlmtRopeShape rs = rope_shape(x, cosb, sinb, c, 1.f);
     check_rc(llmt_qk_norm_rope_part_bwd(&rs, &h, (float)eps, (float)shift, need_w ? part.data_ptr<float>() : nullptr, P,
@@ -1307,8 +1313,8 @@ variable_list qk_norm_rope_part_node(const Tensor& q, const Tensor& k, const Opt
     Tensor cosb = cosb0, sinb = sinb0;
     same_tables(cosb, sinb);
     Tensor xq = unit_inner(q), xk = unit_inner(k), wq = qw.has_value() ? qw->contiguous() : Tensor(), wk = kw.has_value() ? kw->contiguous() : Tensor();
-    yq = torch::empty(q.sizes(), q.options());
-    yk = torch::empty(k.sizes(), k.options());
+    yq = fresh(q.sizes(), q.scalar_type(), q);
+    yk = fresh(k.sizes(), k.scalar_type(), q);
     LlmtHeads hq = heads_of(xq, yq), hk = heads_of(xk, yk);
     hq.w = wq.defined() ? wq.data_ptr() : nullptr;
     hk.w = wk.defined() ? wk.data_ptr() : nullptr;
@@ -1319,14 +1325,15 @@ variable_list qk_norm_rope_part_node(const Tensor& q, const Tensor& k, const Opt
           NativeHeadNormRope::apply(k, kw, cosb0, sinb0, off, interleaved, eps, shift, Computed{yk})};
 }
 
-std::vector<Tensor> rope_tables(const Tensor& positions, const std::vector<double>& inv, double factor) {
+// inv: the frequencies, 64 bits on the host.
+std::vector<Tensor> rope_tables(const Tensor& positions, const Tensor& inv, double factor) {
   c10::cuda::CUDAGuard guard(positions.device());
   TORCH_CHECK(positions.is_cuda() && positions.scalar_type() == at::kLong && positions.dim() == 1, "positions must be int64 [T] on the device");
+  TORCH_CHECK(inv.is_cpu() && inv.scalar_type() == at::kDouble && inv.dim() == 1 && inv.is_contiguous(), "frequencies must be float64 on the host");
   const Tensor p = positions.contiguous();
-  const int64_t P = (int64_t)inv.size();
-  auto o = positions.options().dtype(at::kFloat);
-  Tensor cosb = torch::empty({p.size(0), P}, o), sinb = torch::empty({p.size(0), P}, o);
-  check_rc(llmt_rope_tables(p.data_ptr<int64_t>(), inv.data(), int_of(P, "frequencies"), factor, cosb.data_ptr<float>(), sinb.data_ptr<float>(),
+  const int64_t P = inv.size(0);
+  Tensor cosb = fresh({p.size(0), P}, at::kFloat, p), sinb = fresh({p.size(0), P}, at::kFloat, p);
+  check_rc(llmt_rope_tables(p.data_ptr<int64_t>(), inv.data_ptr<double>(), int_of(P, "frequencies"), factor, cosb.data_ptr<float>(), sinb.data_ptr<float>(),
                             p.size(0), cur_stream()),
            "llmt_rope_tables", p.size(0) > 0);
   return {cosb, sinb};
@@ -1344,7 +1351,7 @@ Tensor tma_rows(const Tensor& t) {
 // Partial sums of a product that is cut along its depth; of this call alone, so graphs and streams share nothing.
 Tensor linear_workspace(int64_t M, int64_t N, int64_t K, bool gradient, const Tensor& like) {
   const int64_t n = llmt_linear_ws_floats((int)M, (int)N, (int)K, gradient);
-  return n > 0 ? torch::empty({n}, like.options().dtype(at::kFloat)) : Tensor();
+  return n > 0 ? fresh({n}, at::kFloat, like) : Tensor();
 }
 inline float* ws_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 inline int64_t ws_size(const Tensor& t) { return t.defined() ? t.numel() : 0; }
@@ -1357,7 +1364,9 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     const int64_t N = w.size(0), K = w.size(1);
     Tensor x2 = tma_rows(rows_2d(x)), w2 = tma_rows(w.stride(1) == 1 ? w : w.contiguous());
     const int64_t M = x2.size(0);
-    Tensor y = like_rows(x, N), bc, r2, pre;
+    auto ysizes = x.sizes().vec();
+    ysizes.back() = N;
+    Tensor y = fresh(ysizes, at::kBFloat16, x), bc, r2, pre;
     if (b.has_value()) {
       TORCH_CHECK(b->device() == x.device() && (b->scalar_type() == at::kBFloat16 || is_f32(*b)) && b->dim() == 1 && b->size(0) == N,
                   "bias must be [N], bfloat16 or float32");
@@ -1369,7 +1378,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
       r2 = rows_2d(*r);
       if (M > 1 && r2.stride(0) < N && r2.stride(0) != 0) r2 = r2.contiguous();
     }
-    if (act != 0 && keep) pre = torch::empty({M, (N + 7) / 8 * 8}, x.options());
+    if (act != 0 && keep) pre = fresh({M, (N + 7) / 8 * 8}, at::kBFloat16, x);
     const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), false, x);
     check_rc(llmt_linear_act(x2.data_ptr(), w2.data_ptr(), y.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, bc.defined() && is_f32(bc),
                              r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, (int)M,
@@ -1414,9 +1423,9 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
     const bool tma_ok = dy.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
     const bool write = (nx || nw) && (act != 0 || !tma_ok);
-    Tensor dz = write ? torch::empty({M, (N + 7) / 8 * 8}, dy.options()).narrow(1, 0, N) : dy;
+    Tensor dz = write ? fresh({M, (N + 7) / 8 * 8}, at::kBFloat16, x) : dy;
     if (write || nb) {
-      if (nb) out[2] = torch::empty(b.sizes(), b.options());
+      if (nb) out[2] = fresh(b.sizes(), b.scalar_type(), x);
       check_rc(llmt_linear_dz(dy.data_ptr(), M > 1 ? dy.stride(0) : (N + 7) / 8 * 8, act != 0 ? pre.data_ptr() : nullptr, act != 0 ? pre.stride(0) : 0,
                               (int)act, write ? dz.data_ptr() : nullptr, write ? dz.stride(0) : 0, nb ? out[2].data_ptr() : nullptr,
                               nb && is_f32(b), (int)M, (int)N, cur_stream()),
@@ -1427,7 +1436,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
       py::gil_scoped_acquire gil;
       try {
         py::object fn = py::reinterpret_borrow<py::object>(py_hooks().linears_backward);
-        auto r = fn(x2, variable_list{w}, variable_list{dz}, nx, std::vector<bool>{nw}).cast<std::vector<OptTensor>>();
+        auto r = fn(x2, variable_list{w}, variable_list{dz.narrow(1, 0, N)}, nx, std::vector<bool>{nw}).cast<std::vector<OptTensor>>();
         if (r[0].has_value()) out[0] = r[0]->reshape(x.sizes());
         if (r[1].has_value()) out[1] = *r[1];
         return out;
@@ -1438,14 +1447,14 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     }
     const int64_t lddz = dz.stride(0);
     if (nx) {
-      out[0] = torch::empty(x.sizes(), x.options());
+      out[0] = fresh(x.sizes(), at::kBFloat16, x);
       const Tensor ws = linear_workspace(M, K, N, true, dz);
       check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),
                "llmt_linear_dx", ws.defined() ? 2 : 1);
     }
     if (nw) {
-      out[1] = torch::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
+      out[1] = fresh(w.sizes(), at::kBFloat16, x);
       const Tensor ws = linear_workspace(N, K, M, true, dz);
       check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),

@@ -177,9 +177,8 @@ static int rope_dispatch(const RopeShape& s, const RopeOperand& a, const RopeOpe
 //   dx = r (g w' - x r^2 mean(g w' x)),  dw = sum over tokens and heads of g x r;  r is computed again from x, which is read anyway.
 // Wide form: a group of G lanes per head, 8 channels per lane (16 bytes of bf16). The rotation is linear, so with the weights folded into the
 // tables a channel is r (x cw + x' nw), x' its partner: in the lane itself (interleaved), or in the lane P / 8 away (half layout), from where the
-// lane's raw 16 bytes come by shuffle. A channel that passes has cw = w, nw = 0. A group walks over a share of one token's heads, several heads
-// at a time, so tables and weights are loaded once per token and operand and several loads are in flight. Needs d, off and P (interleaved: 2 P)
-// divisible by 8, d <= 256 and 16-byte addresses. Bound by memory where there are thousands of tokens.
+// lane's raw 16 bytes come by shuffle. A channel that passes has cw = w, nw = 0. A group takes several heads of one token, so tables and weights are
+// loaded once for them and several loads are in flight. Needs d, off and P (interleaved: 2 P) divisible by 8, d <= 256 and 16-byte addresses. Bound by memory where there are thousands of tokens.
 // General form: a warp per head, the normalised head in shared memory, any d <= 1024.
 struct NormOperand {
   const void *x, *w;
@@ -250,23 +249,43 @@ __device__ __forceinline__ void partners(const Raw<T, 8>& raw, const float* x, i
     q.get(o);
   }
 }
-template <int G>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
+// A group takes HB heads of one token, `shares` apart; their loads are issued before the tables' and weights', so a warp waits for memory once.
+// blockIdx.y: queries or keys.
 template <typename T, int G, bool PAIRS, int HB>
-__device__ __forceinline__ void norm_heads_fwd(const NormOperand& o, const T* px, T* py, int h, int shares, bool on, const LanePlace& p, float inv_d,
-                                               float eps, const float* cw, const float* nw) {
+__global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid_constant__ NormArgs a, int q_shares, int k_shares) {
+  const RopeShape& s = a.s;
+  const NormOperand& o = blockIdx.y ? a.k : a.q;
+  const unsigned shares = blockIdx.y ? k_shares : q_shares;
+  constexpr int GPB = 256 / G;
+  const int g = threadIdx.x % G;
+  const unsigned item = blockIdx.x * GPB + threadIdx.x / G;
+  const unsigned token = item / shares;
+  const int share = (int)(item - token * shares);
+  const bool live = token < (unsigned)s.T, on = live && g * 8 < s.d;
+  const int64_t t = live ? token : s.T - 1;             // the whole warp stays in the shuffles
+  const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + g * 8;
   Raw<T, 8> raw[HB];
-  float sq[HB];
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
     raw[i].zero();
-    if (on && h + i * shares < o.H) raw[i].load(px + (int64_t)(h + i * shares) * o.x_head);
+    if (on && share + i * (int)shares < o.H) raw[i].load(px + (int64_t)(share + i * (int)shares) * o.x_head);
   }
+  const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
+  const LanePlace p = lane_place(s, g);
+  float cw[8], nw[8];
+  {
+    float w[8], wp[8];
+    lane_tables(s, p, t, wide, 1.f, cw, nw);
+    lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
+    lane_weight<T>(o.w, p.partner * 8, s.d, a.shift, wp);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cw[j] *= w[j];
+      nw[j] *= PAIRS ? wp[j ^ 1] : wp[j];
+    }
+  }
+  const float inv_d = 1.f / (float)s.d;
+  float sq[HB];
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
     float x[8];
@@ -279,146 +298,108 @@ __device__ __forceinline__ void norm_heads_fwd(const NormOperand& o, const T* px
   for (int m = G / 2; m > 0; m >>= 1)
 #pragma unroll
     for (int i = 0; i < HB; ++i) sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
+  T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
     float x[8], q[8];
     raw[i].get(x);
     partners<T, G, PAIRS>(raw[i], x, p.partner, q);
-    const float r = rsqrtf(sq[i] * inv_d + eps);
+    const float r = rsqrtf(sq[i] * inv_d + a.eps);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = r * (x[j] * cw[j] + q[j] * nw[j]);
-    if (on && h + i * shares < o.H) store_vec<T, 8>(py + (int64_t)(h + i * shares) * o.y_head, x);
+    if (on && share + i * (int)shares < o.H) store_vec<T, 8>(py + (int64_t)(share + i * (int)shares) * o.y_head, x);
   }
 }
 
-template <typename T, int G, bool PAIRS>
-__global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid_constant__ NormArgs a, int shares) {
-  const RopeShape& s = a.s;
-  constexpr int GPB = 256 / G;
-  const int g = threadIdx.x % G;
-  const int64_t item = (int64_t)blockIdx.x * GPB + threadIdx.x / G;
-  int64_t t = item / shares;
-  const int share = (int)(item - t * shares);
-  const bool live = t < s.T;
-  if (!live) t = s.T - 1;                               // the whole warp stays in the shuffles
-  const bool on = live && g * 8 < s.d;
-  const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
-  const LanePlace p = lane_place(s, g);
-  float c[8], n[8];
-  lane_tables(s, p, t, wide, 1.f, c, n);
-  const float inv_d = 1.f / (float)s.d;
-#pragma unroll 1
-  for (int op = 0; op < 2; ++op) {
-    const NormOperand& o = op ? a.k : a.q;
-    if (o.H == 0) continue;
-    float cw[8], nw[8];
-    {
-      float w[8], wp[8];
-      lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
-      lane_weight<T>(o.w, p.partner * 8, s.d, a.shift, wp);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cw[j] = c[j] * w[j];
-        nw[j] = n[j] * (PAIRS ? wp[j ^ 1] : wp[j]);
-      }
-    }
-    const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + g * 8;
-    T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
-    const int rounds = (o.H + shares - 1) / shares;     // equal for all groups of a warp
-    int i = 0;
-    for (; i + 4 <= rounds; i += 4) norm_heads_fwd<T, G, PAIRS, 4>(o, px, py, i * shares + share, shares, on, p, inv_d, a.eps, cw, nw);
-    if (rounds - i >= 2) {
-      norm_heads_fwd<T, G, PAIRS, 2>(o, px, py, i * shares + share, shares, on, p, inv_d, a.eps, cw, nw);
-      i += 2;
-    }
-    if (rounds > i) norm_heads_fwd<T, G, PAIRS, 1>(o, px, py, i * shares + share, shares, on, p, inv_d, a.eps, cw, nw);
-  }
-}
-
+// The same split for the gradient; a group walks over items (token, share) and holds its sums of the weight's gradient. The operands of the next
+// item are fetched before this one's sums are taken.
 template <typename T, int G, bool PAIRS, int HB>
-__device__ __forceinline__ void norm_heads_bwd(const NormOperand& o, const T* px, const T* pd, T* py, int h, int shares, bool on, const LanePlace& p,
-                                               float inv_d, float eps, const float* c, const float* n, const float* w, float* dw) {
-  Raw<T, 8> rx[HB], rd[HB];
-#pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    rx[i].zero();
-    rd[i].zero();
-    if (on && h + i * shares < o.H) {
-      rx[i].load(px + (int64_t)(h + i * shares) * o.x_head);
-      rd[i].load(pd + (int64_t)(h + i * shares) * o.dy_head);
-    }
-  }
-  float d[HB][8], sq[HB], dot[HB];
-#pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    float x[8], q[8];
-    rd[i].get(d[i]);
-    partners<T, G, PAIRS>(rd[i], d[i], p.partner, q);
-    rx[i].get(x);
-    sq[i] = dot[i] = 0.f;
-    float e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = d[i][j] * c[j] + q[j] * n[j];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      d[i][j] = e[j];
-      sq[i] += x[j] * x[j];
-      dot[i] += e[j] * w[j] * x[j];
-    }
-  }
-#pragma unroll
-  for (int m = G / 2; m > 0; m >>= 1)
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
-      dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], m);
-    }
-#pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    if (!(on && h + i * shares < o.H)) continue;         // a dead head's r may be infinite (eps 0)
-    const float r = rsqrtf(sq[i] * inv_d + eps), k = r * r * r * dot[i] * inv_d;
-    float x[8], out[8];
-    rx[i].get(x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float dr = d[i][j] * r;
-      dw[j] += dr * x[j];
-      out[j] = dr * w[j] - x[j] * k;
-    }
-    store_vec<T, 8>(py + (int64_t)(h + i * shares) * o.y_head, out);
-  }
-}
-
-template <typename T, int G, bool PAIRS>
-__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares) {
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares_) {
   const RopeShape& s = a.s;
   const NormOperand& o = a.q;
   constexpr int GPB = 256 / G;
   __shared__ float sums[GPB][G * 8 + 4];
+  const unsigned shares = shares_, items = (unsigned)s.T * shares, step = gridDim.x * GPB;
   const int g = threadIdx.x % G, grp = threadIdx.x / G;
   const bool in = g * 8 < s.d;
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
   const LanePlace p = lane_place(s, g);
   const float inv_d = 1.f / (float)s.d;
-  const int rounds = (o.H + shares - 1) / shares;
   float dw[8], w[8];
-  lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i] = 0.f;
-  const int64_t items = (int64_t)s.T * shares, step = (int64_t)gridDim.x * GPB;
-  for (int64_t b0 = (int64_t)blockIdx.x * GPB; b0 < items; b0 += step) {     // uniform in the block
-    const int64_t item = b0 + grp < items ? b0 + grp : items - 1;
-    const bool on = in && b0 + grp < items;
-    const int64_t t = item / shares;
-    const int share = (int)(item - t * shares);
+  Raw<T, 8> rx[HB], rd[HB];
+  int64_t t;
+  int share;
+  auto fetch = [&](unsigned item, int64_t& tok, int& sh, Raw<T, 8>* x, Raw<T, 8>* d) {
+    const unsigned it = item < items ? item : items - 1;
+    tok = it / shares;
+    sh = (int)(it - (unsigned)tok * shares);
+    const T* px = reinterpret_cast<const T*>(o.x) + tok * o.x_tok + g * 8;
+    const T* pd = reinterpret_cast<const T*>(o.dy) + tok * o.dy_tok + g * 8;
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      x[i].zero();
+      d[i].zero();
+      if (in && item < items && sh + i * shares_ < o.H) {
+        x[i].load(px + (int64_t)(sh + i * shares_) * o.x_head);
+        d[i].load(pd + (int64_t)(sh + i * shares_) * o.dy_head);
+      }
+    }
+  };
+  unsigned b0 = blockIdx.x * GPB;
+  fetch(b0 + grp, t, share, rx, rd);
+  lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
+  for (; b0 < items; b0 += step) {                      // uniform in the block; items + step fits 32 bits
+    const bool live = in && b0 + grp < items;
     float c[8], n[8];
     lane_tables(s, p, t, wide, -1.f, c, n);
-    const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + g * 8;
-    const T* pd = reinterpret_cast<const T*>(o.dy) + t * o.dy_tok + g * 8;
+    Raw<T, 8> nx[HB], nd[HB];
+    int64_t nt = t;
+    int nshare = share;
+    if (b0 + step < items) fetch(b0 + step + grp, nt, nshare, nx, nd);
+    float d[HB][8], sq[HB], dot[HB];
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      float x[8], q[8], e[8];
+      rd[i].get(e);
+      partners<T, G, PAIRS>(rd[i], e, p.partner, q);
+      rx[i].get(x);
+      sq[i] = dot[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        d[i][j] = e[j] * c[j] + q[j] * n[j];
+        sq[i] += x[j] * x[j];
+        dot[i] += d[i][j] * w[j] * x[j];
+      }
+    }
+#pragma unroll
+    for (int m = G / 2; m > 0; m >>= 1)
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
+        dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], m);
+      }
     T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
-    int i = 0;
-    for (; i + 2 <= rounds; i += 2) norm_heads_bwd<T, G, PAIRS, 2>(o, px, pd, py, i * shares + share, shares, on, p, inv_d, a.eps, c, n, w, dw);
-    if (rounds > i) norm_heads_bwd<T, G, PAIRS, 1>(o, px, pd, py, i * shares + share, shares, on, p, inv_d, a.eps, c, n, w, dw);
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+      if (live && share + i * shares_ < o.H) {           // a dead head's r may be infinite (eps 0)
+        const float r = rsqrtf(sq[i] * inv_d + a.eps), k = r * r * r * dot[i] * inv_d;
+        float x[8], out[8];
+        rx[i].get(x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float dr = d[i][j] * r;
+          dw[j] += dr * x[j];
+          out[j] = dr * w[j] - x[j] * k;
+        }
+        store_vec<T, 8>(py + (int64_t)(share + i * shares_) * o.y_head, out);
+      }
+      rx[i] = nx[i];
+      rd[i] = nd[i];
+    }
+    t = nt;
+    share = nshare;
   }
   if (a.partial == nullptr) return;
   if (in) {
@@ -544,15 +525,18 @@ static bool norm_wide(const NormArgs& a, int size, bool bwd) {
   }
   return true;
 }
-// Groups that share a token's heads: four heads per group (loads in flight, tables read seldom), one where there are too few tokens to fill the
-// machine that way.
+// Heads per group: loads in flight and tables read seldom, or one where there are too few tokens to fill the machine that way. Forward up to four,
+// backward two (registers).
 static int norm_lanes(int d) { return d > 128 ? 32 : d > 64 ? 16 : 8; }
-static int norm_shares(const NormArgs& a) {
-  const int h = a.q.H > a.k.H ? a.q.H : a.k.H, few = (h + 3) / 4;
-  return (int64_t)a.s.T * few * norm_lanes(a.s.d) < (int64_t)sm_count() * 1024 ? h : few;
+static int norm_heads(const NormArgs& a, int H, int most) {
+  int n = H < most ? H : most;
+  if (n == 3) n = 4;
+  while (n > 1 && (int64_t)a.s.T * ((H + n - 1) / n) * norm_lanes(a.s.d) < (int64_t)sm_count() * 1024) n /= 2;
+  return n > 1 ? n : 1;
 }
 static int norm_bwd_grid(const NormArgs& a, bool wide) {
-  const int64_t items = (int64_t)a.s.T * (wide ? norm_shares(a) : a.q.H);
+  const int n = norm_heads(a, a.q.H, 2);
+  const int64_t items = (int64_t)a.s.T * (wide ? (a.q.H + n - 1) / n : a.q.H);
   const int per = wide ? 256 / norm_lanes(a.s.d) : kAnyWarps;
   const int64_t need = (items + per - 1) / per, most = (int64_t)sm_count() * (wide ? 2 : 4);
   return (int)(need < most ? need : most);
@@ -561,11 +545,20 @@ static int norm_bwd_grid(const NormArgs& a, bool wide) {
 template <typename T>
 static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
   if (norm_wide(a, sizeof(T), false)) {
-    const int G = norm_lanes(a.s.d), shares = norm_shares(a);
-    const int64_t blocks = ((int64_t)a.s.T * shares + 256 / G - 1) / (256 / G);
-    if (blocks > 0x7fffffff) return -10;
-#define LLMT_QK(L, I) if (G == L && a.s.interleaved == I) qk_norm_rope_part_fwd_kernel<T, L, I><<<(int)blocks, 256, 0, stream>>>(a, shares);
-    LLMT_QK(32, true) LLMT_QK(32, false) LLMT_QK(16, true) LLMT_QK(16, false) LLMT_QK(8, true) LLMT_QK(8, false)
+    const int G = norm_lanes(a.s.d), H = a.q.H > a.k.H ? a.q.H : a.k.H, n = norm_heads(a, H, 4);
+    const int qs = a.q.H ? (a.q.H + n - 1) / n : 1, ks = a.k.H ? (a.k.H + n - 1) / n : 1;
+    const int64_t items = (int64_t)a.s.T * (qs > ks ? qs : ks);
+    if (items > 0x7fffff00) return -10;
+    // without queries the keys take their place
+    NormArgs b = a;
+    if (a.q.H == 0) { b.q = a.k; b.k.H = 0; }
+    const dim3 grid((unsigned)((items + 256 / G - 1) / (256 / G)), b.k.H ? 2 : 1);
+    const int s0 = a.q.H ? qs : ks;
+#define LLMT_QK(L, I, N) \
+  if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_fwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(b, s0, ks);
+#define LLMT_QK3(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2) LLMT_QK(L, I, 4)
+    LLMT_QK3(32, true) LLMT_QK3(32, false) LLMT_QK3(16, true) LLMT_QK3(16, false) LLMT_QK3(8, true) LLMT_QK3(8, false)
+#undef LLMT_QK3
 #undef LLMT_QK
   } else {
     const int64_t items = (int64_t)a.s.T * (a.q.H + a.k.H), need = (items + kAnyWarps - 1) / kAnyWarps;
@@ -580,9 +573,13 @@ static int norm_bwd(const NormArgs& a, int P, void* dw, cudaStream_t stream) {
   const int grid = norm_bwd_grid(a, wide);
   if (a.partial != nullptr && grid > P) return -10;
   if (wide) {
-    const int G = norm_lanes(a.s.d), shares = norm_shares(a);
-#define LLMT_QK(L, I) if (G == L && a.s.interleaved == I) qk_norm_rope_part_bwd_kernel<T, L, I><<<grid, 256, 0, stream>>>(a, shares);
-    LLMT_QK(32, true) LLMT_QK(32, false) LLMT_QK(16, true) LLMT_QK(16, false) LLMT_QK(8, true) LLMT_QK(8, false)
+    const int G = norm_lanes(a.s.d), n = norm_heads(a, a.q.H, 2), shares = (a.q.H + n - 1) / n;
+    if ((int64_t)a.s.T * shares > 0x7fffff00) return -10;
+#define LLMT_QK(L, I, N) \
+  if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_bwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(a, shares);
+#define LLMT_QK2(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2)
+    LLMT_QK2(32, true) LLMT_QK2(32, false) LLMT_QK2(16, true) LLMT_QK2(16, false) LLMT_QK2(8, true) LLMT_QK2(8, false)
+#undef LLMT_QK2
 #undef LLMT_QK
   } else {
     qk_norm_rope_any_kernel<T, true><<<grid, 32 * kAnyWarps, kAnyWarps * 2 * a.s.d * sizeof(float), stream>>>(a);

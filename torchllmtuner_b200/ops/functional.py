@@ -308,16 +308,22 @@ def linear_act(x, w, bias=None, *, activation: str | None = None, residual=None)
     """act(x W^T + bias) + residual with everything behind the product in its epilogue: x [..., K], w [N, K], bias [N], residual broadcastable to
     [..., N]; activation None, "gelu" (erf), "gelu_tanh", "silu" or "relu". bf16 on the device, any widths and strides. Elsewhere (other types,
     per-op checkpointing and pending peer-memory collectives, which are kept per product, transforms and tracing) the same as tensor expressions."""
-    validate_linear_act_inputs(x, w, bias, activation, residual, _ACTIVATION_CODES)
-    given = [t for t in (x, w, bias, residual) if t is not None]
-    if (_SAC is None and _use_cuda(x) and x.dtype == w.dtype == torch.bfloat16 and x.numel() and w.numel()
-            and (bias is None or bias.dtype in _ROW_TYPES) and (residual is None or residual.dtype == x.dtype) and _has_rules(*given)):
-        shape = (*x.shape[:-1], w.shape[0])
-        if residual is None or torch.broadcast_shapes(residual.shape, shape) == shape:
+    try:
+        if (x.is_cuda and _SAC is None and x.dtype == w.dtype == torch.bfloat16 and x.numel() and w.numel() and (bias is None or bias.dtype in _ROW_TYPES)
+                and (residual is None or residual.dtype == x.dtype) and _has_rules(*(t for t in (x, w, bias, residual) if t is not None))):
             ext = _native()
+            if residual is not None and (residual.dim() != x.dim() or residual.shape[-1] != w.shape[0] or residual.shape[:-1] != x.shape[:-1]):
+                shape = (*x.shape[:-1], w.shape[0])
+                if torch.broadcast_shapes(residual.shape, shape) != shape:
+                    ext = None                             # the residual is the larger one
+                else:
+                    residual = residual.expand(shape)
             if ext is not None:
-                return ext.linear_act_node(x, w, bias, residual if residual is None or residual.shape == shape else residual.expand(shape),
-                                           _ACTIVATION_CODES[activation])
+                return ext.linear_act_node(x, w, bias, residual, _ACTIVATION_CODES[activation])
+    except (*_REFUSED, KeyError, IndexError):
+        validate_linear_act_inputs(x, w, bias, activation, residual, _ACTIVATION_CODES)
+        raise
+    validate_linear_act_inputs(x, w, bias, activation, residual, _ACTIVATION_CODES)
     # the product of `linear` has no rule under functorch transforms, and none for a gradient over no rows
     product = linear if x.numel() and w.numel() and (_NO_TRANSFORM is None or _NO_TRANSFORM()) else ref.linear
     return ref.linear_act(x, w, bias, activation=activation, residual=residual, product=product)
@@ -349,20 +355,39 @@ def add_rms_norm(x, residual, weight, eps: float):
 
 
 # ----------------------------------------------------------------------------------------------- LayerNorm
+# The ops below hand a call to their node first, whose own checks cost nothing beside a launch, and have the arguments named (`ConfigError`) only
+# when it refuses: on the host a small call is bounded by the microseconds in front of it.
 _ROW_TYPES = (torch.bfloat16, torch.float32)
+_REFUSED = (RuntimeError, AttributeError, TypeError)
+
+
+@functools.cache
+def _limits():
+    """Largest LayerNorm widths (bf16, fp32) and head width of the norm with rotation that the kernels have a form for."""
+    ext = _node_ext()
+    return {torch.bfloat16: ext.layer_norm_max_width(False), torch.float32: ext.layer_norm_max_width(True), "head": ext.qk_norm_rope_part_max_dim()}
 
 
 def layer_norm(x, weight, bias, eps: float):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, statistics in fp32."""
+    try:
+        if (x.is_cuda and x.dtype in _ROW_TYPES and weight.dtype == bias.dtype == x.dtype and 0 < x.shape[-1] <= _limits()[x.dtype]
+                and _has_rules(x, weight, bias)):
+            return _node_ext().layer_norm_node(x, weight, bias, eps)
+    except (*_REFUSED, IndexError):
+        validate_layer_norm_inputs(x, weight, bias)
+        raise
     validate_layer_norm_inputs(x, weight, bias)
-    if (_use_cuda(x) and x.dtype in _ROW_TYPES and weight.dtype == bias.dtype == x.dtype and 0 < x.shape[-1] <= _node_ext().layer_norm_max_width(x.dtype == torch.float32)
-            and _has_rules(x, weight, bias)):
-        return _node_ext().layer_norm_node(x, weight, bias, eps)
     return ref.layer_norm(x, weight, bias, eps)
 
 
 # ----------------------------------------------------------------------------------------------- rotary positions, QK-norm + RoPE
-_frequencies = functools.lru_cache(maxsize=64)(lambda head_dim, theta, items: ref.scaled_frequencies(head_dim, theta, dict(items)))
+@functools.lru_cache(maxsize=64)
+def _frequencies(head_dim: int, theta: float, items: tuple):
+    """Scaled inverse frequencies (64-bit tensor on the host) and the factor on both tables."""
+    scaling = validate_rope_scaling(dict(items))
+    inv, factor = ref.scaled_frequencies(head_dim, theta, scaling)
+    return torch.tensor(inv, dtype=torch.float64), factor
 
 
 def rope_tables(positions, head_dim: int, theta: float, dtype=torch.float32, scaling=None):
@@ -371,30 +396,41 @@ def rope_tables(positions, head_dim: int, theta: float, dtype=torch.float32, sca
     original_max_position_embeddings, optionally beta_fast, beta_slow, truncate, attention_factor, mscale, mscale_all_dim); its angles are taken in 64 bits."""
     if scaling is None:
         return ref.rope_tables(positions, head_dim, theta, dtype)
-    validate_rope_scaling(scaling)
     if head_dim < 2 or head_dim % 2 or not theta > 1 or positions.dim() != 1:
         raise ConfigError(f"rotary tables need positions [T], an even head width and theta > 1; got {tuple(positions.shape)}, {head_dim}, {theta}")
-    if not (_use_cuda(positions) and positions.dtype in (torch.int64, torch.int32) and head_dim <= 512 and _has_rules(positions)):
-        return ref.rope_tables(positions, head_dim, theta, dtype, scaling)
-    inv, factor = _frequencies(head_dim, float(theta), tuple(sorted((k, v) for k, v in scaling.items() if v is not None)))
-    cos, sin = _ext().rope_tables(positions.long(), inv, factor)
+    if not (positions.is_cuda and positions.dtype in (torch.int64, torch.int32) and head_dim <= 512 and _has_rules(positions)):
+        return ref.rope_tables(positions, head_dim, theta, dtype, validate_rope_scaling(scaling))
+    try:
+        inv, factor = _frequencies(head_dim, theta, tuple(scaling.items()))
+    except _REFUSED:
+        validate_rope_scaling(scaling)
+        raise
+    cos, sin = _ext().rope_tables(positions if positions.dtype == torch.int64 else positions.long(), inv, factor)
     return (cos, sin) if dtype == torch.float32 else (cos.to(dtype), sin.to(dtype))
 
 
+_INTERLEAVED = {"half": False, "interleaved": True}
+
+
 def _rotary_kernel(cos, sin, *xs) -> bool:
-    return (all(_use_cuda(x) and x.dtype in _ROW_TYPES for x in xs) and cos.dtype == sin.dtype == torch.float32
-            and not (cos.requires_grad or sin.requires_grad) and _has_rules(cos, sin, *xs))
+    return (xs[0].is_cuda and xs[0].dtype in _ROW_TYPES and cos.dtype == sin.dtype == torch.float32 and not (cos.requires_grad or sin.requires_grad)
+            and _has_rules(cos, sin, *xs))
 
 
 def rope(x, cos, sin, *, layout: str = "half", offset: int = 0, inverse: bool = False):
     """x [T, ..., d]: the channels [offset, offset + 2 P) rotate by cos/sin [T, P], the rest pass. `layout` "half" pairs channel j with channel
     j + P of that range, "interleaved" the channels 2j and 2j + 1; `inverse` rotates back. Any strides."""
+    try:
+        if _rotary_kernel(cos, sin, x):
+            node, dims = _node_ext().rope_node, x.dim()
+            if dims == 3:
+                return node(x, cos, sin, offset, _INTERLEAVED[layout], inverse)
+            return node(x.unsqueeze(1) if dims == 2 else x.flatten(1, -2), cos, sin, offset, _INTERLEAVED[layout], inverse).view(x.shape)
+    except (*_REFUSED, KeyError, IndexError):
+        validate_rotary_inputs(x, cos, sin, layout, offset)
+        raise
     validate_rotary_inputs(x, cos, sin, layout, offset)
-    if not _rotary_kernel(cos, sin, x):
-        return ref.rope(x, cos, sin, layout=layout, offset=offset, inverse=inverse)
-    x3 = x if x.dim() == 3 else x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
-    y = _node_ext().rope_node(x3, cos, sin, offset, layout == "interleaved", inverse)
-    return y if x.dim() == 3 else y.view(x.shape)
+    return ref.rope(x, cos, sin, layout=layout, offset=offset, inverse=inverse)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float, *, layout: str = "half", offset: int = 0, norm: bool | None = None,
@@ -406,19 +442,23 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float, *, layout: str 
     plain = norm is None and layout == "half" and offset == 0 and not zero_centered
     if plain and _use_cuda(q) and q.dtype == torch.bfloat16 and q.dim() == 3 and 2 * cos.shape[-1] == q.shape[-1] and q.shape[-1] in (64, 128, 256):
         return tuple(_run_node(_ext().qk_norm_rope_node, q, k, q_weight, k_weight, cos, sin, eps))
+    try:
+        if _rotary_kernel(cos, sin, q, k) and not (plain and q.dtype == torch.float32):
+            nq, nk = norm is not False and (norm or q_weight is not None), norm is not False and (norm or k_weight is not None)
+            ext, inter = _node_ext(), _INTERLEAVED[layout]
+            if not nq and not nk:
+                return tuple(ext.rope_pair_node(q, k, cos, sin, offset, inter))
+            weights = [w for w, n in ((q_weight, nq), (k_weight, nk)) if n and w is not None]
+            if _has_rules(*weights) and all(w.dtype == q.dtype for w in weights) and q.shape[-1] <= _limits()["head"]:
+                if nq and nk:
+                    return tuple(ext.qk_norm_rope_part_node(q, k, q_weight, k_weight, cos, sin, eps, offset, inter, 1.0 if zero_centered else 0.0))
+                kind = dict(layout=layout, offset=offset, zero_centered=zero_centered)
+                return tuple(qk_norm_rope(x, x[:, :0], w, None, cos, sin, eps, norm=n, **kind)[0] for x, w, n in ((q, q_weight, nq), (k, k_weight, nk)))
+    except (*_REFUSED, KeyError, IndexError):
+        validate_qk_inputs(q, k, q_weight, k_weight, cos, sin, layout, offset)
+        raise
     validate_qk_inputs(q, k, q_weight, k_weight, cos, sin, layout, offset)
-    normed = [norm is not False and not (norm is None and w is None) for w in (q_weight, k_weight)]
-    weights = [w for w, n in zip((q_weight, k_weight), normed) if n and w is not None]
-    if ((plain and q.dtype == torch.float32) or not _rotary_kernel(cos, sin, q, k) or not _has_rules(*weights)
-            or any(w.dtype != q.dtype for w in weights) or (any(normed) and q.shape[-1] > _node_ext().qk_norm_rope_part_max_dim())):
-        return ref.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, layout=layout, offset=offset, norm=norm, zero_centered=zero_centered)
-    ext, inter = _node_ext(), layout == "interleaved"
-    if all(normed):
-        return tuple(ext.qk_norm_rope_part_node(q, k, q_weight, k_weight, cos, sin, eps, offset, inter, 1.0 if zero_centered else 0.0))
-    if not any(normed):
-        return tuple(ext.rope_pair_node(q, k, cos, sin, offset, inter))
-    return tuple(qk_norm_rope(x, x[:, :0], w, None, cos, sin, eps, layout=layout, offset=offset, norm=n, zero_centered=zero_centered)[0]
-                 for x, w, n in zip((q, k), (q_weight, k_weight), normed))
+    return ref.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, layout=layout, offset=offset, norm=norm, zero_centered=zero_centered)
 
 
 # ----------------------------------------------------------------------------------------------- SwiGLU
