@@ -1426,10 +1426,12 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     Tensor dz = write ? fresh({M, (N + 7) / 8 * 8}, at::kBFloat16, x) : dy;
     if (write || nb) {
       if (nb) out[2] = fresh(b.sizes(), b.scalar_type(), x);
+      const int P = nb ? llmt_linear_db_partials((int)M, (int)N) : 0;
+      const Tensor part = P > 0 ? fresh({P, N}, at::kFloat, x) : Tensor();
       check_rc(llmt_linear_dz(dy.data_ptr(), M > 1 ? dy.stride(0) : (N + 7) / 8 * 8, act != 0 ? pre.data_ptr() : nullptr, act != 0 ? pre.stride(0) : 0,
                               (int)act, write ? dz.data_ptr() : nullptr, write ? dz.stride(0) : 0, nb ? out[2].data_ptr() : nullptr,
-                              nb && is_f32(b), (int)M, (int)N, cur_stream()),
-               "llmt_linear_dz");
+                              nb && is_f32(b), ws_ptr(part), P, (int)M, (int)N, cur_stream()),
+               "llmt_linear_dz", P > 0 ? 2 : 1);
     }
     if (!nx && !nw) return out;
     if (python_side) {                     // a pending collective rides on the products, or the weight's gradient goes to its owner's buffer

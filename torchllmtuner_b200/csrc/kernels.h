@@ -39,8 +39,9 @@ int llmt_linear_dx(const void* dz, const void* w, void* dx, int M, int N, int K,
                    int* status, cudaStream_t stream);
 int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, int N, int K, int64_t lddz, int64_t ldx, int64_t lddw, float* ws, int64_t ws_floats,
                    int* status, cudaStream_t stream);
-int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, int M, int N,
-                   cudaStream_t stream);
+int llmt_linear_db_partials(int M, int N);
+int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, float* partial,
+                   int P, int M, int N, cudaStream_t stream);
 
 // ---- rotary positions (rope.cu), LayerNorm (layer_norm.cu) ----
 // One operand of a rotation: H heads per token; strides in elements. `w` and `dy` only where the entry point reads them.

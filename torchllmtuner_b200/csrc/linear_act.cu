@@ -23,7 +23,8 @@ constexpr int kLThreads = 64 + 32 * kLEpiWarps;
 constexpr int kLMaxStages = 8;
 constexpr int kLStageA = kLM * kLK * 2;
 constexpr int kLSmem = 227 * 1024;
-constexpr int kLSmemFixed = kLEpiWarps * 4096 + 1024 /*alignment*/ + 512 /*barriers*/;
+constexpr int kLStage = 4096 + 256;        // per epilogue warp: 32 rows of 128 bytes, 64 bias values
+constexpr int kLSmemFixed = kLEpiWarps * kLStage + 1024 /*alignment*/ + 512 /*barriers*/;
 constexpr int kMaxWorkers = 160;
 
 // What becomes of a product: stored as it is, or (`fwd`) with bias, activation and residual.
@@ -96,19 +97,21 @@ struct LinWalk {
   }
 };
 
-__device__ __forceinline__ void load_bias8(const LinOut& o, int col, float* f) {
-  if (o.bias_f32) load_vec<float, 8>(reinterpret_cast<const float*>(o.bias) + col, f);
-  else load_vec<__nv_bfloat16, 8>(reinterpret_cast<const __nv_bfloat16*>(o.bias) + col, f);
-}
-// 32 rows x 64 columns of an operand of the epilogue, as 16 bytes per lane: row it * 4 + lane / 8, columns 8 (lane % 8) on. Clamped instead of
-// skipped, so that the eight loads are in flight together.
-__device__ __forceinline__ void load_patch(const __nv_bfloat16* p, int64_t ld, int row0, int col, int M, int end, int lane, uint4* v) {
-  const int c = col + (lane & 7) * 8 < end ? col + (lane & 7) * 8 : 0;
+// 32 rows x 64 columns of the residual into the warp's staging rows, asynchronously (wait_patch), 16 bytes per lane. Clamped instead of skipped where
+// the patch leaves the matrix. Chunks of 16 bytes are XORed with the row: no bank conflicts.
+__device__ __forceinline__ void load_patch(uint8_t* stg, const LinOut& o, int row0, int col, int end, int lane) {
+  const int cc = lane & 7, c = col + cc * 8 < end ? col + cc * 8 : 0;
+  const __nv_bfloat16* p = o.res + c;
 #pragma unroll
-  for (int it = 0; it < 8; ++it)
-    v[it] = *reinterpret_cast<const uint4*>(p + (int64_t)min(row0 + it * 4 + (lane >> 3), M - 1) * ld + c);
+  for (int it = 0; it < 8; ++it) {
+    const int rr = it * 4 + (lane >> 3);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + rr * 128 + ((cc ^ (rr & 7)) << 4))),
+                 "l"(p + (int64_t)min(row0 + rr, o.M - 1) * o.ldres)
+                 : "memory");
+  }
 }
-// The staging rows (64 bf16 each) of a warp, to global memory in whole 128-byte lines. Chunks of 16 bytes are XORed with the row: no bank conflicts.
+__device__ __forceinline__ void wait_patch() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// The staging rows (64 bf16 each) of a warp, to global memory in whole 128-byte lines.
 __device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p, int64_t ld, int row0, int col, int M, int end, int lane) {
   const int cc = lane & 7;
   if (col + cc * 8 >= end) return;
@@ -119,49 +122,61 @@ __device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p
     if (row0 + rr < M) *reinterpret_cast<uint4*>(p + (int64_t)(row0 + rr) * ld + col + cc * 8) = v;
   }
 }
-__device__ __forceinline__ void stage_row(uint8_t* stg, int lane, const uint32_t* packed) {
+// 64 columns of row `lane`, rounded, into the staging rows.
+__device__ __forceinline__ void stage_row(uint8_t* stg, int lane, const float2* v) {
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
+    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_uint4(pack_bf16x2(v[4 * j].x, v[4 * j].y), pack_bf16x2(v[4 * j + 1].x, v[4 * j + 1].y), pack_bf16x2(v[4 * j + 2].x, v[4 * j + 2].y),
+                   pack_bf16x2(v[4 * j + 3].x, v[4 * j + 3].y));
 }
 
-// A warp's 32 rows x 64 columns of sums (`acc`: 64 columns of row row0 + lane) become results: z = sum + bias, act(z) + residual in fp32, one
-// rounding. Columns from `end` on belong to another tile or to none. `res`: this patch of the residual (load_patch), used where RES. The bf16 rows are turned around in the warp's staging buffer, so
-// that global accesses run along rows.
+// A warp's 32 rows x 64 columns of sums (`acc`: 64 columns of row row0 + lane, in pairs) become results: z = sum + bias, act(z) + residual in fp32,
+// one rounding. Columns from `end` on belong to another tile or to none. The bf16 rows are turned around in the warp's staging buffer, so that global
+// accesses run along rows; the residual comes the same way: asked for by early_patch before the sums are there, or here where z goes first.
+template <int ACT, bool RES>
+__device__ __forceinline__ void early_patch(const LinOut& o, uint8_t* stg, int lane, int row0, int col0, int end) {
+  if (!RES || !o.vec || (ACT != kActNone && o.pre != nullptr)) return;
+  __syncwarp();                                          // the patch before has been read
+  load_patch(stg, o, row0, col0, end, lane);
+}
 template <bool FWD, int ACT, bool RES>
-__device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int lane, int row0, int col0, int end, float* acc, const uint4* res) {
+__device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int lane, int row0, int col0, int end, float2* acc) {
   if (o.vec) {
-    if (FWD && o.bias != nullptr) {
+    if (FWD && o.bias != nullptr) {                      // two values per lane, from where every lane reads them all
+      const int c = col0 + 2 * lane;
+      float b[2] = {0.f, 0.f};
+      if (c < end) {
+        if (o.bias_f32) load_vec<float, 2>(reinterpret_cast<const float*>(o.bias) + c, b);
+        else load_vec<__nv_bfloat16, 2>(reinterpret_cast<const __nv_bfloat16*>(o.bias) + c, b);
+      }
+      float* bs = reinterpret_cast<float*>(stg + 4096);
+      __syncwarp();
+      *reinterpret_cast<float2*>(bs + 2 * lane) = make_float2(b[0], b[1]);
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (col0 + 8 * j < end) {
-          float b[8];
-          load_bias8(o, col0 + 8 * j, b);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[8 * j + i] += b[i];
-        }
+      for (int j = 0; j < 16; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(bs + 4 * j);
+        acc[2 * j] = add2(acc[2 * j], make_float2(v.x, v.y));
+        acc[2 * j + 1] = add2(acc[2 * j + 1], make_float2(v.z, v.w));
       }
     }
-    uint32_t packed[32];
     if (FWD && ACT != kActNone && o.pre != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) packed[j] = pack_bf16x2(acc[2 * j], acc[2 * j + 1]);
       __syncwarp();
-      stage_row(stg, lane, packed);
+      stage_row(stg, lane, acc);
       __syncwarp();
       store_patch(stg, o.pre, o.ldpre, row0, col0, o.M, end, lane);
+      if (RES) {
+        __syncwarp();
+        load_patch(stg, o, row0, col0, end, lane);
+      }
     }
     if (FWD) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = activate<ACT>(acc[j]);
+      for (int j = 0; j < 32; ++j) acc[j] = activate<ACT>(acc[j]);
     }
     if (FWD && RES) {
-      __syncwarp();
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int rr = it * 4 + (lane >> 3);
-        *reinterpret_cast<uint4*>(stg + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4)) = res[it];
-      }
+      wait_patch();
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -169,13 +184,11 @@ __device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int 
         float q[8];
         unpack_bf16x2(v.x, q); unpack_bf16x2(v.y, q + 2); unpack_bf16x2(v.z, q + 4); unpack_bf16x2(v.w, q + 6);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[8 * j + i] += q[i];
+        for (int i = 0; i < 4; ++i) acc[4 * j + i] = add2(acc[4 * j + i], make_float2(q[2 * i], q[2 * i + 1]));
       }
     }
-#pragma unroll
-    for (int j = 0; j < 32; ++j) packed[j] = pack_bf16x2(acc[2 * j], acc[2 * j + 1]);
     __syncwarp();
-    stage_row(stg, lane, packed);
+    stage_row(stg, lane, acc);
     __syncwarp();
     store_patch(stg, o.C, o.ldc, row0, col0, o.M, end, lane);
     return;
@@ -186,7 +199,7 @@ __device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int 
     float* turn = reinterpret_cast<float*>(stg);
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) turn[lane * 32 + ((j + lane) & 31)] = acc[32 * half + j];
+    for (int j = 0; j < 32; ++j) turn[lane * 32 + ((j + lane) & 31)] = j & 1 ? acc[16 * half + j / 2].y : acc[16 * half + j / 2].x;
     __syncwarp();
     const int col = col0 + 32 * half + lane;
     if (col >= end) continue;
@@ -195,18 +208,23 @@ __device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int 
       if (o.bias_f32) bias = reinterpret_cast<const float*>(o.bias)[col];
       else bias = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(o.bias)[col]);
     }
+    const int rows = min(32, o.M - row0);
 #pragma unroll 4
-    for (int rr = 0; rr < 32; ++rr) {
-      const int row = row0 + rr;
-      if (row >= o.M) break;
-      float v = turn[rr * 32 + ((lane + rr) & 31)];
+    for (int rr = 0; rr < rows; rr += 2) {               // two rows at a time, as the activations come in pairs
+      const int next = rr + 1 < rows ? rr + 1 : rr;
+      float2 v = make_float2(turn[rr * 32 + ((lane + rr) & 31)], turn[next * 32 + ((lane + next) & 31)]);
+      const int64_t r0 = row0 + rr, r1 = row0 + next;
       if (FWD) {
-        v += bias;
-        if (ACT != kActNone && o.pre != nullptr) o.pre[(int64_t)row * o.ldpre + col] = __float2bfloat16_rn(v);
+        v = add2(v, make_float2(bias, bias));
+        if (ACT != kActNone && o.pre != nullptr) {
+          o.pre[r0 * o.ldpre + col] = __float2bfloat16_rn(v.x);
+          o.pre[r1 * o.ldpre + col] = __float2bfloat16_rn(v.y);
+        }
         v = activate<ACT>(v);
-        if (RES) v += __bfloat162float(o.res[(int64_t)row * o.ldres + col]);
+        if (RES) v = add2(v, make_float2(__bfloat162float(o.res[r0 * o.ldres + col]), __bfloat162float(o.res[r1 * o.ldres + col])));
       }
-      o.C[(int64_t)row * o.ldc + col] = __float2bfloat16_rn(v);
+      o.C[r0 * o.ldc + col] = __float2bfloat16_rn(v.x);
+      o.C[r1 * o.ldc + col] = __float2bfloat16_rn(v.y);
     }
   }
 }
@@ -220,7 +238,7 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
   const LinPlan& plan = a.plan;
   const int stages = plan.stages, stage_bytes = plan.stage_bytes;
   uint8_t* epi = smem + stages * stage_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(epi + kLEpiWarps * 4096);
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi + kLEpiWarps * kLStage);
   uint64_t* empty = full + kLMaxStages;
   uint64_t* tfull = empty + kLMaxStages;
   uint64_t* tempty = tfull + 2;
@@ -379,7 +397,7 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
     // ------------------------------------------------------------------ epilogue
     // Two warps share a quarter of the rows (the TMEM lanes a warp may read) and take alternate patches of 64 columns.
     const int quarter = warp & 3, side = (warp - 2) >> 2;
-    uint8_t* stg = epi + (warp - 2) * 4096;
+    uint8_t* stg = epi + (warp - 2) * kLStage;
     int acc = 0;
     uint32_t acc_phase = 0;
     while (walk.step(plan, a.out.N, kGroup, u)) {
@@ -394,11 +412,10 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
 #pragma unroll 1
       for (int c = side * 64; c < cols; c += 128) {
-        uint32_t r[64];
+        __align__(8) uint32_t r[64];
         tmem_ld_32x32(t_row + c, r);
         tmem_ld_32x32(t_row + c + 32, r + 32);
-        uint4 res[RES ? 8 : 1];
-        if (RES && a.out.vec) load_patch(a.out.res, a.out.ldres, row0, u.n0 + c, a.out.M, u.n0 + cols, lane, res);
+        early_patch<ACT, RES>(a.out, stg, lane, row0, u.n0 + c, u.n0 + cols);
         tmem_wait_ld();
         if constexpr (SPLIT) {
           const int64_t tiles = (int64_t)plan.num_m * plan.full_n + (a.out.N % plan.bn ? plan.num_m : 0);
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
             if (c + 4 * j < u.width)
               w[j * 32] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
         } else {
-          finish_patch<FWD, ACT, RES>(a.out, stg, lane, row0, u.n0 + c, u.n0 + cols, reinterpret_cast<float*>(r), res);
+          finish_patch<FWD, ACT, RES>(a.out, stg, lane, row0, u.n0 + c, u.n0 + cols, reinterpret_cast<float2*>(r));
         }
       }
       tc_fence_before();
@@ -432,7 +449,7 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
 constexpr int kJoinWarps = 4;
 template <bool FWD, int ACT, bool RES>
 __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __grid_constant__ LinArgs a, int cg, int patches) {
-  __shared__ __align__(16) uint8_t stage[kJoinWarps][4096];
+  __shared__ __align__(16) uint8_t stage[kJoinWarps][kLStage];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int id = blockIdx.x * kJoinWarps + wid;
   if (id >= patches) return;
@@ -450,94 +467,140 @@ __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __gr
   const int width = n >= p.full_n ? (a.out.N - n * p.bn + 31) & ~31 : p.bn;
   const int64_t tiles = (int64_t)whole + (a.out.N % p.bn ? p.num_m : 0), part = tiles * blocks * (p.bn / 4) * 32;
   const float4* w = reinterpret_cast<const float4*>(p.ws) + (((int64_t)tile * blocks + block) * (p.bn / 4) + c / 4) * 32 + lane;
-  uint4 res[8];
-  if (RES && a.out.vec) load_patch(a.out.res, a.out.ldres, row0, col0, a.out.M, a.out.N, lane, res);
-  float acc[64];
+  early_patch<ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N);
+  float2 acc[32];
 #pragma unroll
-  for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+  for (int j = 0; j < 32; ++j) acc[j] = make_float2(0.f, 0.f);
   for (int s = 0; s < p.splits; ++s) {
 #pragma unroll
     for (int j = 0; j < 16; ++j)
       if (c + 4 * j < width) {
         const float4 v = w[s * part + j * 32];
-        acc[4 * j] += v.x; acc[4 * j + 1] += v.y; acc[4 * j + 2] += v.z; acc[4 * j + 3] += v.w;
+        acc[2 * j] = add2(acc[2 * j], make_float2(v.x, v.y));
+        acc[2 * j + 1] = add2(acc[2 * j + 1], make_float2(v.z, v.w));
       }
   }
-  finish_patch<FWD, ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N, acc, res);
+  finish_patch<FWD, ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N, acc);
 }
 
 // ------------------------------------------------------------------------------------------ dz and db
-// A block owns a strip of columns and every eighth group of rows; the eight blocks of a cluster add their column sums through distributed
-// shared memory in rank order, so db needs neither a second launch nor a workspace nor atomics.
+// A block owns a strip of LANES * V columns and every blocks-th group of rows, and sums its columns in a fixed order. Few rows (CLUSTER): the eight
+// blocks of a strip are a cluster and add their sums through distributed shared memory in rank order, so db needs no second launch. Many rows:
+// sums per block go to partial [blocks][N] and linear_db_kernel adds them; clusters of eight would leave SMs idle then (a GPC's 16 or 18 SMs hold
+// two of them: half of the machine's time at 16384 x 4608).
 constexpr int kStripBlocks = 8;
-template <int V, int THREADS, int ACT>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy, const __nv_bfloat16* __restrict__ z,
-                                                            int64_t ldz, __nv_bfloat16* __restrict__ dz, int64_t lddz, void* __restrict__ db,
-                                                            int db_f32, int M, int N) {
-  constexpr int LANES = V == 8 ? 8 : 32, COLS = LANES * V, ROWS = THREADS / LANES;
-  __shared__ float part[ROWS / (THREADS / 256)][COLS + 1];
-  __shared__ float total[COLS];
+template <int V, int LANES, bool CLUSTER, int ACT>
+__global__ void __launch_bounds__(256, ACT == kActNone ? 4 : 3) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy, const __nv_bfloat16* __restrict__ z,
+                                                           int64_t ldz, __nv_bfloat16* __restrict__ dz, int64_t lddz, void* __restrict__ db, int db_f32,
+                                                           float* __restrict__ partial, int M, int N) {
+  constexpr int COLS = LANES * V, ROWS = 256 / LANES;
+  __shared__ float part[ROWS][COLS + 4];
+  __shared__ float total[CLUSTER ? COLS : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const int col = blockIdx.x * COLS + lane * V;
-  const uint32_t rank = blockIdx.y;
-  float acc[V];
+  constexpr int W = V > 1 ? V / 2 : 1;                   // pairs; a single column takes two rows as a pair instead
+  float2 acc[W];
 #pragma unroll
-  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  for (int j = 0; j < W; ++j) acc[j] = make_float2(0.f, 0.f);
   if (col < N) {
-    constexpr int U = 4;                                 // rows in flight per thread
-    const int64_t step = (int64_t)ROWS * kStripBlocks;
-    for (int64_t row = (int64_t)rank * ROWS + sub; row < M; row += U * step) {
+    constexpr int U = V > 1 ? 4 : 8;                     // rows in flight per thread
+    const int64_t step = (int64_t)ROWS * gridDim.y;
+    for (int64_t row = (int64_t)blockIdx.y * ROWS + sub; row < M; row += U * step) {
       Raw<__nv_bfloat16, V> rg[U], rz[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        rg[u].zero();
+        rz[u].zero();
         if (row + u * step < M) {
           rg[u].load(dy + (row + u * step) * ldy + col);
           if (ACT != kActNone) rz[u].load(z + (row + u * step) * ldz + col);
         }
+      }
+      if constexpr (V > 1) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (row + u * step >= M) break;
-        float g[V], p[V];
-        rg[u].get(g);
-        if (ACT != kActNone) {
-          rz[u].get(p);
+        for (int u = 0; u < U; ++u) {
+          float g[V], p[V], out[V];
+          rg[u].get(g);
+          if (ACT != kActNone) rz[u].get(p);
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[j] = activate_grad<ACT>(p[j], g[j]);
+          for (int j = 0; j < W; ++j) {
+            float2 v = make_float2(g[2 * j], g[2 * j + 1]);
+            if (ACT != kActNone) v = activate_grad<ACT>(make_float2(p[2 * j], p[2 * j + 1]), v);
+            acc[j] = add2(acc[j], v);                    // rows past the end were loaded as zeros: their gradient is zero
+            out[2 * j] = v.x;
+            out[2 * j + 1] = v.y;
+          }
+          if (dz != nullptr && row + u * step < M) store_vec<__nv_bfloat16, V>(dz + (row + u * step) * lddz + col, out);
         }
+      } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += g[j];
-        if (dz != nullptr) store_vec<__nv_bfloat16, V>(dz + (row + u * step) * lddz + col, g);
+        for (int u = 0; u < U; u += 2) {
+          float2 v, p;
+          rg[u].get(&v.x);
+          rg[u + 1].get(&v.y);
+          rz[u].get(&p.x);
+          rz[u + 1].get(&p.y);
+          if (ACT != kActNone) v = activate_grad<ACT>(p, v);
+          acc[0] = add2(acc[0], v);
+          if (dz != nullptr) {
+            if (row + u * step < M) dz[(row + u * step) * lddz + col] = __float2bfloat16_rn(v.x);
+            if (row + (u + 1) * step < M) dz[(row + (u + 1) * step) * lddz + col] = __float2bfloat16_rn(v.y);
+          }
+        }
       }
     }
   }
   if (db == nullptr) return;
-  constexpr int HELD = ROWS / (THREADS / 256);          // rows of sums in shared memory; the groups of HELD threads' rows follow one another
+  if constexpr (V > 1) {
 #pragma unroll
-  for (int k = 0; k < THREADS / 256; ++k) {
-    if (sub / HELD == k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) part[sub % HELD][lane * V + j] = k ? part[sub % HELD][lane * V + j] + acc[j] : acc[j];
-    __syncthreads();
+    for (int j = 0; j < W; ++j) {
+      part[sub][lane * V + 2 * j] = acc[j].x;
+      part[sub][lane * V + 2 * j + 1] = acc[j].y;
+    }
+  } else {
+    part[sub][lane] = acc[0].x + acc[0].y;
   }
+  __syncthreads();
+  const int oc = blockIdx.x * COLS + threadIdx.x;
   if (threadIdx.x < COLS) {
     float s = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < HELD; ++i) s += part[i][threadIdx.x];
-    total[threadIdx.x] = s;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) s += part[i][threadIdx.x];
+    if constexpr (CLUSTER) total[threadIdx.x] = s;
+    else if (oc < N) partial[(int64_t)blockIdx.y * N + oc] = s;
   }
-  cluster_sync();
-  const int oc = blockIdx.x * COLS + threadIdx.x;
-  if (rank == 0 && threadIdx.x < COLS && oc < N) {
-    float s = total[threadIdx.x];
-    for (int k = 1; k < kStripBlocks; ++k) {
-      float v;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map_u32(smem_u32(&total[threadIdx.x]), k)));
-      s += v;
+  if constexpr (CLUSTER) {
+    cluster_sync();
+    if (blockIdx.y == 0 && threadIdx.x < COLS && oc < N) {
+      float v[kStripBlocks], s = 0.f;
+#pragma unroll
+      for (int k = 0; k < kStripBlocks; ++k)
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[k]) : "r"(cluster_map_u32(smem_u32(&total[threadIdx.x]), k)));
+#pragma unroll
+      for (int k = 0; k < kStripBlocks; ++k) s += v[k];
+      if (db_f32) reinterpret_cast<float*>(db)[oc] = s;
+      else reinterpret_cast<__nv_bfloat16*>(db)[oc] = __float2bfloat16_rn(s);
     }
-    if (db_f32) reinterpret_cast<float*>(db)[oc] = s;
-    else reinterpret_cast<__nv_bfloat16*>(db)[oc] = __float2bfloat16_rn(s);
+    cluster_sync();                                     // no block leaves while its sums are being read
   }
-  cluster_sync();                                       // no block leaves while its sums are being read
+}
+
+// db from partial [P][N]: 32 columns per block, its 32 warps take every 32nd row, fixed order.
+__global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict__ partial, void* __restrict__ db, int db_f32, int P, int N) {
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < N) {
+#pragma unroll 4
+    for (int q = wid; q < P; q += 32) s += partial[(int64_t)q * N + c];
+  }
+  part[wid][lane] = s;
+  __syncthreads();
+  s = warp_sum(part[lane][wid]);
+  const int oc = blockIdx.x * 32 + wid;
+  if (lane != 0 || oc >= N) return;
+  if (db_f32) reinterpret_cast<float*>(db)[oc] = s;
+  else reinterpret_cast<__nv_bfloat16*>(db)[oc] = __float2bfloat16_rn(s);
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -655,7 +718,7 @@ static LinCut lin_find_cut(int M, int N, int K, bool b_mn) {
       for (int splits = 1; splits == 1 || (splits <= 8 && splits * 2 <= kb); ++splits) {
         if (splits > 1 && (bn % 64 || tiles * (splits - 1) >= 2 * most || (int64_t)num_m * splits > 65535)) break;
         double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, b_mn);
-        if (cg == 1) t *= 1.04;                          // a single CTA reads 1.5 times the operands per product
+        if (cg == 1) t *= 1.08;                          // a single CTA reads 1.5 times the operands per product
         if (splits > 1) t += 5.5 + 4e-6 * splits * (double)M * N / 4.0;
         if (t < least) {
           least = t;
@@ -731,22 +794,38 @@ static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda,
   return -4;
 }
 
-template <int V, int THREADS, int ACT>
-static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int db_f32, int M, int N,
-                     cudaStream_t stream) {
-  constexpr int COLS = V == 8 ? 64 : 32;
+// Blocks per strip of the form without clusters; 0: few rows and strips, clusters.
+static int dz_blocks(int M, int N) {
+  if (M <= 2048 && (N + 63) / 64 * kStripBlocks <= 2 * sm_count()) return 0;
+  const int strips = (N + 255) / 256, fill = sm_count() * 3 / strips, rows = (M + 31) / 32;      // at least 32 rows per block
+  return fill < 1 ? 1 : fill < rows ? fill : rows;
+}
+
+template <int V, int LANES, bool CLUSTER, int ACT>
+static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int db_f32, float* partial, int blocks,
+                     int M, int N, cudaStream_t stream) {
+  constexpr int COLS = LANES * V;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((N + COLS - 1) / COLS, kStripBlocks);
-  cfg.blockDim = dim3(THREADS);
+  cfg.gridDim = dim3((N + COLS - 1) / COLS, blocks);
+  cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = 1; at.val.clusterDim.y = kStripBlocks; at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = CLUSTER ? 1 : 0;
   using B = __nv_bfloat16;
-  return cudaLaunchKernelEx(&cfg, linear_dz_kernel<V, THREADS, ACT>, reinterpret_cast<const B*>(dy), ldy, reinterpret_cast<const B*>(z), ldz,
-                            reinterpret_cast<B*>(dz), lddz, db, db_f32, M, N) == cudaSuccess ? 0 : -3;
+  return cudaLaunchKernelEx(&cfg, linear_dz_kernel<V, LANES, CLUSTER, ACT>, reinterpret_cast<const B*>(dy), ldy, reinterpret_cast<const B*>(z), ldz,
+                            reinterpret_cast<B*>(dz), lddz, db, db_f32, partial, M, N) == cudaSuccess ? 0 : -3;
+}
+template <int ACT>
+static int dz_dispatch(bool vec, int blocks, const void* dy, int64_t ldy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int db_f32,
+                       float* partial, int M, int N, cudaStream_t stream) {
+  if (blocks == 0)
+    return vec ? dz_launch<8, 8, true, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, nullptr, kStripBlocks, M, N, stream)
+               : dz_launch<1, 32, true, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, nullptr, kStripBlocks, M, N, stream);
+  return vec ? dz_launch<8, 32, false, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, blocks, M, N, stream)
+             : dz_launch<1, 32, false, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, blocks, M, N, stream);
 }
 
 }  // namespace llmt
@@ -789,20 +868,22 @@ extern "C" int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, in
   a.status = status;
   return lin_gemm(dz, x, a, M, lddz, ldx, true, true, false, 0, ws, ws_floats, stream);
 }
+// Rows of `partial` ([rows][N] floats) that llmt_linear_dz needs for db; 0: none.
+extern "C" int llmt_linear_db_partials(int M, int N) { return dz_blocks(M, N); }
 // dz = dy act'(z) (act 0: dz = dy; dz nullptr: not written), db = column sums of dz in fp32 before rounding (nullptr: not computed).
-extern "C" int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32, int M,
-                              int N, cudaStream_t stream) {
+extern "C" int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32,
+                              float* partial, int P, int M, int N, cudaStream_t stream) {
   if (M < 0 || N <= 0 || act < 0 || act >= kActKinds || (act != 0 && z == nullptr)) return -10;
+  const int blocks = dz_blocks(M, N);
+  if (db != nullptr && blocks > 0 && (partial == nullptr || P < blocks)) return -10;
   auto at16 = [](const void* p, int64_t ld) { return p == nullptr || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % 8 == 0); };
   const bool vec = N % 8 == 0 && at16(dy, ldy) && at16(act ? z : nullptr, ldz) && at16(dz, lddz);
-  // few strips of columns and many rows: larger blocks, so that an SM has enough loads in flight (16384 x 1152: 18 strips, 144 blocks)
-  const bool few = (int64_t)((N + 63) / 64) * kStripBlocks < 3 * sm_count() && M > 2048;
-#define LLMT_DZ(ACT)                                                                                              \
-  if (act == ACT)                                                                                                 \
-    return !vec ? dz_launch<1, 256, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, M, N, stream)                     \
-           : few ? dz_launch<8, 1024, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, M, N, stream)                   \
-                 : dz_launch<8, 256, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, M, N, stream);
+  int rc = -4;
+#define LLMT_DZ(ACT) \
+  if (act == ACT) rc = dz_dispatch<ACT>(vec, blocks, dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, M, N, stream);
   LLMT_DZ(0) LLMT_DZ(1) LLMT_DZ(2) LLMT_DZ(3) LLMT_DZ(4)
 #undef LLMT_DZ
-  return -4;
+  if (rc || db == nullptr || blocks == 0) return rc;
+  linear_db_kernel<<<(N + 31) / 32, 1024, 0, stream>>>(partial, db, db_f32, blocks, N);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

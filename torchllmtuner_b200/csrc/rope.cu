@@ -236,19 +236,20 @@ __device__ __forceinline__ void lane_weight(const void* w, int c, int d, float s
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] += shift;
 }
-// The partners of the lane's 8 channels.
+// The partners of the lane's 8 channels (pairs x).
 template <typename T, int G, bool PAIRS>
-__device__ __forceinline__ void partners(const Raw<T, 8>& raw, const float* x, int partner, float* o) {
+__device__ __forceinline__ void partners(const Raw<T, 8>& raw, const float2* x, int partner, float2* o) {
   if constexpr (PAIRS) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = x[i ^ 1];
+    for (int i = 0; i < 4; ++i) o[i] = make_float2(x[i].y, x[i].x);
   } else {
     Raw<T, 8> q;
 #pragma unroll
     for (int i = 0; i < Raw<T, 8>::kWords; ++i) q.w[i] = __shfl_sync(0xffffffffu, raw.w[i], partner, G);
-    q.get(o);
+    get2(q, o);
   }
 }
+
 // A group takes HB heads of one token, `shares` apart; their loads are issued before the tables' and weights', so a warp waits for memory once.
 // blockIdx.y: queries or keys.
 template <typename T, int G, bool PAIRS, int HB>
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid
   const unsigned shares = blockIdx.y ? k_shares : q_shares;
   constexpr int GPB = 256 / G;
   const int g = threadIdx.x % G;
+  if (blockIdx.x * GPB >= (unsigned)s.T * shares) return;      // queries and keys need different numbers of blocks
   const unsigned item = blockIdx.x * GPB + threadIdx.x / G;
   const unsigned token = item / shares;
   const int share = (int)(item - token * shares);
@@ -272,27 +274,27 @@ __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid
   }
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
   const LanePlace p = lane_place(s, g);
-  float cw[8], nw[8];
+  float2 cw[4], nw[4];
   {
-    float w[8], wp[8];
-    lane_tables(s, p, t, wide, 1.f, cw, nw);
+    float c[8], n[8], w[8], wp[8];
+    lane_tables(s, p, t, wide, 1.f, c, n);
     lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
     lane_weight<T>(o.w, p.partner * 8, s.d, a.shift, wp);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      cw[j] *= w[j];
-      nw[j] *= PAIRS ? wp[j ^ 1] : wp[j];
+    for (int j = 0; j < 4; ++j) {
+      cw[j] = make_float2(c[2 * j] * w[2 * j], c[2 * j + 1] * w[2 * j + 1]);
+      nw[j] = make_float2(n[2 * j] * wp[PAIRS ? 2 * j + 1 : 2 * j], n[2 * j + 1] * wp[PAIRS ? 2 * j : 2 * j + 1]);
     }
   }
   const float inv_d = 1.f / (float)s.d;
   float sq[HB];
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
-    float x[8];
-    raw[i].get(x);
-    sq[i] = 0.f;
+    float2 x[4], q = make_float2(0.f, 0.f);
+    get2(raw[i], x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sq[i] += x[j] * x[j];
+    for (int j = 0; j < 4; ++j) q = fma2(x[j], x[j], q);
+    sq[i] = q.x + q.y;
   }
 #pragma unroll
   for (int m = G / 2; m > 0; m >>= 1)
@@ -301,77 +303,92 @@ __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid
   T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
-    float x[8], q[8];
-    raw[i].get(x);
+    float2 x[4], q[4];
+    get2(raw[i], x);
     partners<T, G, PAIRS>(raw[i], x, p.partner, q);
     const float r = rsqrtf(sq[i] * inv_d + a.eps);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = r * (x[j] * cw[j] + q[j] * nw[j]);
-    if (on && share + i * (int)shares < o.H) store_vec<T, 8>(py + (int64_t)(share + i * (int)shares) * o.y_head, x);
+    for (int j = 0; j < 4; ++j) x[j] = mul2(make_float2(r, r), fma2(x[j], cw[j], mul2(q[j], nw[j])));
+    if (on && share + i * (int)shares < o.H) store2(py + (int64_t)(share + i * (int)shares) * o.y_head, x);
   }
 }
 
-// The same split for the gradient; a group walks over items (token, share) and holds its sums of the weight's gradient. The operands of the next
-// item are fetched before this one's sums are taken.
+// The same split for the gradient; a group walks over a run of items (token, share), reads the tables where the token changes and holds its sums of
+// the weight's gradient. The operands of the next item are fetched before this one's sums are taken.
 template <typename T, int G, bool PAIRS, int HB>
-__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares_) {
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares) {
   const RopeShape& s = a.s;
   const NormOperand& o = a.q;
   constexpr int GPB = 256 / G;
   __shared__ float sums[GPB][G * 8 + 4];
-  const unsigned shares = shares_, items = (unsigned)s.T * shares, step = gridDim.x * GPB;
+  const unsigned items = (unsigned)s.T * shares, groups = gridDim.x * GPB;
   const int g = threadIdx.x % G, grp = threadIdx.x / G;
   const bool in = g * 8 < s.d;
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
   const LanePlace p = lane_place(s, g);
   const float inv_d = 1.f / (float)s.d;
-  float dw[8], w[8];
+  const unsigned each = items / groups, more = items % groups, me = blockIdx.x * GPB + grp;      // the first `more` groups have one item more
+  unsigned item = me * each + (me < more ? me : more);
+  const unsigned end = item + each + (me < more ? 1 : 0), rounds = each + (more ? 1 : 0);      // rounds: the same for the whole block
+  float2 dw[4], w[4], c[4], n[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dw[i] = 0.f;
+  for (int i = 0; i < 4; ++i) dw[i] = c[i] = n[i] = make_float2(0.f, 0.f);
   Raw<T, 8> rx[HB], rd[HB];
-  int64_t t;
-  int share;
-  auto fetch = [&](unsigned item, int64_t& tok, int& sh, Raw<T, 8>* x, Raw<T, 8>* d) {
-    const unsigned it = item < items ? item : items - 1;
-    tok = it / shares;
-    sh = (int)(it - (unsigned)tok * shares);
+  int64_t t = item / (unsigned)shares, tables_of = -1;
+  int share = (int)(item - (unsigned)t * shares);
+  auto fetch = [&](bool valid, int64_t tok, int sh, Raw<T, 8>* x, Raw<T, 8>* d) {
     const T* px = reinterpret_cast<const T*>(o.x) + tok * o.x_tok + g * 8;
     const T* pd = reinterpret_cast<const T*>(o.dy) + tok * o.dy_tok + g * 8;
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       x[i].zero();
       d[i].zero();
-      if (in && item < items && sh + i * shares_ < o.H) {
-        x[i].load(px + (int64_t)(sh + i * shares_) * o.x_head);
-        d[i].load(pd + (int64_t)(sh + i * shares_) * o.dy_head);
+      if (valid && sh + i * shares < o.H) {
+        x[i].load(px + (int64_t)(sh + i * shares) * o.x_head);
+        d[i].load(pd + (int64_t)(sh + i * shares) * o.dy_head);
       }
     }
   };
-  unsigned b0 = blockIdx.x * GPB;
-  fetch(b0 + grp, t, share, rx, rd);
-  lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
-  for (; b0 < items; b0 += step) {                      // uniform in the block; items + step fits 32 bits
-    const bool live = in && b0 + grp < items;
-    float c[8], n[8];
-    lane_tables(s, p, t, wide, -1.f, c, n);
+  fetch(in && item < end, t, share, rx, rd);
+  {
+    float f[8];
+    lane_weight<T>(o.w, g * 8, s.d, a.shift, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = make_float2(f[2 * i], f[2 * i + 1]);
+  }
+  for (unsigned round = 0; round < rounds; ++round, ++item) {
+    const bool live = in && item < end;
+    if (item < end && t != tables_of) {
+      float fc[8], fn[8];
+      lane_tables(s, p, t, wide, -1.f, fc, fn);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = make_float2(fc[2 * i], fc[2 * i + 1]);
+        n[i] = make_float2(fn[2 * i], fn[2 * i + 1]);
+      }
+      tables_of = t;
+    }
+    const bool wrap = share + 1 == shares;
+    const int64_t nt = wrap ? t + 1 : t;
+    const int nshare = wrap ? 0 : share + 1;
     Raw<T, 8> nx[HB], nd[HB];
-    int64_t nt = t;
-    int nshare = share;
-    if (b0 + step < items) fetch(b0 + step + grp, nt, nshare, nx, nd);
-    float d[HB][8], sq[HB], dot[HB];
+    fetch(in && item + 1 < end, nt, nshare, nx, nd);
+    float2 d[HB][4];
+    float sq[HB], dot[HB];
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
-      float x[8], q[8], e[8];
-      rd[i].get(e);
+      float2 x[4], q[4], e[4], s2 = make_float2(0.f, 0.f), d2 = s2;
+      get2(rd[i], e);
       partners<T, G, PAIRS>(rd[i], e, p.partner, q);
-      rx[i].get(x);
-      sq[i] = dot[i] = 0.f;
+      get2(rx[i], x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        d[i][j] = e[j] * c[j] + q[j] * n[j];
-        sq[i] += x[j] * x[j];
-        dot[i] += d[i][j] * w[j] * x[j];
+      for (int j = 0; j < 4; ++j) {
+        d[i][j] = fma2(e[j], c[j], mul2(q[j], n[j]));
+        s2 = fma2(x[j], x[j], s2);
+        d2 = fma2(mul2(d[i][j], w[j]), x[j], d2);
       }
+      sq[i] = s2.x + s2.y;
+      dot[i] = d2.x + d2.y;
     }
 #pragma unroll
     for (int m = G / 2; m > 0; m >>= 1)
@@ -383,17 +400,17 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __g
     T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
-      if (live && share + i * shares_ < o.H) {           // a dead head's r may be infinite (eps 0)
-        const float r = rsqrtf(sq[i] * inv_d + a.eps), k = r * r * r * dot[i] * inv_d;
-        float x[8], out[8];
-        rx[i].get(x);
+      if (live && share + i * shares < o.H) {            // a dead head's r may be infinite (eps 0)
+        const float r = rsqrtf(sq[i] * inv_d + a.eps), k = -(r * r * r * dot[i] * inv_d);
+        float2 x[4], out[4];
+        get2(rx[i], x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float dr = d[i][j] * r;
-          dw[j] += dr * x[j];
-          out[j] = dr * w[j] - x[j] * k;
+        for (int j = 0; j < 4; ++j) {
+          const float2 dr = mul2(d[i][j], make_float2(r, r));
+          dw[j] = fma2(dr, x[j], dw[j]);
+          out[j] = fma2(dr, w[j], mul2(x[j], make_float2(k, k)));
         }
-        store_vec<T, 8>(py + (int64_t)(share + i * shares_) * o.y_head, out);
+        store2(py + (int64_t)(share + i * shares) * o.y_head, out);
       }
       rx[i] = nx[i];
       rd[i] = nd[i];
@@ -404,7 +421,7 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __g
   if (a.partial == nullptr) return;
   if (in) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sums[grp][g * 8 + j] = dw[j];
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(&sums[grp][g * 8 + 2 * j]) = dw[j];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < s.d; i += 256) {        // the groups of a block in their order

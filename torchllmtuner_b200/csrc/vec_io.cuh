@@ -86,4 +86,38 @@ __device__ __forceinline__ void store_vec(T* p, const float* f) {
   r.store(p);
 }
 
+// Pairs of fp32 values in one instruction, each rounded as the scalar one.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<uint64_t*>(&r)) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<uint64_t*>(&r)) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t*>(&r))
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return r;
+}
+// Eight values as four pairs.
+template <typename T>
+__device__ __forceinline__ void get2(const Raw<T, 8>& r, float2* f) {
+  float v[8];
+  r.get(v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+template <typename T>
+__device__ __forceinline__ void store2(T* p, const float2* f) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = f[i].x; v[2 * i + 1] = f[i].y; }
+  store_vec<T, 8>(p, v);
+}
+
 }  // namespace llmt
