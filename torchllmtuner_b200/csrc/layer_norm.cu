@@ -385,7 +385,7 @@ static int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void
   if (!ln_same_shift<T>(x, ldx, D, {y}) || ldx < D || vecs > kLnMaxVecs || wb % sizeof(T)) return -10;
   const LnShape s = ln_fwd_shape(vecs);
   const int V = Granule<T>::V, threads = s.tr * s.groups;
-  const int most = sm_count() * (s.tr == 32 ? (s.nv <= 5 ? 4 : 2) : 1024 / threads);
+  const int most = sm_count() * (s.tr == 32 ? (s.nv <= 2 ? 4 : s.nv <= 5 ? 2 : 1) : 1024 / threads);
   const int need = (R + s.groups - 1) / s.groups;
   const int grid = ((need < most ? need : most) + V - 1) / V * V;
   const T *xp = reinterpret_cast<const T*>(x), *wp = reinterpret_cast<const T*>(w), *bp = reinterpret_cast<const T*>(b);

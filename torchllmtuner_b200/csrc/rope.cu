@@ -41,6 +41,25 @@ __device__ __forceinline__ void load_table(const float* t, int j, bool wide, flo
   }
 }
 
+// For V channels from c0 on: the factor of the channel and of its partner when rotating by `sign`, and how far away the partner is (0: the channel
+// passes).
+template <int V>
+__device__ __forceinline__ void channel_tables(const RopeShape& s, int c0, int64_t t, float sign, float* c, float* n, int* gap) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int at = c0 + j - s.off;
+    c[j] = 1.f;
+    n[j] = 0.f;
+    gap[j] = 0;
+    if (at < 0 || at >= 2 * s.P) continue;
+    const bool second = s.interleaved ? at & 1 : at >= s.P;
+    const int pair = s.interleaved ? at >> 1 : second ? at - s.P : at, step = s.interleaved ? 1 : s.P;
+    c[j] = s.cosb[t * s.ldt + pair];
+    n[j] = s.sinb[t * s.ldt + pair] * (second ? sign : -sign);
+    gap[j] = second ? -step : step;
+  }
+}
+
 // ------------------------------------------------------------------------------------------ rotation
 // A thread owns one unit of one token in up to four heads, so its cos and sin are read once: a pair of vectors (half layout), a vector that
 // holds whole pairs (interleaved), or a vector that passes. Neighbouring threads own neighbouring units, then neighbouring heads, so a warp
@@ -122,16 +141,55 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeShape s, RopeWork wa, Rop
   }
 }
 
+// Pairs that straddle vectors (half layout with P or off no multiple of the vector, interleaved pairs that start on an odd channel): a thread owns V
+// channels in a row, which it reads and writes as vectors, and reads their partners one by one (they are in L1).
+template <typename T, int V>
+__global__ void __launch_bounds__(256) rope_gather_kernel(RopeShape s, RopeWork wa, RopeWork wb) {
+  const RopeWork& k = blockIdx.y ? wb : wa;
+  const int units = s.d / V, per_token = units * k.shares;
+  const int lt = per_token >= 256 ? 0 : threadIdx.x / per_token;
+  const int64_t t = (int64_t)blockIdx.x * k.tokens + lt;
+  if (lt >= k.tokens || t >= s.T) return;
+  const int64_t x_step = k.o.x_head * k.shares, y_step = k.o.y_head * k.shares;
+  for (int w = threadIdx.x - lt * per_token; w < per_token; w += 256) {
+    const int share = w / units, c0 = (w - share * units) * V;
+    const T* px = reinterpret_cast<const T*>(k.o.x) + t * k.o.x_tok + share * k.o.x_head + c0;
+    T* py = reinterpret_cast<T*>(k.o.y) + t * k.o.y_tok + share * k.o.y_head + c0;
+    Raw<T, V> r[kRopeHeads];
+#pragma unroll
+    for (int i = 0; i < kRopeHeads; ++i)
+      if (share + i * k.shares < k.o.H) r[i].load(px + i * x_step);
+    float c[V], n[V];
+    int gap[V];
+    channel_tables<V>(s, c0, t, s.sign, c, n, gap);
+#pragma unroll
+    for (int i = 0; i < kRopeHeads; ++i) {
+      if (share + i * k.shares >= k.o.H) continue;
+      float x[V];
+      r[i].get(x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (gap[j] == 0) continue;                       // passes
+        float q;
+        load_vec<T, 1>(px + i * x_step + j + gap[j], &q);
+        x[j] = x[j] * c[j] + q * n[j];
+      }
+      store_vec<T, V>(py + i * y_step, x);
+    }
+  }
+}
+
 static bool div_by(int v, std::initializer_list<int64_t> xs) {
   for (int64_t x : xs)
     if (x % v) return false;
   return true;
 }
-// The widest vector (at most `most` values) that divides the parts of a head and fits every address.
-static int rope_vec(const RopeShape& s, const RopeOperand& a, const RopeOperand& b, int size, int most) {
+// The widest vector (at most `most` values) that divides a head and fits every address, and, with `pairs`, the parts of a head as well.
+static int rope_vec(const RopeShape& s, const RopeOperand& a, const RopeOperand& b, int size, int most, bool pairs) {
   for (int v = most; v > 1; v /= 2) {
     const int64_t part = s.interleaved ? 2 * s.P : s.P;
-    if (!div_by(v, {part, s.off, s.d, a.x_tok, a.x_head, a.y_tok, a.y_head})) continue;
+    if (pairs && !div_by(v, {part, s.off})) continue;
+    if (!div_by(v, {s.d, a.x_tok, a.x_head, a.y_tok, a.y_head})) continue;
     if (b.H && !div_by(v, {b.x_tok, b.x_head, b.y_tok, b.y_head})) continue;
     const uintptr_t bytes = v * size < 16 ? v * size : 16;
     uintptr_t at = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y);
@@ -141,9 +199,10 @@ static int rope_vec(const RopeShape& s, const RopeOperand& a, const RopeOperand&
   return 1;
 }
 
-template <typename T, int V, bool PAIRS>
+// GATHER: rope_gather_kernel, else rope_kernel with pairs side by side (PAIRS) or in halves.
+template <typename T, int V, bool PAIRS, bool GATHER>
 static int rope_launch(const RopeShape& s, const RopeOperand& a, const RopeOperand& b, cudaStream_t stream) {
-  const int units = (PAIRS ? (V == 1 ? s.P : 2 * s.P / V) : s.P / V) + (s.d - 2 * s.P) / V;
+  const int units = GATHER ? s.d / V : (PAIRS ? (V == 1 ? s.P : 2 * s.P / V) : s.P / V) + (s.d - 2 * s.P) / V;
   int64_t blocks = 0;
   auto work = [&](const RopeOperand& o) {
     RopeWork w{o, (o.H + kRopeHeads - 1) / kRopeHeads, 1};
@@ -155,17 +214,26 @@ static int rope_launch(const RopeShape& s, const RopeOperand& a, const RopeOpera
     if (need > blocks) blocks = need;
     return w;
   };
-  const RopeWork wa = work(a), wb = work(b);
+  const RopeWork wa = work(a.H ? a : b), wb = work(b);
   if (blocks > 0x7fffffff) return -10;
-  if (a.H == 0) rope_kernel<T, V, PAIRS><<<(int)blocks, 256, 0, stream>>>(s, wb, wb, units);
-  else rope_kernel<T, V, PAIRS><<<dim3((int)blocks, b.H ? 2 : 1), 256, 0, stream>>>(s, wa, wb, units);
+  const dim3 grid((int)blocks, a.H && b.H ? 2 : 1);
+  if constexpr (GATHER) rope_gather_kernel<T, V><<<grid, 256, 0, stream>>>(s, wa, wb);
+  else rope_kernel<T, V, PAIRS><<<grid, 256, 0, stream>>>(s, wa, wb, units);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 template <typename T>
 static int rope_dispatch(const RopeShape& s, const RopeOperand& a, const RopeOperand& b, cudaStream_t stream) {
-  const int v = rope_vec(s, a, b, sizeof(T), 16 / (int)sizeof(T));
+  constexpr int kMost = 16 / (int)sizeof(T);
+  const int v = rope_vec(s, a, b, sizeof(T), kMost, true), g = rope_vec(s, a, b, sizeof(T), kMost, false);
+  // the partners one by one cost less than narrow vectors for everything (9000 x 20 heads of 80, 34 rotated in halves: 36 us with V = 1)
+  if (g >= 4 * v || (g > v && v == 1)) {
+#define LLMT_ROPE(N) if (g == N) return rope_launch<T, N, false, true>(s, a, b, stream);
+    if constexpr (sizeof(T) == 2) { LLMT_ROPE(8) }
+    LLMT_ROPE(4) LLMT_ROPE(2)
+#undef LLMT_ROPE
+  }
 #define LLMT_ROPE(N) \
-  if (v == N) return s.interleaved ? rope_launch<T, N, true>(s, a, b, stream) : rope_launch<T, N, false>(s, a, b, stream);
+  if (v == N) return s.interleaved ? rope_launch<T, N, true, false>(s, a, b, stream) : rope_launch<T, N, false, false>(s, a, b, stream);
   if constexpr (sizeof(T) == 2) { LLMT_ROPE(8) }
   LLMT_ROPE(4) LLMT_ROPE(2) LLMT_ROPE(1)
 #undef LLMT_ROPE
@@ -179,7 +247,7 @@ static int rope_dispatch(const RopeShape& s, const RopeOperand& a, const RopeOpe
 // tables a channel is r (x cw + x' nw), x' its partner: in the lane itself (interleaved), or in the lane P / 8 away (half layout), from where the
 // lane's raw 16 bytes come by shuffle. A channel that passes has cw = w, nw = 0. A group takes several heads of one token, so tables and weights are
 // loaded once for them and several loads are in flight. Needs d, off and P (interleaved: 2 P) divisible by 8, d <= 256 and 16-byte addresses. Bound by memory where there are thousands of tokens.
-// General form: a warp per head, the normalised head in shared memory, any d <= 1024.
+// Gather form (below): any parts of a head up to d = 256. General form: a warp per head, the normalised head in shared memory, any d <= 1024.
 struct NormOperand {
   const void *x, *w;
   void* y;                       // forward: the result; backward: dx
@@ -432,6 +500,180 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __g
   }
 }
 
+// The form for everything else up to d = 256: a lane still holds 8 channels (read and written VL at a time, as d and the addresses allow), and the
+// partners come through shared memory: channel c lies at (c % 8) G + c / 8, so that neighbouring lanes read neighbouring words whatever P and off.
+template <typename T, int VL>
+__device__ __forceinline__ void load_lane(const T* p, int c, int d, float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; i += VL) {
+#pragma unroll
+    for (int j = 0; j < VL; ++j) f[i + j] = 0.f;
+    if (c + i < d) load_vec<T, VL>(p + i, f + i);
+  }
+}
+template <typename T, int VL>
+__device__ __forceinline__ void store_lane(T* p, int c, int d, const float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; i += VL)
+    if (c + i < d) store_vec<T, VL>(p + i, f + i);
+}
+// The partners of the lane's channels; `box`: 8 G words of the lane's group.
+template <int G>
+__device__ __forceinline__ void gather_lane(float* box, int g, const float* x, const int* at, float* q) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) box[j * G + g] = x[j];
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = box[at[j]];
+}
+template <int G>
+__device__ __forceinline__ void lane_channels(const RopeShape& s, int g, int64_t t, float sign, float* c, float* n, int* at) {
+  channel_tables<8>(s, g * 8, t, sign, c, n, at);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int p = g * 8 + j + at[j];
+    at[j] = (p & 7) * G + (p >> 3);
+  }
+}
+template <typename T, int VL>
+__device__ __forceinline__ void lane_weights(const void* w, int c, int d, float shift, float* f) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 1.f;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f[j] = 0.f;
+    if (c + j < d) {
+      load_vec<T, 1>(reinterpret_cast<const T*>(w) + c + j, f + j);
+      f[j] += shift;
+    }
+  }
+}
+constexpr int kGatherHeads = 2;
+template <typename T, int G, int VL>
+__global__ void __launch_bounds__(256) qk_norm_rope_gather_fwd_kernel(const __grid_constant__ NormArgs a, int q_shares, int k_shares) {
+  const RopeShape& s = a.s;
+  const NormOperand& o = blockIdx.y ? a.k : a.q;
+  const unsigned shares = blockIdx.y ? k_shares : q_shares;
+  constexpr int GPB = 256 / G;
+  __shared__ float boxes[GPB][8 * G];
+  if (blockIdx.x * GPB >= (unsigned)s.T * shares) return;
+  const int g = threadIdx.x % G, c0 = g * 8;
+  const unsigned item = blockIdx.x * GPB + threadIdx.x / G, token = item / shares;
+  const int share = (int)(item - token * shares);
+  const bool live = token < (unsigned)s.T;
+  const int64_t t = live ? token : s.T - 1;             // the whole warp stays in the shuffles
+  float x[kGatherHeads][8];
+#pragma unroll
+  for (int i = 0; i < kGatherHeads; ++i) {
+    const int h = share + i * (int)shares;
+    load_lane<T, VL>(reinterpret_cast<const T*>(o.x) + t * o.x_tok + (int64_t)h * o.x_head + c0, live && h < o.H ? c0 : s.d, s.d, x[i]);
+  }
+  float c[8], n[8], w[8];
+  int at[8];
+  lane_channels<G>(s, g, t, 1.f, c, n, at);
+  lane_weights<T, VL>(o.w, c0, s.d, a.shift, w);
+#pragma unroll
+  for (int i = 0; i < kGatherHeads; ++i) {
+    float sq = 0.f, q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sq += x[i][j] * x[i][j];
+#pragma unroll
+    for (int m = G / 2; m > 0; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
+    const float r = rsqrtf(sq / (float)s.d + a.eps);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[i][j] *= r * w[j];
+    gather_lane<G>(boxes[threadIdx.x / G], g, x[i], at, q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[i][j] = at[j] == j * G + g ? x[i][j] : x[i][j] * c[j] + q[j] * n[j];      // its own partner: it passes
+    const int h = share + i * (int)shares;
+    store_lane<T, VL>(reinterpret_cast<T*>(o.y) + t * o.y_tok + (int64_t)h * o.y_head + c0, live && h < o.H ? c0 : s.d, s.d, x[i]);
+  }
+}
+
+template <typename T, int G, int VL>
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_gather_bwd_kernel(const __grid_constant__ NormArgs a, int shares) {
+  const RopeShape& s = a.s;
+  const NormOperand& o = a.q;
+  constexpr int GPB = 256 / G;
+  __shared__ float boxes[GPB][8 * G];
+  const int g = threadIdx.x % G, grp = threadIdx.x / G, c0 = g * 8;
+  const unsigned items = (unsigned)s.T * shares, groups = gridDim.x * GPB;
+  const unsigned each = items / groups, more = items % groups, me = blockIdx.x * GPB + grp;      // the first `more` groups have one item more
+  unsigned item = me * each + (me < more ? me : more);
+  const unsigned end = item + each + (me < more ? 1 : 0), rounds = each + (more ? 1 : 0);
+  int64_t t = item / (unsigned)shares, tables_of = -1;
+  int share = (int)(item - (unsigned)t * shares);
+  float dw[8], w[8], c[8], n[8];
+  int at[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    dw[j] = c[j] = n[j] = 0.f;
+    at[j] = j * G + g;
+  }
+  lane_weights<T, VL>(o.w, c0, s.d, a.shift, w);
+  for (unsigned round = 0; round < rounds; ++round, ++item) {
+    const bool live = item < end;
+    float x[kGatherHeads][8], d[kGatherHeads][8];
+#pragma unroll
+    for (int i = 0; i < kGatherHeads; ++i) {
+      const int h = share + i * shares, from = live && h < o.H ? c0 : s.d;
+      load_lane<T, VL>(reinterpret_cast<const T*>(o.x) + t * o.x_tok + (int64_t)h * o.x_head + c0, from, s.d, x[i]);
+      load_lane<T, VL>(reinterpret_cast<const T*>(o.dy) + t * o.dy_tok + (int64_t)h * o.dy_head + c0, from, s.d, d[i]);
+    }
+    if (live && t != tables_of) {
+      lane_channels<G>(s, g, t, -1.f, c, n, at);
+      tables_of = t;
+    }
+#pragma unroll
+    for (int i = 0; i < kGatherHeads; ++i) {
+      const int h = share + i * shares;
+      float q[8], sq = 0.f, dot = 0.f;
+      gather_lane<G>(boxes[grp], g, d[i], at, q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (at[j] != j * G + g) d[i][j] = d[i][j] * c[j] + q[j] * n[j];
+        sq += x[i][j] * x[i][j];
+        dot += d[i][j] * w[j] * x[i][j];
+      }
+#pragma unroll
+      for (int m = G / 2; m > 0; m >>= 1) {
+        sq += __shfl_xor_sync(0xffffffffu, sq, m);
+        dot += __shfl_xor_sync(0xffffffffu, dot, m);
+      }
+      if (live && h < o.H) {                             // a dead head's r may be infinite (eps 0)
+        const float r = rsqrtf(sq / (float)s.d + a.eps), k = r * r * r * dot / (float)s.d;
+        float out[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float dr = d[i][j] * r;
+          if (c0 + j < s.d) dw[j] += dr * x[i][j];
+          out[j] = dr * w[j] - x[i][j] * k;
+        }
+        store_lane<T, VL>(reinterpret_cast<T*>(o.y) + t * o.y_tok + (int64_t)h * o.y_head + c0, c0, s.d, out);
+      }
+    }
+    if (++share == shares) {
+      share = 0;
+      ++t;
+    }
+  }
+  if (a.partial == nullptr) return;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) boxes[grp][c0 + j] = dw[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < s.d; i += 256) {        // the groups of a block in their order
+    float v = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < GPB; ++k) v += boxes[k][i];
+    a.partial[(int64_t)blockIdx.x * s.d + i] = v;
+  }
+}
+
 // General form. Four warps per block, each with one head at a time; buf: the head before the rotation.
 constexpr int kAnyWarps = 4;
 __device__ __forceinline__ float rotated(const RopeShape& s, const float* buf, int c, int64_t t, float sign) {
@@ -527,20 +769,31 @@ __global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float* __rest
   if (lane == 0 && oc < d) store_vec<T, 1>(dw + oc, &v);
 }
 
-static bool norm_wide(const NormArgs& a, int size, bool bwd) {
-  const RopeShape& s = a.s;
-  if (s.d > 256 || !div_by(8, {s.d, s.off, s.interleaved ? 2 * s.P : s.P})) return false;
-  for (const NormOperand* o : {&a.q, &a.k}) {
-    if (!o->H) continue;
-    uintptr_t at = reinterpret_cast<uintptr_t>(o->x) | reinterpret_cast<uintptr_t>(o->y) | reinterpret_cast<uintptr_t>(o->w);
-    if (!div_by(16 / size, {o->x_tok, o->x_head, o->y_tok, o->y_head})) return false;
-    if (bwd) {
-      at |= reinterpret_cast<uintptr_t>(o->dy);
-      if (!div_by(16 / size, {o->dy_tok, o->dy_head})) return false;
+// Values per access that d and the addresses of a call allow (16 bytes at most).
+static int norm_vec(const NormArgs& a, int size, bool bwd) {
+  for (int v = 16 / size; v > 1; v /= 2) {
+    const uintptr_t bytes = v * size;
+    bool ok = a.s.d % v == 0;
+    for (const NormOperand* o : {&a.q, &a.k}) {
+      if (!o->H) continue;
+      uintptr_t at = reinterpret_cast<uintptr_t>(o->x) | reinterpret_cast<uintptr_t>(o->y);
+      ok = ok && div_by(v, {o->x_tok, o->x_head, o->y_tok, o->y_head});
+      if (bwd) {
+        at |= reinterpret_cast<uintptr_t>(o->dy);
+        ok = ok && div_by(v, {o->dy_tok, o->dy_head});
+      }
+      ok = ok && at % bytes == 0;
     }
-    if (at & 15) return false;
+    if (ok) return v;
   }
-  return true;
+  return 1;
+}
+// 2: the wide form, 1: the gather form, 0: the general one.
+static int norm_form(const NormArgs& a, int size, bool bwd) {
+  const RopeShape& s = a.s;
+  if (s.d > 256) return 0;
+  const bool aligned = !((reinterpret_cast<uintptr_t>(a.q.w) | reinterpret_cast<uintptr_t>(a.k.w)) & 15);
+  return aligned && div_by(8, {s.d, s.off, s.interleaved ? 2 * s.P : s.P}) && norm_vec(a, size, bwd) == 16 / size ? 2 : 1;
 }
 // Heads per group: loads in flight and tables read seldom, or one where there are too few tokens to fill the machine that way. Forward up to four,
 // backward two (registers).
@@ -551,18 +804,20 @@ static int norm_heads(const NormArgs& a, int H, int most) {
   while (n > 1 && (int64_t)a.s.T * ((H + n - 1) / n) * norm_lanes(a.s.d) < (int64_t)sm_count() * 1024) n /= 2;
   return n > 1 ? n : 1;
 }
-static int norm_bwd_grid(const NormArgs& a, bool wide) {
-  const int n = norm_heads(a, a.q.H, 2);
-  const int64_t items = (int64_t)a.s.T * (wide ? (a.q.H + n - 1) / n : a.q.H);
-  const int per = wide ? 256 / norm_lanes(a.s.d) : kAnyWarps;
-  const int64_t need = (items + per - 1) / per, most = (int64_t)sm_count() * (wide ? 2 : 4);
+static int norm_bwd_grid(const NormArgs& a, int form) {
+  const int n = norm_heads(a, a.q.H, 2), H = a.q.H;
+  const int64_t items = (int64_t)a.s.T * (form == 2 ? (H + n - 1) / n : form == 1 ? (H + kGatherHeads - 1) / kGatherHeads : H);
+  const int lanes = form == 2 ? norm_lanes(a.s.d) : a.s.d > 128 ? 32 : 16, per = form ? 256 / lanes : kAnyWarps;
+  const int64_t need = (items + per - 1) / per, most = (int64_t)sm_count() * (form ? 2 : 4);
   return (int)(need < most ? need : most);
 }
 
 template <typename T>
 static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
-  if (norm_wide(a, sizeof(T), false)) {
-    const int G = norm_lanes(a.s.d), H = a.q.H > a.k.H ? a.q.H : a.k.H, n = norm_heads(a, H, 4);
+  const int form = norm_form(a, sizeof(T), false);
+  if (form) {
+    const int G = form == 2 ? norm_lanes(a.s.d) : a.s.d > 128 ? 32 : 16, H = a.q.H > a.k.H ? a.q.H : a.k.H;
+    const int n = form == 2 ? norm_heads(a, H, 4) : kGatherHeads;
     const int qs = a.q.H ? (a.q.H + n - 1) / n : 1, ks = a.k.H ? (a.k.H + n - 1) / n : 1;
     const int64_t items = (int64_t)a.s.T * (qs > ks ? qs : ks);
     if (items > 0x7fffff00) return -10;
@@ -570,13 +825,20 @@ static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
     NormArgs b = a;
     if (a.q.H == 0) { b.q = a.k; b.k.H = 0; }
     const dim3 grid((unsigned)((items + 256 / G - 1) / (256 / G)), b.k.H ? 2 : 1);
-    const int s0 = a.q.H ? qs : ks;
+    const int s0 = a.q.H ? qs : ks, vl = norm_vec(a, sizeof(T), false);
+    if (form == 2) {
 #define LLMT_QK(L, I, N) \
   if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_fwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(b, s0, ks);
 #define LLMT_QK3(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2) LLMT_QK(L, I, 4)
-    LLMT_QK3(32, true) LLMT_QK3(32, false) LLMT_QK3(16, true) LLMT_QK3(16, false) LLMT_QK3(8, true) LLMT_QK3(8, false)
+      LLMT_QK3(32, true) LLMT_QK3(32, false) LLMT_QK3(16, true) LLMT_QK3(16, false) LLMT_QK3(8, true) LLMT_QK3(8, false)
 #undef LLMT_QK3
 #undef LLMT_QK
+    } else {
+#define LLMT_QK(L, N) if (G == L && vl == N) qk_norm_rope_gather_fwd_kernel<T, L, N><<<grid, 256, 0, stream>>>(b, s0, ks);
+      if constexpr (sizeof(T) == 2) { LLMT_QK(32, 8) LLMT_QK(16, 8) }
+      LLMT_QK(32, 4) LLMT_QK(16, 4) LLMT_QK(32, 2) LLMT_QK(16, 2) LLMT_QK(32, 1) LLMT_QK(16, 1)
+#undef LLMT_QK
+    }
   } else {
     const int64_t items = (int64_t)a.s.T * (a.q.H + a.k.H), need = (items + kAnyWarps - 1) / kAnyWarps;
     const int64_t most = (int64_t)sm_count() * 64;
@@ -586,18 +848,25 @@ static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
 }
 template <typename T>
 static int norm_bwd(const NormArgs& a, int P, void* dw, cudaStream_t stream) {
-  const bool wide = norm_wide(a, sizeof(T), true);
-  const int grid = norm_bwd_grid(a, wide);
+  const int form = norm_form(a, sizeof(T), true), grid = norm_bwd_grid(a, form);
   if (a.partial != nullptr && grid > P) return -10;
-  if (wide) {
-    const int G = norm_lanes(a.s.d), n = norm_heads(a, a.q.H, 2), shares = (a.q.H + n - 1) / n;
+  if (form) {
+    const int G = form == 2 ? norm_lanes(a.s.d) : a.s.d > 128 ? 32 : 16;
+    const int n = form == 2 ? norm_heads(a, a.q.H, 2) : kGatherHeads, shares = (a.q.H + n - 1) / n, vl = norm_vec(a, sizeof(T), true);
     if ((int64_t)a.s.T * shares > 0x7fffff00) return -10;
+    if (form == 2) {
 #define LLMT_QK(L, I, N) \
   if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_bwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(a, shares);
 #define LLMT_QK2(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2)
-    LLMT_QK2(32, true) LLMT_QK2(32, false) LLMT_QK2(16, true) LLMT_QK2(16, false) LLMT_QK2(8, true) LLMT_QK2(8, false)
+      LLMT_QK2(32, true) LLMT_QK2(32, false) LLMT_QK2(16, true) LLMT_QK2(16, false) LLMT_QK2(8, true) LLMT_QK2(8, false)
 #undef LLMT_QK2
 #undef LLMT_QK
+    } else {
+#define LLMT_QK(L, N) if (G == L && vl == N) qk_norm_rope_gather_bwd_kernel<T, L, N><<<grid, 256, 0, stream>>>(a, shares);
+      if constexpr (sizeof(T) == 2) { LLMT_QK(32, 8) LLMT_QK(16, 8) }
+      LLMT_QK(32, 4) LLMT_QK(16, 4) LLMT_QK(32, 2) LLMT_QK(16, 2) LLMT_QK(32, 1) LLMT_QK(16, 1)
+#undef LLMT_QK
+    }
   } else {
     qk_norm_rope_any_kernel<T, true><<<grid, 32 * kAnyWarps, kAnyWarps * 2 * a.s.d * sizeof(float), stream>>>(a);
   }
@@ -637,7 +906,7 @@ __device__ __forceinline__ void angle_tables(double p, double quarter, float fac
 }
 // A thread keeps the frequencies of its V columns and walks over rows.
 template <bool VEC>
-__global__ void __launch_bounds__(256) rope_tables_kernel(const int64_t* __restrict__ pos, const __grid_constant__ Freqs f, float factor,
+__global__ void __launch_bounds__(256, 6) rope_tables_kernel(const int64_t* __restrict__ pos, const __grid_constant__ Freqs f, float factor,
                                                           float* __restrict__ cosb, float* __restrict__ sinb, int64_t T, int P) {
   constexpr int V = VEC ? 4 : 1;
   const int per_row = P / V, rows = 256 / per_row;      // at most 256 columns: a row fits a block
@@ -706,8 +975,12 @@ extern "C" int llmt_qk_norm_rope_part_fwd(const LlmtRopeShape* sh, const LlmtHea
 extern "C" int llmt_qk_norm_rope_part_partials(int T, int H, int d) {
   NormArgs a{};
   a.s.T = T; a.s.d = d; a.q.H = H;
-  const int w = norm_bwd_grid(a, true), n = norm_bwd_grid(a, false);
-  return w > n ? w : n;
+  int most = 0;
+  for (int form = 0; form < 3; ++form) {
+    const int g = norm_bwd_grid(a, form);
+    most = g > most ? g : most;
+  }
+  return most;
 }
 extern "C" int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* sh, const LlmtHeads* x, float eps, float shift, float* partial, int P, void* dw, int f32,
                                           cudaStream_t stream) {
@@ -723,7 +996,7 @@ extern "C" int llmt_rope_tables(const int64_t* pos, const double* inv, int P, do
   for (int j = 0; j < P; ++j) f.quarter[j] = inv[j] * 2.0 / 3.14159265358979323846;
   const bool vec = P % 4 == 0 && !((reinterpret_cast<uintptr_t>(cosb) | reinterpret_cast<uintptr_t>(sinb)) & 15);
   const int rows = 256 / (vec ? P / 4 : P);
-  const int64_t need = (T + rows - 1) / rows, most = (int64_t)sm_count() * 8;
+  const int64_t need = (T + rows - 1) / rows, most = (int64_t)sm_count() * 6;
   const int grid = (int)(need < most ? need : most);
   if (vec) rope_tables_kernel<true><<<grid, 256, 0, stream>>>(pos, f, (float)factor, cosb, sinb, T, P);
   else rope_tables_kernel<false><<<grid, 256, 0, stream>>>(pos, f, (float)factor, cosb, sinb, T, P);
