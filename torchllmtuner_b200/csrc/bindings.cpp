@@ -1385,7 +1385,9 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
                              (int)N, (int)K, x2.stride(0), w2.stride(0), N, r2.defined() ? r2.stride(0) : 0, pre.defined() ? pre.stride(0) : 0,
                              ws_ptr(ws), ws_size(ws), status_ptr(), cur_stream()),
              "llmt_linear_act", ws.defined() ? 2 : 1);
-    ctx->save_for_backward({x, w, b.has_value() ? *b : Tensor(), pre});
+    // rows that were copied for TMA are kept, so that the backward does not copy them again
+    const Tensor kx = x2.data_ptr() != x.data_ptr() ? x2 : Tensor(), kw = w2.data_ptr() != w.data_ptr() ? w2 : Tensor();
+    ctx->save_for_backward({x, w, b.has_value() ? *b : Tensor(), pre, keep ? kx : Tensor(), keep ? kw : Tensor()});
     ctx->saved_data["act"] = act;
     ctx->saved_data["residual"] = r.has_value();
     return y;
@@ -1418,7 +1420,8 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     }
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t N = w.size(0), K = w.size(1);
-    Tensor x2 = tma_rows(rows_2d(x)), w2 = tma_rows(w.stride(1) == 1 ? w : w.contiguous()), dy = rows_2d(d[0]);
+    Tensor x2 = s[4].defined() ? s[4] : tma_rows(rows_2d(x)), w2 = s[5].defined() ? s[5] : tma_rows(w.stride(1) == 1 ? w : w.contiguous()),
+           dy = rows_2d(d[0]);
     const int64_t M = x2.size(0);
     if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
     const bool tma_ok = dy.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;

@@ -484,81 +484,76 @@ __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __gr
 }
 
 // ------------------------------------------------------------------------------------------ dz and db
-// A block owns a strip of LANES * V columns and every blocks-th group of rows, and sums its columns in a fixed order. Few rows (CLUSTER): the eight
+// A block owns a strip of LANES * 8 columns and every blocks-th group of rows, and sums its columns in a fixed order. Few rows (CLUSTER): the eight
 // blocks of a strip are a cluster and add their sums through distributed shared memory in rank order, so db needs no second launch. Many rows:
 // sums per block go to partial [blocks][N] and linear_db_kernel adds them; clusters of eight would leave SMs idle then (a GPC's 16 or 18 SMs hold
 // two of them: half of the machine's time at 16384 x 4608).
 constexpr int kStripBlocks = 8;
-template <int V, int LANES, bool CLUSTER, int ACT>
-__global__ void __launch_bounds__(256, ACT == kActNone ? 4 : 3) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy, const __nv_bfloat16* __restrict__ z,
-                                                           int64_t ldz, __nv_bfloat16* __restrict__ dz, int64_t lddz, void* __restrict__ db, int db_f32,
-                                                           float* __restrict__ partial, int M, int N) {
-  constexpr int COLS = LANES * V, ROWS = 256 / LANES;
+// z and dz have rows on 16 bytes (the caller's buffers); dy may lie anywhere (VEC false): then its values are read one by one.
+template <bool VEC, int LANES, bool CLUSTER, int ACT>
+__global__ void __launch_bounds__(256, ACT == kActNone ? 4 : 3) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy,
+                                                                                const __nv_bfloat16* __restrict__ z, int64_t ldz,
+                                                                                __nv_bfloat16* __restrict__ dz, int64_t lddz, void* __restrict__ db,
+                                                                                int db_f32, float* __restrict__ partial, int M, int N) {
+  constexpr int V = 8, COLS = LANES * V, ROWS = 256 / LANES;
   __shared__ float part[ROWS][COLS + 4];
   __shared__ float total[CLUSTER ? COLS : 1];
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const int col = blockIdx.x * COLS + lane * V;
-  constexpr int W = V > 1 ? V / 2 : 1;                   // pairs; a single column takes two rows as a pair instead
+  constexpr int W = V / 2;
   float2 acc[W];
 #pragma unroll
   for (int j = 0; j < W; ++j) acc[j] = make_float2(0.f, 0.f);
   if (col < N) {
-    constexpr int U = V > 1 ? 4 : 8;                     // rows in flight per thread
+    constexpr int U = VEC ? 4 : 2;                       // rows in flight per thread
     const int64_t step = (int64_t)ROWS * gridDim.y;
     for (int64_t row = (int64_t)blockIdx.y * ROWS + sub; row < M; row += U * step) {
-      Raw<__nv_bfloat16, V> rg[U], rz[U];
+      Raw<__nv_bfloat16, V> rg[VEC ? U : 1], rz[U];
+      float gs[VEC ? 1 : U][V];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        rg[u].zero();
         rz[u].zero();
+        if constexpr (VEC) rg[u].zero();
+        else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) gs[u][j] = 0.f;
+        }
         if (row + u * step < M) {
-          rg[u].load(dy + (row + u * step) * ldy + col);
+          if constexpr (VEC) rg[u].load(dy + (row + u * step) * ldy + col);
+          else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+              if (col + j < N) load_vec<__nv_bfloat16, 1>(dy + (row + u * step) * ldy + col + j, &gs[u][j]);
+          }
           if (ACT != kActNone) rz[u].load(z + (row + u * step) * ldz + col);
         }
       }
-      if constexpr (V > 1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float g[V], p[V], out[V];
-          rg[u].get(g);
-          if (ACT != kActNone) rz[u].get(p);
+      for (int u = 0; u < U; ++u) {
+        float g[V], p[V], out[V];
+        if constexpr (VEC) rg[u].get(g);
+        if (ACT != kActNone) rz[u].get(p);
 #pragma unroll
-          for (int j = 0; j < W; ++j) {
-            float2 v = make_float2(g[2 * j], g[2 * j + 1]);
-            if (ACT != kActNone) v = activate_grad<ACT>(make_float2(p[2 * j], p[2 * j + 1]), v);
-            acc[j] = add2(acc[j], v);                    // rows past the end were loaded as zeros: their gradient is zero
-            out[2 * j] = v.x;
-            out[2 * j + 1] = v.y;
+        for (int j = 0; j < W; ++j) {
+          float2 v = VEC ? make_float2(g[2 * j], g[2 * j + 1]) : make_float2(gs[VEC ? 0 : u][2 * j], gs[VEC ? 0 : u][2 * j + 1]);
+          if (ACT != kActNone) {
+            v = activate_grad<ACT>(make_float2(p[2 * j], p[2 * j + 1]), v);
+            if (!VEC && col + 2 * j >= N) v.x = 0.f;     // behind the last column z was never written
+            if (!VEC && col + 2 * j + 1 >= N) v.y = 0.f;
           }
-          if (dz != nullptr && row + u * step < M) store_vec<__nv_bfloat16, V>(dz + (row + u * step) * lddz + col, out);
+          acc[j] = add2(acc[j], v);                      // rows past the end were loaded as zeros: their gradient is zero
+          out[2 * j] = v.x;
+          out[2 * j + 1] = v.y;
         }
-      } else {
-#pragma unroll
-        for (int u = 0; u < U; u += 2) {
-          float2 v, p;
-          rg[u].get(&v.x);
-          rg[u + 1].get(&v.y);
-          rz[u].get(&p.x);
-          rz[u + 1].get(&p.y);
-          if (ACT != kActNone) v = activate_grad<ACT>(p, v);
-          acc[0] = add2(acc[0], v);
-          if (dz != nullptr) {
-            if (row + u * step < M) dz[(row + u * step) * lddz + col] = __float2bfloat16_rn(v.x);
-            if (row + (u + 1) * step < M) dz[(row + (u + 1) * step) * lddz + col] = __float2bfloat16_rn(v.y);
-          }
-        }
+        if (dz != nullptr && row + u * step < M) store_vec<__nv_bfloat16, V>(dz + (row + u * step) * lddz + col, out);
       }
     }
   }
   if (db == nullptr) return;
-  if constexpr (V > 1) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      part[sub][lane * V + 2 * j] = acc[j].x;
-      part[sub][lane * V + 2 * j + 1] = acc[j].y;
-    }
-  } else {
-    part[sub][lane] = acc[0].x + acc[0].y;
+  for (int j = 0; j < W; ++j) {
+    part[sub][lane * V + 2 * j] = acc[j].x;
+    part[sub][lane * V + 2 * j + 1] = acc[j].y;
   }
   __syncthreads();
   const int oc = blockIdx.x * COLS + threadIdx.x;
@@ -801,10 +796,10 @@ static int dz_blocks(int M, int N) {
   return fill < 1 ? 1 : fill < rows ? fill : rows;
 }
 
-template <int V, int LANES, bool CLUSTER, int ACT>
+template <bool VEC, int LANES, bool CLUSTER, int ACT>
 static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int db_f32, float* partial, int blocks,
                      int M, int N, cudaStream_t stream) {
-  constexpr int COLS = LANES * V;
+  constexpr int COLS = LANES * 8;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((N + COLS - 1) / COLS, blocks);
   cfg.blockDim = dim3(256);
@@ -815,17 +810,17 @@ static int dz_launch(const void* dy, int64_t ldy, const void* z, int64_t ldz, vo
   cfg.attrs = &at;
   cfg.numAttrs = CLUSTER ? 1 : 0;
   using B = __nv_bfloat16;
-  return cudaLaunchKernelEx(&cfg, linear_dz_kernel<V, LANES, CLUSTER, ACT>, reinterpret_cast<const B*>(dy), ldy, reinterpret_cast<const B*>(z), ldz,
+  return cudaLaunchKernelEx(&cfg, linear_dz_kernel<VEC, LANES, CLUSTER, ACT>, reinterpret_cast<const B*>(dy), ldy, reinterpret_cast<const B*>(z), ldz,
                             reinterpret_cast<B*>(dz), lddz, db, db_f32, partial, M, N) == cudaSuccess ? 0 : -3;
 }
 template <int ACT>
 static int dz_dispatch(bool vec, int blocks, const void* dy, int64_t ldy, const void* z, int64_t ldz, void* dz, int64_t lddz, void* db, int db_f32,
                        float* partial, int M, int N, cudaStream_t stream) {
   if (blocks == 0)
-    return vec ? dz_launch<8, 8, true, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, nullptr, kStripBlocks, M, N, stream)
-               : dz_launch<1, 32, true, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, nullptr, kStripBlocks, M, N, stream);
-  return vec ? dz_launch<8, 32, false, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, blocks, M, N, stream)
-             : dz_launch<1, 32, false, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, blocks, M, N, stream);
+    return vec ? dz_launch<true, 8, true, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, nullptr, kStripBlocks, M, N, stream)
+               : dz_launch<false, 8, true, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, nullptr, kStripBlocks, M, N, stream);
+  return vec ? dz_launch<true, 32, false, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, blocks, M, N, stream)
+             : dz_launch<false, 32, false, ACT>(dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, blocks, M, N, stream);
 }
 
 }  // namespace llmt
@@ -870,14 +865,18 @@ extern "C" int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, in
 }
 // Rows of `partial` ([rows][N] floats) that llmt_linear_dz needs for db; 0: none.
 extern "C" int llmt_linear_db_partials(int M, int N) { return dz_blocks(M, N); }
-// dz = dy act'(z) (act 0: dz = dy; dz nullptr: not written), db = column sums of dz in fp32 before rounding (nullptr: not computed).
+// dz = dy act'(z) (act 0: dz = dy; dz nullptr: not written), db = column sums of dz in fp32 before rounding (nullptr: not computed). z and dz have
+// rows on 16 bytes of at least N values rounded up to a multiple of 8.
 extern "C" int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32,
                               float* partial, int P, int M, int N, cudaStream_t stream) {
   if (M < 0 || N <= 0 || act < 0 || act >= kActKinds || (act != 0 && z == nullptr)) return -10;
   const int blocks = dz_blocks(M, N);
   if (db != nullptr && blocks > 0 && (partial == nullptr || P < blocks)) return -10;
   auto at16 = [](const void* p, int64_t ld) { return p == nullptr || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % 8 == 0); };
-  const bool vec = N % 8 == 0 && at16(dy, ldy) && at16(act ? z : nullptr, ldz) && at16(dz, lddz);
+  const int64_t N8 = (N + 7) / 8 * 8;
+  if (act && (!at16(z, ldz) || ldz < N8)) return -10;
+  if (dz != nullptr && (!at16(dz, lddz) || lddz < N8)) return -10;
+  const bool vec = N % 8 == 0 && at16(dy, ldy);
   int rc = -4;
 #define LLMT_DZ(ACT) \
   if (act == ACT) rc = dz_dispatch<ACT>(vec, blocks, dy, ldy, z, ldz, dz, lddz, db, db_f32, partial, M, N, stream);
