@@ -24,7 +24,8 @@ constexpr int kLMaxStages = 8;
 constexpr int kLStageA = kLM * kLK * 2;
 constexpr int kLSmem = 227 * 1024;
 constexpr int kLStage = 4096 + 256;        // per epilogue warp: 32 rows of 128 bytes, 64 bias values
-constexpr int kLSmemFixed = kLEpiWarps * kLStage + 1024 /*alignment*/ + 512 /*barriers*/;
+constexpr int kLSlack = 512;              // for the 1024-byte alignment of the stages; dynamic shared memory starts on 1024 bytes (checked)
+constexpr int kLSmemFixed = kLEpiWarps * kLStage + kLSlack + 512 /*barriers*/;      // leaves four stages of 128 x 256 tiles to the byte
 constexpr int kMaxWorkers = 160;
 
 // What becomes of a product: stored as it is, or (`fwd`) with bias, activation and residual.
@@ -235,6 +236,10 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
                                                               const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ LinArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (smem - smem_raw > kLSlack) {                       // the same in every block: none goes on
+    if (threadIdx.x == 0) report_status(a.status, kStatusBadArgument, 900, (int)(smem - smem_raw));
+    return;
+  }
   const LinPlan& plan = a.plan;
   const int stages = plan.stages, stage_bytes = plan.stage_bytes;
   uint8_t* epi = smem + stages * stage_bytes;
@@ -650,7 +655,7 @@ static int64_t lin_ws_floats(int M, int N, const LinCut& c) {
 // with every SM at it the operands, which come from L2 at 10 to 13 TB/s: 256 columns 420, 192 360, 128 260 (16384 x 4608 x 1152). `loaded`: columns
 // that the TMA boxes fetch, more than `bn` where B is stored [K][N] and half a tile is no multiple of 64.
 static double lin_kb_ns(int bn, int loaded, double busy) {
-  const double alone = bn * 1.18 > 200 ? bn * 1.18 : 200, crowded = 90 + 0.65 * (bn + loaded);
+  const double alone = bn * 1.18 > 200 ? bn * 1.18 : 200, crowded = 120 + 0.6 * (bn + loaded);
   return crowded > alone ? alone + (crowded - alone) * busy : alone;
 }
 // Units of whole tiles go round the workers; those of narrow tiles go one by one to the worker that is free first.
@@ -676,11 +681,11 @@ static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb,
   const int most = sm_count() / cg, full_n = N / bn, rest = N - full_n * bn, whole = num_m * full_n * splits, narrow = rest ? num_m * splits : 0;
   const int workers = whole + narrow < most ? whole + narrow : most;
   const double depth = (double)((kb + splits - 1) / splits);
-  const int loaded = b_mn ? (bn + 64 * cg - 1) / (64 * cg) * 64 * cg : bn;
   // a tile is not done before its sums are drained: about 0.9 us per 128 columns, hidden under the next tile's products where there are two
-  // accumulators
+  // accumulators; 0.5 us pass between two tiles
   auto unit = [&](int w, int running) {
-    const double drain = 0.9 * w / 128, mma = depth * lin_kb_ns(w, loaded, (double)running * cg / sm_count()) * 1e-3;
+    const int loaded = b_mn ? (w + 64 * cg - 1) / (64 * cg) * 64 * cg : w;
+    const double drain = 0.9 * w / 128, mma = 0.5 + depth * lin_kb_ns(w, loaded, (double)running * cg / sm_count()) * 1e-3;
     return bn > 256 ? mma + drain : mma > drain ? mma : drain;
   };
   const int rounds = whole / workers, ahead = whole % workers, behind = ahead ? workers - ahead : 0;
