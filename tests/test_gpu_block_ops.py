@@ -558,3 +558,79 @@ def test_residual_broadcast_over_columns():
     g, = torch.autograd.grad(y, r, dy)
     ref = dy.double().sum(1, keepdim=True)
     _near(g, ref, _u(torch.bfloat16) * ref.abs() + 32 * E32 * dy.double().abs().sum(1, keepdim=True), "dr")
+
+
+# ------------------------------------------------------------------------------------------------------ a run of them
+def _tower_block(kind):
+    from torchllmtuner_b200.models import moonvit, qwen_vit
+    cfg = dict(hidden_size=288, intermediate_size=520, num_heads=4)                      # heads of 72
+    return (qwen_vit.QwenViTBlock(qwen_vit.QwenViTConfig(**cfg)) if kind == "qwen" else moonvit.MoonViTBlock(moonvit.MoonViTConfig(**cfg)))
+
+
+@pytest.mark.parametrize("kind", ["qwen", "moon"])
+def test_tower_block_against_its_fp32_statement(kind):
+    """LayerNorm -> packed projection with bias -> rotation -> attention -> projection + residual -> LayerNorm -> two-layer GELU MLP + residual, as the
+    towers call it, forward and every gradient. About 12 roundings to bf16 lie on a path forwards and as many again backwards, each off by at most
+    half a step: 12 and 24 times 2^-8 in the 2-norm."""
+    import copy
+
+    from torchllmtuner_b200.ops import AttnMeta
+    from torchllmtuner_b200.ops.cuda_ext import load
+    torch.manual_seed(3)
+    block = _tower_block(kind)
+    with torch.no_grad():
+        for name, p in block.named_parameters():
+            p.copy_(1 + 0.1 * torch.randn(p.shape) if "norm" in name and name.endswith("weight") else torch.randn(p.shape) * (0.1 if p.dim() == 1 else p.shape[-1] ** -0.5))
+    block = block.bfloat16()
+    plain = copy.deepcopy(block).float()
+    block = block.to(DEV)
+    x = torch.randn(300, 288).bfloat16()
+    dy = torch.randn(300, 288).bfloat16()
+    ang = torch.rand(300, 36) * 6
+    ang = torch.cat((ang, ang), -1) if kind == "qwen" else ang
+    cuts = torch.tensor([0, 77, 300])
+
+    def run(m, dev, dtype):
+        leaf = x.to(dev, dtype).requires_grad_()
+        y = m(leaf, ang.cos().to(dev), ang.sin().to(dev), AttnMeta.build(cuts, causal=False, device=dev if dev == DEV else None))
+        names = [n for n, _ in m.named_parameters()]
+        return {"y": y, **dict(zip(["x", *names], torch.autograd.grad(y, [leaf, *m.parameters()], dy.to(dev, dtype))))}
+    before = load().launch_count()
+    got = run(block, DEV, torch.bfloat16)
+    assert load().launch_count() - before >= 20
+    want = run(plain, "cpu", torch.float32)
+    for name, ref in want.items():
+        off = (got[name].detach().float().cpu() - ref.detach()).norm() / ref.detach().norm()
+        # the key's bias shifts every score of a query alike: its gradient is zero but for rounding, and shares a tensor with the queries' and values'
+        assert off <= (12 if name == "y" else 24) * 2.0 ** -8, (name, off.item())
+
+
+def test_gated_attention_against_its_fp32_statement():
+    """The gated attention of Qwen3.5: queries beside their gates, zero-centred norms and partial rotation in one pass; about 10 roundings each way."""
+    import copy
+
+    from torchllmtuner_b200.models.qwen3_5 import GatedFullAttention, Qwen35Config, Qwen35Context, mrope_tables
+    from torchllmtuner_b200.ops import AttnMeta
+    torch.manual_seed(4)
+    cfg = Qwen35Config(hidden_size=128, num_attention_heads=4, num_key_value_heads=2, head_dim=64, num_experts=0)
+    block = GatedFullAttention(cfg)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.copy_(torch.randn(p.shape) * (0.1 if p.dim() == 1 else p.shape[-1] ** -0.5))
+    block = block.bfloat16()
+    plain = copy.deepcopy(block).float()
+    block = block.to(DEV)
+    x, dy = torch.randn(150, 128).bfloat16(), torch.randn(150, 128).bfloat16()
+    cuts = torch.tensor([0, 61, 150])
+    pos = torch.cat((torch.arange(61), torch.arange(89)))
+
+    def run(m, dev, dtype):
+        cos, sin = mrope_tables(pos.to(dev), cfg.rotary_dim, cfg.rope_theta, cfg.mrope_section)
+        ctx = Qwen35Context(cos, sin, AttnMeta.build(cuts, causal=True, device=dev if dev == DEV else None), positions=pos.to(dev))
+        leaf = x.to(dev, dtype).requires_grad_()
+        y = m(leaf, ctx)
+        return {"y": y, **dict(zip(["x", *(n for n, _ in m.named_parameters())], torch.autograd.grad(y, [leaf, *m.parameters()], dy.to(dev, dtype))))}
+    got, want = run(block, DEV, torch.bfloat16), run(plain, "cpu", torch.float32)
+    for name, ref in want.items():
+        off = (got[name].detach().float().cpu() - ref.detach()).norm() / ref.detach().norm()
+        assert off <= (10 if name == "y" else 20) * 2.0 ** -8, (name, off.item())
