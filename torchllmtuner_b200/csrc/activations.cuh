@@ -24,6 +24,12 @@ __device__ __forceinline__ float rcp_of(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// v within [-limit, limit]; NaN stays.
+__device__ __forceinline__ float clamp_of(float v, float limit) {
+  float r;
+  asm("{ .reg .f32 t; min.NaN.f32 t, %1, %2; max.NaN.f32 %0, t, %3; }" : "=f"(r) : "f"(v), "f"(limit), "f"(-limit));
+  return r;
+}
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float2 exp2_of(float2 v) { return make_float2(exp2_of(v.x), exp2_of(v.y)); }
 __device__ __forceinline__ float2 rcp_of(float2 v) { return make_float2(rcp_of(v.x), rcp_of(v.y)); }
@@ -74,6 +80,7 @@ __device__ __forceinline__ float2 activate_grad(float2 z, float2 g) {
     return mul2(g, fma2(mul2(z, both(kInvSqrt2Pi)), e, cdf));
   }
   if constexpr (ACT == kActGeluTanh) {
+    z = make_float2(clamp_of(z.x, 100.f), clamp_of(z.y, 100.f));       // there act' is 0 or 1; u of a z beyond 1e12 would be inf, and 0 inf NaN
     const float2 z2 = mul2(z, z), s = gelu_sigmoid(z, z2), u = mul2(z, fma2(z2, both(6.f * kSqrt2OverPi * kGeluCubic), both(2.f * kSqrt2OverPi)));
     return mul2(g, fma2(fma2(mul2(s, both(-1.f)), s, s), u, s));
   }

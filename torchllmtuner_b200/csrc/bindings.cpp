@@ -1349,8 +1349,8 @@ Tensor tma_rows(const Tensor& t) {
   return r;
 }
 // Partial sums of a product that is cut along its depth; of this call alone, so graphs and streams share nothing.
-Tensor linear_workspace(int64_t M, int64_t N, int64_t K, bool gradient, const Tensor& like) {
-  const int64_t n = llmt_linear_ws_floats((int)M, (int)N, (int)K, gradient);
+Tensor linear_workspace(int64_t M, int64_t N, int64_t K, bool gradient, int64_t act, bool res, bool pre, const Tensor& like) {
+  const int64_t n = llmt_linear_ws_floats((int)M, (int)N, (int)K, gradient, (int)act, res, pre);
   return n > 0 ? fresh({n}, at::kFloat, like) : Tensor();
 }
 inline float* ws_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
@@ -1379,7 +1379,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
       if (M > 1 && r2.stride(0) < N && r2.stride(0) != 0) r2 = r2.contiguous();
     }
     if (act != 0 && keep) pre = fresh({M, (N + 7) / 8 * 8}, at::kBFloat16, x);
-    const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), false, x);
+    const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), false, act, r2.defined(), pre.defined(), x);
     check_rc(llmt_linear_act(x2.data_ptr(), w2.data_ptr(), y.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, bc.defined() && is_f32(bc),
                              r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, (int)M,
                              (int)N, (int)K, x2.stride(0), w2.stride(0), N, r2.defined() ? r2.stride(0) : 0, pre.defined() ? pre.stride(0) : 0,
@@ -1453,14 +1453,14 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     const int64_t lddz = dz.stride(0);
     if (nx) {
       out[0] = fresh(x.sizes(), at::kBFloat16, x);
-      const Tensor ws = linear_workspace(M, K, N, true, dz);
+      const Tensor ws = linear_workspace(M, K, N, true, 0, false, false, dz);
       check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),
                "llmt_linear_dx", ws.defined() ? 2 : 1);
     }
     if (nw) {
       out[1] = fresh(w.sizes(), at::kBFloat16, x);
-      const Tensor ws = linear_workspace(N, K, M, true, dz);
+      const Tensor ws = linear_workspace(N, K, M, true, 0, false, false, dz);
       check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),
                "llmt_linear_dw", ws.defined() ? 2 : 1);

@@ -51,7 +51,7 @@ struct LinPlan {
   int bn, num_m, full_n, splits, kb;
   int stages, stage_bytes, b2_offset, workers;      // b2_offset: of the second MMA's columns of B in a stage
   float* ws;                             // splits > 1: [splits][tiles][rows / 32][bn / 4][32][4] partial sums
-  uint16_t narrow_begin[kMaxWorkers + 1];
+  int narrow_begin[kMaxWorkers + 1];
 };
 struct LinArgs {
   LinOut out;
@@ -670,22 +670,29 @@ static void lin_plan(LinPlan& p, int N, int num_tiles_m, int most) {
   const int catch_up = narrow < behind * fit ? narrow : behind * fit, left = narrow - catch_up;
   int at = 0;
   for (int w = 0; w < p.workers; ++w) {
-    p.narrow_begin[w] = (uint16_t)at;
+    p.narrow_begin[w] = at;
     if (w >= ahead && behind) at += catch_up / behind + (w - ahead < catch_up % behind ? 1 : 0);
     at += left / p.workers + (w < left % p.workers ? 1 : 0);
   }
-  p.narrow_begin[p.workers] = (uint16_t)at;
+  p.narrow_begin[p.workers] = at;
+}
+// What an epilogue adds to the time in which two warps drain 32 rows of 128 columns, in tenths of a us: 9 for the sums alone, and what activation,
+// residual and z add (16384 x 1152 -> 4608 on tiles of 512 columns, whose drain nothing hides: 112 us plain, relu 120, silu 137, gelu_tanh 145, gelu
+// 154, and z another 22 to 24).
+static int lin_drain(int act, bool res, bool pre) {
+  const int cost[kActKinds] = {0, 13, 10, 8, 3};         // in the order of ActKind
+  return 9 + cost[act] + (res ? 3 : 0) + (act != kActNone && pre ? 8 : 0);
 }
 // The longest worker's units, in us (kb deep, `splits` parts).
-static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb, bool b_mn) {
+static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb, bool b_mn, int tenths) {
   const int most = sm_count() / cg, full_n = N / bn, rest = N - full_n * bn, whole = num_m * full_n * splits, narrow = rest ? num_m * splits : 0;
   const int workers = whole + narrow < most ? whole + narrow : most;
   const double depth = (double)((kb + splits - 1) / splits);
-  // a tile is not done before its sums are drained: about 0.9 us per 128 columns, hidden under the next tile's products where there are two
+  // a tile is not done before its sums are drained: see lin_drain, hidden under the next tile's products where there are two
   // accumulators; 0.5 us pass between two tiles
   auto unit = [&](int w, int running) {
     const int loaded = b_mn ? (w + 64 * cg - 1) / (64 * cg) * 64 * cg : w;
-    const double drain = 0.9 * w / 128, mma = 0.5 + depth * lin_kb_ns(w, loaded, (double)running * cg / sm_count()) * 1e-3;
+    const double drain = 0.1 * tenths * w / 128, mma = 0.5 + depth * lin_kb_ns(w, loaded, (double)running * cg / sm_count()) * 1e-3;
     return bn > 256 ? mma + drain : mma > drain ? mma : drain;
   };
   const int rounds = whole / workers, ahead = whole % workers, behind = ahead ? workers - ahead : 0;
@@ -695,13 +702,13 @@ static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb,
     const int fit = full_n ? (int)(unit(bn, workers) / tn + 0.1) : 0, left = narrow - (narrow < behind * fit ? narrow : behind * fit);
     t += tn * ((left + workers - 1) / workers);
   }
-  return t + (bn > 256 ? 0 : 0.9 * (full_n ? bn : rest) / 128);
+  return t + (bn > 256 ? 0 : 0.1 * tenths * (full_n ? bn : rest) / 128);
 }
 
 // How a product is cut: CTAs per tile, tile width and parts along K. The shortest of the candidates by the estimate: tile widths that divide N
 // evenly into 1, 2, ... columns of tiles, one CTA or a pair, and parts along K where the tiles leave workers idle. The parts cost a second
 // launch and their sums in memory: 5.5 us and 4 bytes per sum and part at 4 TB/s (1152 x 1152 in 3 parts: 8.0 us).
-static LinCut lin_find_cut(int M, int N, int K, bool b_mn) {
+static LinCut lin_find_cut(int M, int N, int K, bool b_mn, int drain) {
   const int kb = (K + kLK - 1) / kLK;
   LinCut best{1, 128, 1};
   double least = 1e30;
@@ -709,15 +716,14 @@ static LinCut lin_find_cut(int M, int N, int K, bool b_mn) {
     const int num_m = (M + kLM * cg - 1) / (kLM * cg), most = sm_count() / cg;
     const int widest = cg == 2 ? 512 : 256;              // at least four stages of operands fit shared memory
     int last = 0;
-    if (num_m > 65535) continue;
     for (int n = (N + widest - 1) / widest; n <= (N + 127) / 128; ++n) {
       const int bn = ((N + n - 1) / n + 31) / 32 * 32;
       if (bn == last) continue;
       last = bn;
       const int tiles = num_m * ((N + bn - 1) / bn);
       for (int splits = 1; splits == 1 || (splits <= 8 && splits * 2 <= kb); ++splits) {
-        if (splits > 1 && (bn % 64 || tiles * (splits - 1) >= 2 * most || (int64_t)num_m * splits > 65535)) break;
-        double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, b_mn);
+        if (splits > 1 && (bn % 64 || tiles * (splits - 1) >= 2 * most)) break;
+        double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, b_mn, splits > 1 ? lin_drain(0, false, false) : drain);
         if (cg == 1) t *= 1.08;                          // a single CTA reads 1.5 times the operands per product
         if (splits > 1) t += 5.5 + 4e-6 * splits * (double)M * N / 4.0;
         if (t < least) {
@@ -730,11 +736,12 @@ static LinCut lin_find_cut(int M, int N, int K, bool b_mn) {
   return best;
 }
 // The cut of a size is found once per thread and place in a small table (it takes the host some 10 us).
-static LinCut lin_cut(int M, int N, int K, bool b_mn) {
-  struct Found { int M, N, K, b_mn; LinCut cut; };
+static LinCut lin_cut(int M, int N, int K, bool b_mn, int drain) {
+  struct Found { int M, N, K, kind; LinCut cut; };
   static thread_local Found table[64];
-  Found& f = table[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 9176u ^ (unsigned)b_mn) >> 7 & 63];
-  if (f.M != M || f.N != N || f.K != K || f.b_mn != (int)b_mn) f = Found{M, N, K, b_mn, lin_find_cut(M, N, K, b_mn)};
+  const int kind = drain * 2 + b_mn;
+  Found& f = table[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 9176u ^ (unsigned)kind * 97u) >> 7 & 63];
+  if (f.M != M || f.N != N || f.K != K || f.kind != kind) f = Found{M, N, K, kind, lin_find_cut(M, N, K, b_mn, drain)};
   return f.cut;
 }
 
@@ -744,14 +751,14 @@ static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda,
   LinOut& o = a.out;
   if (o.M <= 0 || o.N <= 0) return 0;
   if (K <= 0 || (lda & 7) || (ldb & 7) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return -10;
-  const LinCut cut = lin_cut(o.M, o.N, K, b_mn);
+  const LinCut cut = lin_cut(o.M, o.N, K, b_mn, lin_drain(fwd ? act : 0, o.res != nullptr, o.pre != nullptr));
   if (lin_ws_floats(o.M, o.N, cut) > (ws == nullptr ? 0 : ws_floats) || sm_count() / cut.cg > kMaxWorkers) return -10;
   LinPlan& p = a.plan;
   p.bn = cut.bn;
   p.splits = cut.splits;
   p.ws = ws;
   p.kb = (K + kLK - 1) / kLK;
-  if (p.splits > p.kb || (int64_t)((o.M + kLM * cut.cg - 1) / (kLM * cut.cg)) * p.splits > 65535) return -10;
+  if (p.splits > p.kb) return -10;
   lin_plan(p, o.N, (o.M + kLM * cut.cg - 1) / (kLM * cut.cg), sm_count() / cut.cg);
   const int first = p.bn < 256 ? p.bn : 256, b_rows = first / cut.cg, b2_rows = (p.bn - first) / cut.cg;
   auto rows = [&](int r) { return (b_mn ? (r + 63) / 64 * 64 : r) * kLK * 2; };        // column blocks of 64 where B is stored [K][N]
@@ -832,8 +839,12 @@ static int dz_dispatch(bool vec, int blocks, const void* dy, int64_t ldy, const 
 
 using namespace llmt;
 
-// Workspace of a product out [M, N] of depth K, in floats (0: none is needed). `gradient`: of llmt_linear_dx or llmt_linear_dw.
-extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int gradient) { return lin_ws_floats(M, N, lin_cut(M, N, K, gradient != 0)); }
+// Workspace of a product out [M, N] of depth K, in floats (0: none is needed): of llmt_linear_dx or llmt_linear_dw (`gradient`; act, res and pre 0),
+// or of llmt_linear_act with that activation, with a residual (`res`) and with z (`pre`).
+extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int gradient, int act, int res, int pre) {
+  if (act < 0 || act >= kActKinds) return 0;             // refused by the launch
+  return lin_ws_floats(M, N, lin_cut(M, N, K, gradient != 0, lin_drain(act, res != 0, pre != 0)));
+}
 
 // y [M, N] = act(x [M, K] W [N, K]^T + bias) + res; pre (optional, read by llmt_linear_dz) receives x W^T + bias where there is an activation.
 extern "C" int llmt_linear_act(const void* x, const void* w, void* y, const void* bias, int bias_f32, const void* res, void* pre, int act, int M, int N,
