@@ -2,7 +2,7 @@
 // MLPs and mergers of llmtuner/models/qwen/qwen3_5/multimodal.py:47-290 and llmtuner/models/kimi/kimi_k3/multimodal.py:146-914).
 //   z = x W^T + b,  y = act(z) + r;   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum_rows dz,  dr = dy.
 //
-// The products run on tcgen05 with the roles of gemm.cu: one warp issues TMA loads, one the products, eight drain the accumulator; persistent
+// The products run on tcgen05 with the roles of gemm.cu: one warp issues TMA loads, one the products, sixteen drain the accumulator; persistent
 // workers, each one CTA (128-row tiles) or a pair of CTAs (256-row tiles, cta_group::2). The epilogue of the forward adds the bias, applies the
 // activation and adds the residual in fp32 and rounds once; for the backward it also writes z (rounded to bf16: act' of the rounded z is off by
 // at most |act''| |z| 2^-9, of the order of the rounding of dz itself). The bias gradient is summed in fp32 from dz before it is rounded.
@@ -18,12 +18,13 @@ int make_tmap_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t*
 
 constexpr int kLM = 128;                 // rows of a CTA's tile
 constexpr int kLK = 64;                  // 64 bf16: one 128-byte swizzle row
-constexpr int kLEpiWarps = 8;
+constexpr int kLEpiWarps = 16;
 constexpr int kLThreads = 64 + 32 * kLEpiWarps;
 constexpr int kLMaxStages = 8;
 constexpr int kLStageA = kLM * kLK * 2;
 constexpr int kLSmem = 227 * 1024;
-constexpr int kLStage = 4096 + 256;        // per epilogue warp: 32 rows of 128 bytes, 64 bias values
+constexpr int kLPatch = 2048;            // of an epilogue warp: 32 rows of 64 bytes
+constexpr int kLStage = kLPatch + 128;     // and 32 bias values
 constexpr int kLSlack = 512;              // for the 1024-byte alignment of the stages; dynamic shared memory starts on 1024 bytes (checked)
 constexpr int kLSmemFixed = kLEpiWarps * kLStage + kLSlack + 512 /*barriers*/;      // leaves four stages of 128 x 256 tiles to the byte
 constexpr int kMaxWorkers = 160;
@@ -98,136 +99,122 @@ struct LinWalk {
   }
 };
 
-// 32 rows x 64 columns of the residual into the warp's staging rows, asynchronously (wait_patch), 16 bytes per lane. Clamped instead of skipped where
-// the patch leaves the matrix. Chunks of 16 bytes are XORed with the row: no bank conflicts.
+// A warp's patch is 32 rows x 32 columns. In its staging buffer rows are 64 bytes; their 16-byte chunks are XORed with the row so that neither a lane
+// per row nor eight lanes over two rows meet a bank twice.
+__device__ __forceinline__ uint32_t patch_at(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
+// The residual's patch into the staging buffer. Rows on 16 bytes: asynchronously (wait_patch), clamped instead of skipped where the patch leaves the
+// matrix. Others: a lane per column.
 __device__ __forceinline__ void load_patch(uint8_t* stg, const LinOut& o, int row0, int col, int end, int lane) {
-  const int cc = lane & 7, c = col + cc * 8 < end ? col + cc * 8 : 0;
-  const __nv_bfloat16* p = o.res + c;
+  if (o.vec) {
+    const int cc = lane & 3, c = col + cc * 8 < end ? col + cc * 8 : 0;
+    const __nv_bfloat16* p = o.res + c;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int rr = it * 4 + (lane >> 3);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + rr * 128 + ((cc ^ (rr & 7)) << 4))),
-                 "l"(p + (int64_t)min(row0 + rr, o.M - 1) * o.ldres)
-                 : "memory");
+    for (int it = 0; it < 4; ++it) {
+      const int rr = it * 8 + (lane >> 2);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stg + patch_at(rr, cc))), "l"(p + (int64_t)min(row0 + rr, o.M - 1) * o.ldres)
+                   : "memory");
+    }
+    return;
   }
+  if (col + lane >= end) return;
+#pragma unroll 8
+  for (int rr = 0; rr < 32; ++rr)
+    *reinterpret_cast<__nv_bfloat16*>(stg + patch_at(rr, lane >> 3) + (lane & 7) * 2) = o.res[(int64_t)min(row0 + rr, o.M - 1) * o.ldres + col + lane];
 }
 __device__ __forceinline__ void wait_patch() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// The staging rows (64 bf16 each) of a warp, to global memory in whole 128-byte lines.
-__device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p, int64_t ld, int row0, int col, int M, int end, int lane) {
-  const int cc = lane & 7;
-  if (col + cc * 8 >= end) return;
+// The staging buffer's patch to global memory, along its rows.
+__device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p, int64_t ld, const LinOut& o, int row0, int col, int end, int lane) {
+  if (o.vec) {
+    const int cc = lane & 3;
+    if (col + cc * 8 >= end) return;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int rr = it * 4 + (lane >> 3);
-    const uint4 v = *reinterpret_cast<const uint4*>(stg + rr * 128 + ((cc ^ (rr & 7)) << 4));
-    if (row0 + rr < M) *reinterpret_cast<uint4*>(p + (int64_t)(row0 + rr) * ld + col + cc * 8) = v;
+    for (int it = 0; it < 4; ++it) {
+      const int rr = it * 8 + (lane >> 2);
+      const uint4 v = *reinterpret_cast<const uint4*>(stg + patch_at(rr, cc));
+      if (row0 + rr < o.M) *reinterpret_cast<uint4*>(p + (int64_t)(row0 + rr) * ld + col + cc * 8) = v;
+    }
+    return;
   }
+  if (col + lane >= end) return;
+  p += (int64_t)row0 * ld + col + lane;
+#pragma unroll 8
+  for (int rr = 0; rr < 32; ++rr)
+    if (row0 + rr < o.M) p[rr * ld] = *reinterpret_cast<const __nv_bfloat16*>(stg + patch_at(rr, lane >> 3) + (lane & 7) * 2);
 }
-// 64 columns of row `lane`, rounded, into the staging rows.
+// Row `lane` of a patch, rounded, into the staging buffer.
 __device__ __forceinline__ void stage_row(uint8_t* stg, int lane, const float2* v) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(stg + patch_at(lane, j)) =
         make_uint4(pack_bf16x2(v[4 * j].x, v[4 * j].y), pack_bf16x2(v[4 * j + 1].x, v[4 * j + 1].y), pack_bf16x2(v[4 * j + 2].x, v[4 * j + 2].y),
                    pack_bf16x2(v[4 * j + 3].x, v[4 * j + 3].y));
 }
 
-// A warp's 32 rows x 64 columns of sums (`acc`: 64 columns of row row0 + lane, in pairs) become results: z = sum + bias, act(z) + residual in fp32,
-// one rounding. Columns from `end` on belong to another tile or to none. The bf16 rows are turned around in the warp's staging buffer, so that global
+// A warp's patch of sums (`acc`: the 32 columns of row row0 + lane, in pairs) becomes results: z = sum + bias, act(z) + residual in fp32, one
+// rounding. Columns from `end` on belong to another tile or to none. The bf16 rows are turned around in the warp's staging buffer, so that global
 // accesses run along rows; the residual comes the same way: asked for by early_patch before the sums are there, or here where z goes first.
 template <int ACT, bool RES>
 __device__ __forceinline__ void early_patch(const LinOut& o, uint8_t* stg, int lane, int row0, int col0, int end) {
-  if (!RES || !o.vec || (ACT != kActNone && o.pre != nullptr)) return;
+  if (!RES || (ACT != kActNone && o.pre != nullptr)) return;
   __syncwarp();                                          // the patch before has been read
   load_patch(stg, o, row0, col0, end, lane);
 }
 template <bool FWD, int ACT, bool RES>
 __device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int lane, int row0, int col0, int end, float2* acc) {
-  if (o.vec) {
-    if (FWD && o.bias != nullptr) {                      // two values per lane, from where every lane reads them all
-      const int c = col0 + 2 * lane;
-      float b[2] = {0.f, 0.f};
-      if (c < end) {
-        if (o.bias_f32) load_vec<float, 2>(reinterpret_cast<const float*>(o.bias) + c, b);
-        else load_vec<__nv_bfloat16, 2>(reinterpret_cast<const __nv_bfloat16*>(o.bias) + c, b);
-      }
-      float* bs = reinterpret_cast<float*>(stg + 4096);
-      __syncwarp();
-      *reinterpret_cast<float2*>(bs + 2 * lane) = make_float2(b[0], b[1]);
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float4 v = *reinterpret_cast<const float4*>(bs + 4 * j);
-        acc[2 * j] = add2(acc[2 * j], make_float2(v.x, v.y));
-        acc[2 * j + 1] = add2(acc[2 * j + 1], make_float2(v.z, v.w));
-      }
+  if (FWD && o.bias != nullptr) {                        // a value per lane, to where every lane reads them all
+    const int c = col0 + lane;
+    float b = 0.f;
+    if (c < end) {
+      if (o.bias_f32) b = reinterpret_cast<const float*>(o.bias)[c];
+      else b = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(o.bias)[c]);
     }
-    if (FWD && ACT != kActNone && o.pre != nullptr) {
-      __syncwarp();
-      stage_row(stg, lane, acc);
-      __syncwarp();
-      store_patch(stg, o.pre, o.ldpre, row0, col0, o.M, end, lane);
-      if (RES) {
-        __syncwarp();
-        load_patch(stg, o, row0, col0, end, lane);
-      }
-    }
-    if (FWD) {
+    float* bs = reinterpret_cast<float*>(stg + kLPatch);
+    __syncwarp();
+    bs[lane] = b;
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) acc[j] = activate<ACT>(acc[j]);
+    for (int j = 0; j < 8; ++j) {
+      const float4 v = *reinterpret_cast<const float4*>(bs + 4 * j);
+      acc[2 * j] = add2(acc[2 * j], make_float2(v.x, v.y));
+      acc[2 * j + 1] = add2(acc[2 * j + 1], make_float2(v.z, v.w));
     }
-    if (FWD && RES) {
-      wait_patch();
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint4 v = *reinterpret_cast<const uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4));
-        float q[8];
-        unpack_bf16x2(v.x, q); unpack_bf16x2(v.y, q + 2); unpack_bf16x2(v.z, q + 4); unpack_bf16x2(v.w, q + 6);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[4 * j + i] = add2(acc[4 * j + i], make_float2(q[2 * i], q[2 * i + 1]));
-      }
-    }
+  }
+  if (FWD && ACT != kActNone && o.pre != nullptr) {
     __syncwarp();
     stage_row(stg, lane, acc);
     __syncwarp();
-    store_patch(stg, o.C, o.ldc, row0, col0, o.M, end, lane);
-    return;
-  }
-  // rows off a 16-byte boundary: fp32 sums turned around 32 columns at a time, then a lane per column, one row after another
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float* turn = reinterpret_cast<float*>(stg);
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 32; ++j) turn[lane * 32 + ((j + lane) & 31)] = j & 1 ? acc[16 * half + j / 2].y : acc[16 * half + j / 2].x;
-    __syncwarp();
-    const int col = col0 + 32 * half + lane;
-    if (col >= end) continue;
-    float bias = 0.f;
-    if (FWD && o.bias != nullptr) {
-      if (o.bias_f32) bias = reinterpret_cast<const float*>(o.bias)[col];
-      else bias = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(o.bias)[col]);
-    }
-    const int rows = min(32, o.M - row0);
-#pragma unroll 4
-    for (int rr = 0; rr < rows; rr += 2) {               // two rows at a time, as the activations come in pairs
-      const int next = rr + 1 < rows ? rr + 1 : rr;
-      float2 v = make_float2(turn[rr * 32 + ((lane + rr) & 31)], turn[next * 32 + ((lane + next) & 31)]);
-      const int64_t r0 = row0 + rr, r1 = row0 + next;
-      if (FWD) {
-        v = add2(v, make_float2(bias, bias));
-        if (ACT != kActNone && o.pre != nullptr) {
-          o.pre[r0 * o.ldpre + col] = __float2bfloat16_rn(v.x);
-          o.pre[r1 * o.ldpre + col] = __float2bfloat16_rn(v.y);
-        }
-        v = activate<ACT>(v);
-        if (RES) v = add2(v, make_float2(__bfloat162float(o.res[r0 * o.ldres + col]), __bfloat162float(o.res[r1 * o.ldres + col])));
-      }
-      o.C[r0 * o.ldc + col] = __float2bfloat16_rn(v.x);
-      o.C[r1 * o.ldc + col] = __float2bfloat16_rn(v.y);
+    store_patch(stg, o.pre, o.ldpre, o, row0, col0, end, lane);
+    if (RES) {
+      __syncwarp();
+      load_patch(stg, o, row0, col0, end, lane);
     }
   }
+  if (FWD) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = activate<ACT>(acc[j]);
+  }
+  if (FWD && RES) {
+    wait_patch();
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(stg + patch_at(lane, j));
+      float q[8];
+      unpack_bf16x2(v.x, q); unpack_bf16x2(v.y, q + 2); unpack_bf16x2(v.z, q + 4); unpack_bf16x2(v.w, q + 6);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[4 * j + i] = add2(acc[4 * j + i], make_float2(q[2 * i], q[2 * i + 1]));
+    }
+  }
+  __syncwarp();
+  stage_row(stg, lane, acc);
+  __syncwarp();
+  store_patch(stg, o.C, o.ldc, o, row0, col0, end, lane);
+}
+
+// Says that sums have been read: they are in registers (tcgen05.wait::ld has returned, the fence before it orders the reads), so the arrival has no
+// memory to release, and a release would wait for every store that the thread has in flight (16384 x 1152 -> 4608 with gelu_tanh and z: 133 us, 125).
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // WIDE: tiles of more than 256 columns (CTA pairs only).
@@ -262,7 +249,7 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], CG * 32 * kLEpiWarps);
+      mbar_init(&tempty[i], CG * kLEpiWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -400,7 +387,9 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ epilogue
-    // Two warps share a quarter of the rows (the TMEM lanes a warp may read) and take alternate patches of 64 columns.
+    // Four warps share a quarter of the rows (the TMEM lanes a warp may read) and take patches of 32 columns in turn. A warp waits most of the time,
+    // for TMEM, shared memory and the exponential unit, about 10 clocks per instruction: with 8 warps of 64 columns the drain of a tile outlasted its
+    // products where an activation was applied (16384 x 1152 -> 4608, gelu_tanh and z: 168 us against 112 plain).
     const int quarter = warp & 3, side = (warp - 2) >> 2;
     uint8_t* stg = epi + (warp - 2) * kLStage;
     int acc = 0;
@@ -410,32 +399,38 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
       const int cols = min(u.width, a.out.N - u.n0);
       if (RES) {                                        // the residual's rows come into L2 while the product is computed
         const uint8_t* line = reinterpret_cast<const uint8_t*>(a.out.res + (int64_t)min(row0 + lane, a.out.M - 1) * a.out.ldres + u.n0);
-        for (int o = side * 128; o < cols * 2; o += 256) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + o));
+        for (int o = side * 128; o < cols * 2; o += 512) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + o));
       }
       if (!mbar_wait_bounded(&tfull[acc], acc_phase, abort_flag, a.status, 800 + acc)) break;
       tc_fence_after();
+      // the warp's last sums are in registers: the accumulator may be overwritten as far as it goes
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) arrive_relaxed(cluster_map_u32(smem_u32(&tempty[acc]), 0));
+          else mbar_arrive(&tempty[acc]);
+        }
+      };
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
+      if (side * 32 >= cols) release();
 #pragma unroll 1
-      for (int c = side * 64; c < cols; c += 128) {
-        __align__(8) uint32_t r[64];
+      for (int c = side * 32; c < cols; c += 128) {
+        __align__(8) uint32_t r[32];
         tmem_ld_32x32(t_row + c, r);
-        tmem_ld_32x32(t_row + c + 32, r + 32);
         early_patch<ACT, RES>(a.out, stg, lane, row0, u.n0 + c, u.n0 + cols);
         tmem_wait_ld();
+        if (c + 128 >= cols) release();
         if constexpr (SPLIT) {
           const int64_t tiles = (int64_t)plan.num_m * plan.full_n + (a.out.N % plan.bn ? plan.num_m : 0);
           float4* w = reinterpret_cast<float4*>(plan.ws) + (((u.part * tiles + u.tile) * (CG * 4) + rank * 4 + quarter) * (plan.bn / 4) + c / 4) * 32 + lane;
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c + 4 * j < u.width)
-              w[j * 32] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+          for (int j = 0; j < 8; ++j)
+            w[j * 32] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]), __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
         } else {
           finish_patch<FWD, ACT, RES>(a.out, stg, lane, row0, u.n0 + c, u.n0 + cols, reinterpret_cast<float2*>(r));
         }
       }
-      tc_fence_before();
-      if constexpr (CG == 2) mbar_arrive_cluster(cluster_map_u32(smem_u32(&tempty[acc]), 0));
-      else mbar_arrive(&tempty[acc]);
       if (++acc == accs) { acc = 0; acc_phase ^= 1; }
     }
   }
@@ -450,7 +445,7 @@ __global__ void __launch_bounds__(kLThreads, 1) linear_kernel(const __grid_const
   }
 }
 
-// The parts of every tile added in their order, and the epilogue: a warp per 32 rows x 64 columns.
+// The parts of every tile added in their order, and the epilogue: a warp per patch.
 constexpr int kJoinWarps = 4;
 template <bool FWD, int ACT, bool RES>
 __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __grid_constant__ LinArgs a, int cg, int patches) {
@@ -459,8 +454,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __gr
   const int id = blockIdx.x * kJoinWarps + wid;
   if (id >= patches) return;
   const LinPlan& p = a.plan;
-  const int blocks = cg * 4, per_tile_row = (a.out.N + 63) / 64;
-  const int mb = id / per_tile_row, col0 = (id - mb * per_tile_row) * 64;      // 32-row block, first column
+  const int blocks = cg * 4, per_tile_row = (a.out.N + 31) / 32;
+  const int mb = id / per_tile_row, col0 = (id - mb * per_tile_row) * 32;      // 32-row block, first column
   const int row0 = mb * 32, m = mb / blocks, block = mb - m * blocks;
   const int n = col0 / p.bn, c = col0 - n * p.bn, whole = p.num_m * p.full_n;
   int tile;
@@ -469,21 +464,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __gr
     const int group = 16 / cg, g = m / group, first = g * group, gm = p.num_m - first < group ? p.num_m - first : group;
     tile = g * group * p.full_n + n * gm + (m - first);
   }
-  const int width = n >= p.full_n ? (a.out.N - n * p.bn + 31) & ~31 : p.bn;
   const int64_t tiles = (int64_t)whole + (a.out.N % p.bn ? p.num_m : 0), part = tiles * blocks * (p.bn / 4) * 32;
   const float4* w = reinterpret_cast<const float4*>(p.ws) + (((int64_t)tile * blocks + block) * (p.bn / 4) + c / 4) * 32 + lane;
   early_patch<ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N);
-  float2 acc[32];
+  float2 acc[16];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) acc[j] = make_float2(0.f, 0.f);
+  for (int j = 0; j < 16; ++j) acc[j] = make_float2(0.f, 0.f);
+#pragma unroll 2
   for (int s = 0; s < p.splits; ++s) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (c + 4 * j < width) {
-        const float4 v = w[s * part + j * 32];
-        acc[2 * j] = add2(acc[2 * j], make_float2(v.x, v.y));
-        acc[2 * j + 1] = add2(acc[2 * j + 1], make_float2(v.z, v.w));
-      }
+    for (int j = 0; j < 8; ++j) {
+      const float4 v = w[s * part + j * 32];
+      acc[2 * j] = add2(acc[2 * j], make_float2(v.x, v.y));
+      acc[2 * j + 1] = add2(acc[2 * j + 1], make_float2(v.z, v.w));
+    }
   }
   finish_patch<FWD, ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N, acc);
 }
@@ -639,7 +633,7 @@ static int lin_launch(int cg, const CUtensorMap& ta, const CUtensorMap& tb, cons
 }
 template <bool FWD, int ACT, bool RES>
 static int lin_join(int cg, const LinArgs& a, cudaStream_t stream) {
-  const int patches = a.plan.num_m * cg * 4 * ((a.out.N + 63) / 64);
+  const int patches = a.plan.num_m * cg * 4 * ((a.out.N + 31) / 32);
   linear_join_kernel<FWD, ACT, RES><<<(patches + kJoinWarps - 1) / kJoinWarps, 32 * kJoinWarps, 0, stream>>>(a, cg, patches);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
@@ -722,7 +716,7 @@ static LinCut lin_find_cut(int M, int N, int K, bool b_mn, int drain) {
       last = bn;
       const int tiles = num_m * ((N + bn - 1) / bn);
       for (int splits = 1; splits == 1 || (splits <= 8 && splits * 2 <= kb); ++splits) {
-        if (splits > 1 && (bn % 64 || tiles * (splits - 1) >= 2 * most)) break;
+        if (splits > 1 && tiles * (splits - 1) >= 2 * most) break;
         double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, b_mn, splits > 1 ? lin_drain(0, false, false) : drain);
         if (cg == 1) t *= 1.08;                          // a single CTA reads 1.5 times the operands per product
         if (splits > 1) t += 5.5 + 4e-6 * splits * (double)M * N / 4.0;
@@ -782,7 +776,7 @@ static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda,
     if (make_tmap_bf16(&tb2, B, 2, dims, str, box)) return -12;
   }
   auto at16 = [](const void* q, int64_t ld) { return q == nullptr || (!(reinterpret_cast<uintptr_t>(q) & 15) && ld % 8 == 0); };
-  o.vec = o.N % 8 == 0 && at16(o.C, o.ldc) && at16(o.res, o.ldres) && at16(o.pre, o.ldpre) && !(reinterpret_cast<uintptr_t>(o.bias) & 15);
+  o.vec = o.N % 8 == 0 && at16(o.C, o.ldc) && at16(o.res, o.ldres) && at16(o.pre, o.ldpre);
   const bool split = p.splits > 1;
   if (!fwd) {
     int rc;
