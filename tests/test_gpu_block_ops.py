@@ -634,3 +634,35 @@ def test_gated_attention_against_its_fp32_statement():
     for name, ref in want.items():
         off = (got[name].detach().float().cpu() - ref.detach()).norm() / ref.detach().norm()
         assert off <= (10 if name == "y" else 20) * 2.0 ** -8, (name, off.item())
+
+
+def test_linear_act_with_more_rows_than_a_grid_of_16_bit_tiles():
+    """2^24 + 300 rows: 131 075 tile rows of one narrow column. A row is 8 products of values that bf16 holds exactly, so z is off by fp32's rounding
+    alone, 8 steps of 2^-24 of the sum of magnitudes, and y by one rounding to bf16 more; dW sums 2^24 rows of magnitude 1 and random sign."""
+    from torchllmtuner_b200 import ops
+    m = (1 << 24) + 300
+    g = torch.Generator(DEV).manual_seed(5)
+    x = torch.randint(-8, 9, (m, 8), device=DEV, generator=g).bfloat16() / 8
+    w = (torch.randint(-8, 9, (8, 8), device=DEV, generator=g).bfloat16() / 8).requires_grad_()
+    y = ops.linear_act(x, w, activation="relu")
+    dw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    for rows in (slice(0, 600), slice(m // 2, m // 2 + 600), slice(m - 600, m)):
+        want = (x[rows].double() @ w.detach().double().t()).relu()
+        assert ((y[rows].double() - want).abs() <= want * 2.0 ** -8 + 8 * 8 * 2.0 ** -24).all()
+    z = x.double() @ w.detach().double().t()
+    want = (z > 0).double().t() @ x.double()
+    # exact multiples of 1/8 up to 2^24: fp32 sums (in parts) are off by at most a few hundred half steps of their magnitude; one rounding to bf16
+    assert ((dw.double() - want).abs() <= want.abs() * 2.0 ** -8 + x.double().abs().sum(0) * 2.0 ** -12).all()
+
+
+def test_gelu_tanh_gradient_of_enormous_values():
+    """act' is 1 and 0 far out, also where z^3 overflows fp32."""
+    from torchllmtuner_b200 import ops
+    z = torch.tensor([1e3, 1e10, 1e20, 3e38, -1e3, -1e10, -1e20, -3e38], device=DEV).bfloat16().unsqueeze(1)
+    one = torch.zeros(8, 8, device=DEV, dtype=torch.bfloat16)
+    one[:, 0] = 1
+    x = torch.cat((z, torch.zeros(8, 7, device=DEV, dtype=torch.bfloat16)), 1).requires_grad_()
+    for act in ("gelu_tanh", "gelu", "silu", "relu"):
+        y = ops.linear_act(x, one, activation=act)
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert (dx[:4, 0] == 8).all() and (dx[4:, 0] == 0).all(), (act, dx[:, 0])

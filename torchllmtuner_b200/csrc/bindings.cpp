@@ -1342,16 +1342,21 @@ std::vector<Tensor> rope_tables(const Tensor& positions, const Tensor& inv, doub
 // -------- linear layers with an epilogue
 // Rows as TMA reads them: unit inner stride, row stride a multiple of 8, 16-byte start; otherwise a copy with padded rows (the padding is never
 // read: the tensor map ends at the last column).
+// Rows of a buffer that TMA reads: on 128 bytes where that adds at most an eighth (a row of a box then lies in one line), else on 16.
+int64_t row_pitch(int64_t n) {
+  const int64_t lines = (n + 63) / 64 * 64;
+  return lines - n <= n / 8 ? lines : (n + 7) / 8 * 8;
+}
 Tensor tma_rows(const Tensor& t) {
   if ((t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
-  Tensor r = torch::empty({t.size(0), (t.size(1) + 7) / 8 * 8}, t.options()).narrow(1, 0, t.size(1));
+  Tensor r = torch::empty({t.size(0), row_pitch(t.size(1))}, t.options()).narrow(1, 0, t.size(1));
   r.copy_(t);
   return r;
 }
 // Partial sums of a product that is cut along its depth; of this call alone, so graphs and streams share nothing.
-Tensor linear_workspace(int64_t M, int64_t N, int64_t K, bool gradient, int64_t act, bool res, bool pre, const Tensor& like) {
-  const int64_t n = llmt_linear_ws_floats((int)M, (int)N, (int)K, gradient, (int)act, res, pre);
-  return n > 0 ? fresh({n}, at::kFloat, like) : Tensor();
+Tensor linear_workspace(int64_t M, int64_t N, int64_t K, const Tensor& a, const Tensor& b, bool gradient, int64_t act, bool res, bool pre) {
+  const int64_t n = llmt_linear_ws_floats((int)M, (int)N, (int)K, a.stride(0), b.stride(0), gradient, (int)act, res, pre);
+  return n > 0 ? fresh({n}, at::kFloat, a) : Tensor();
 }
 inline float* ws_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 inline int64_t ws_size(const Tensor& t) { return t.defined() ? t.numel() : 0; }
@@ -1378,8 +1383,9 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
       r2 = rows_2d(*r);
       if (M > 1 && r2.stride(0) < N && r2.stride(0) != 0) r2 = r2.contiguous();
     }
-    if (act != 0 && keep) pre = fresh({M, (N + 7) / 8 * 8}, at::kBFloat16, x);
-    const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), false, act, r2.defined(), pre.defined(), x);
+    if (act != 0 && keep) pre = fresh({M, row_pitch(N)}, at::kBFloat16, x);
+    const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), x2, w2, false, act, r2.defined(),
+                                       pre.defined());
     check_rc(llmt_linear_act(x2.data_ptr(), w2.data_ptr(), y.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, bc.defined() && is_f32(bc),
                              r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, (int)M,
                              (int)N, (int)K, x2.stride(0), w2.stride(0), N, r2.defined() ? r2.stride(0) : 0, pre.defined() ? pre.stride(0) : 0,
@@ -1426,7 +1432,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
     const bool tma_ok = dy.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
     const bool write = (nx || nw) && (act != 0 || !tma_ok);
-    Tensor dz = write ? fresh({M, (N + 7) / 8 * 8}, at::kBFloat16, x) : dy;
+    Tensor dz = write ? fresh({M, row_pitch(N)}, at::kBFloat16, x) : dy;
     if (write || nb) {
       if (nb) out[2] = fresh(b.sizes(), b.scalar_type(), x);
       const int P = nb ? llmt_linear_db_partials((int)M, (int)N) : 0;
@@ -1453,14 +1459,14 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     const int64_t lddz = dz.stride(0);
     if (nx) {
       out[0] = fresh(x.sizes(), at::kBFloat16, x);
-      const Tensor ws = linear_workspace(M, K, N, true, 0, false, false, dz);
+      const Tensor ws = linear_workspace(M, K, N, dz, w2, true, 0, false, false);
       check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),
                "llmt_linear_dx", ws.defined() ? 2 : 1);
     }
     if (nw) {
       out[1] = fresh(w.sizes(), at::kBFloat16, x);
-      const Tensor ws = linear_workspace(N, K, M, true, 0, false, false, dz);
+      const Tensor ws = linear_workspace(N, K, M, dz, x2, true, 0, false, false);
       check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),
                "llmt_linear_dw", ws.defined() ? 2 : 1);

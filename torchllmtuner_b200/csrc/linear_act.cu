@@ -647,10 +647,13 @@ static int64_t lin_ws_floats(int M, int N, const LinCut& c) {
 
 // Time of one k-block of a tile, in ns. Alone the products bound it (256 columns 302, 192 230, 128 and fewer about 200 with the loop around them);
 // with every SM at it the operands, which come from L2 at 10 to 13 TB/s: 256 columns 420, 192 360, 128 260 (16384 x 4608 x 1152). `loaded`: columns
-// that the TMA boxes fetch, more than `bn` where B is stored [K][N] and half a tile is no multiple of 64.
-static double lin_kb_ns(int bn, int loaded, double busy) {
-  const double alone = bn * 1.18 > 200 ? bn * 1.18 : 200, crowded = 120 + 0.6 * (bn + loaded);
-  return crowded > alone ? alone + (crowded - alone) * busy : alone;
+// that the TMA boxes fetch, more than `bn` where B is stored [K][N] and half a tile is no multiple of 64. `skewed`: rows of 128 bytes that a CTA
+// fetches from matrices whose rows do not start on 128 bytes, each from two lines: 1.75 ns (products of 1000 x 1000 over 3000 and 6000 rows: 485
+// ns a k-block for 128 columns, 660 for 256, against 230 where the rows have 1024 elements).
+static double lin_kb_ns(int bn, int loaded, int skewed, double busy) {
+  const double alone = bn * 1.18 > 200 ? bn * 1.18 : 200, crowded = 120 + 0.6 * (bn + loaded), lines = 1.75 * skewed;
+  const double t = crowded > alone ? alone + (crowded - alone) * busy : alone;
+  return t > lines ? t : lines;
 }
 // Units of whole tiles go round the workers; those of narrow tiles go one by one to the worker that is free first.
 static void lin_plan(LinPlan& p, int N, int num_tiles_m, int most) {
@@ -660,7 +663,7 @@ static void lin_plan(LinPlan& p, int N, int num_tiles_m, int most) {
   p.workers = whole + narrow < most ? whole + narrow : most;
   const int ahead = whole % p.workers;                   // workers [0, ahead) have one whole unit more
   const int behind = ahead ? p.workers - ahead : 0;
-  const int fit = rest ? (int)(lin_kb_ns(p.bn, p.bn, 0) / lin_kb_ns((rest + 31) / 32 * 32, 0, 0) + 0.1) : 0;       // narrow units in the time of a whole one
+  const int fit = rest ? (int)(lin_kb_ns(p.bn, p.bn, 0, 0) / lin_kb_ns((rest + 31) / 32 * 32, 0, 0, 0) + 0.1) : 0;       // narrow units in the time of a whole one
   const int catch_up = narrow < behind * fit ? narrow : behind * fit, left = narrow - catch_up;
   int at = 0;
   for (int w = 0; w < p.workers; ++w) {
@@ -670,24 +673,25 @@ static void lin_plan(LinPlan& p, int N, int num_tiles_m, int most) {
   }
   p.narrow_begin[p.workers] = at;
 }
-// What an epilogue adds to the time in which two warps drain 32 rows of 128 columns, in tenths of a us: 9 for the sums alone, and what activation,
-// residual and z add (16384 x 1152 -> 4608 on tiles of 512 columns, whose drain nothing hides: 112 us plain, relu 120, silu 137, gelu_tanh 145, gelu
-// 154, and z another 22 to 24).
+// A product as the estimate sees it: B stored [K][N], matrices whose rows are no multiple of 128 bytes, what the epilogue takes (lin_drain).
+struct LinKind { int b_mn, skew_a, skew_b, drain; };
+// Time in which 128 columns of a tile are drained, in tenths of a us: 9 for the sums (every SM writes at the same time), 3 for a residual, 8 for z,
+// which is a second result, and what the activation takes beyond its wait for memory.
 static int lin_drain(int act, bool res, bool pre) {
-  const int cost[kActKinds] = {0, 13, 10, 8, 3};         // in the order of ActKind
+  const int cost[kActKinds] = {0, 4, 1, 1, 0};           // in the order of ActKind
   return 9 + cost[act] + (res ? 3 : 0) + (act != kActNone && pre ? 8 : 0);
 }
 // The longest worker's units, in us (kb deep, `splits` parts).
-static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb, bool b_mn, int tenths) {
+static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb, const LinKind& kind, int tenths) {
   const int most = sm_count() / cg, full_n = N / bn, rest = N - full_n * bn, whole = num_m * full_n * splits, narrow = rest ? num_m * splits : 0;
   const int workers = whole + narrow < most ? whole + narrow : most;
   const double depth = (double)((kb + splits - 1) / splits);
   // a tile is not done before its sums are drained: see lin_drain, hidden under the next tile's products where there are two
   // accumulators; 0.5 us pass between two tiles
   auto unit = [&](int w, int running) {
-    const int loaded = b_mn ? (w + 64 * cg - 1) / (64 * cg) * 64 * cg : w;
-    const double drain = 0.1 * tenths * w / 128, mma = 0.5 + depth * lin_kb_ns(w, loaded, (double)running * cg / sm_count()) * 1e-3;
-    return bn > 256 ? mma + drain : mma > drain ? mma : drain;
+    const int loaded = kind.b_mn ? (w + 64 * cg - 1) / (64 * cg) * 64 * cg : w, skewed = (kind.skew_a ? kLM : 0) + (kind.skew_b ? loaded / cg : 0);
+    const double drain = 0.1 * tenths * w / 128, mma = 0.5 + depth * lin_kb_ns(w, loaded, skewed, (double)running * cg / sm_count()) * 1e-3;
+    return bn > 256 ? 1.1 * mma + drain : mma > drain ? mma : drain;        // 1.1: 4096 x 2048 x 2048 takes 32.9 us on 512 columns, 30.4 on 256
   };
   const int rounds = whole / workers, ahead = whole % workers, behind = ahead ? workers - ahead : 0;
   double t = rounds * unit(bn, workers) + (ahead ? unit(bn, ahead + (narrow < behind ? narrow : behind)) : 0);
@@ -702,7 +706,7 @@ static double lin_makespan(int cg, int bn, int splits, int num_m, int N, int kb,
 // How a product is cut: CTAs per tile, tile width and parts along K. The shortest of the candidates by the estimate: tile widths that divide N
 // evenly into 1, 2, ... columns of tiles, one CTA or a pair, and parts along K where the tiles leave workers idle. The parts cost a second
 // launch and their sums in memory: 5.5 us and 4 bytes per sum and part at 4 TB/s (1152 x 1152 in 3 parts: 8.0 us).
-static LinCut lin_find_cut(int M, int N, int K, bool b_mn, int drain) {
+static LinCut lin_find_cut(int M, int N, int K, const LinKind& kind) {
   const int kb = (K + kLK - 1) / kLK;
   LinCut best{1, 128, 1};
   double least = 1e30;
@@ -717,7 +721,7 @@ static LinCut lin_find_cut(int M, int N, int K, bool b_mn, int drain) {
       const int tiles = num_m * ((N + bn - 1) / bn);
       for (int splits = 1; splits == 1 || (splits <= 8 && splits * 2 <= kb); ++splits) {
         if (splits > 1 && tiles * (splits - 1) >= 2 * most) break;
-        double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, b_mn, splits > 1 ? lin_drain(0, false, false) : drain);
+        double t = (cg == 2 ? 1.2 : 0.0) + lin_makespan(cg, bn, splits, num_m, N, kb, kind, splits > 1 ? lin_drain(0, false, false) : kind.drain);
         if (cg == 1) t *= 1.08;                          // a single CTA reads 1.5 times the operands per product
         if (splits > 1) t += 5.5 + 4e-6 * splits * (double)M * N / 4.0;
         if (t < least) {
@@ -730,13 +734,16 @@ static LinCut lin_find_cut(int M, int N, int K, bool b_mn, int drain) {
   return best;
 }
 // The cut of a size is found once per thread and place in a small table (it takes the host some 10 us).
-static LinCut lin_cut(int M, int N, int K, bool b_mn, int drain) {
+static LinCut lin_cut(int M, int N, int K, const LinKind& kind) {
   struct Found { int M, N, K, kind; LinCut cut; };
   static thread_local Found table[64];
-  const int kind = drain * 2 + b_mn;
-  Found& f = table[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 9176u ^ (unsigned)kind * 97u) >> 7 & 63];
-  if (f.M != M || f.N != N || f.K != K || f.kind != kind) f = Found{M, N, K, kind, lin_find_cut(M, N, K, b_mn, drain)};
+  const int bits = kind.drain * 8 + kind.b_mn * 4 + kind.skew_a * 2 + kind.skew_b;
+  Found& f = table[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 9176u ^ (unsigned)bits * 97u) >> 7 & 63];
+  if (f.M != M || f.N != N || f.K != K || f.kind != bits) f = Found{M, N, K, bits, lin_find_cut(M, N, K, kind)};
   return f.cut;
+}
+static LinKind lin_kind(bool b_mn, int64_t lda, int64_t ldb, int act, bool res, bool pre) {
+  return LinKind{b_mn ? 1 : 0, lda % 64 != 0, ldb % 64 != 0, lin_drain(act, res, pre)};
 }
 
 // out [M, N] = op(A) op(B), K deep: A stored [M][K] or (a_mn) [K][M], B stored [N][K] or (b_mn) [K][N]. ws: lin_ws_floats of the same sizes.
@@ -745,7 +752,7 @@ static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda,
   LinOut& o = a.out;
   if (o.M <= 0 || o.N <= 0) return 0;
   if (K <= 0 || (lda & 7) || (ldb & 7) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return -10;
-  const LinCut cut = lin_cut(o.M, o.N, K, b_mn, lin_drain(fwd ? act : 0, o.res != nullptr, o.pre != nullptr));
+  const LinCut cut = lin_cut(o.M, o.N, K, lin_kind(b_mn, lda, ldb, fwd ? act : 0, o.res != nullptr, o.pre != nullptr));
   if (lin_ws_floats(o.M, o.N, cut) > (ws == nullptr ? 0 : ws_floats) || sm_count() / cut.cg > kMaxWorkers) return -10;
   LinPlan& p = a.plan;
   p.bn = cut.bn;
@@ -833,11 +840,12 @@ static int dz_dispatch(bool vec, int blocks, const void* dy, int64_t ldy, const 
 
 using namespace llmt;
 
-// Workspace of a product out [M, N] of depth K, in floats (0: none is needed): of llmt_linear_dx or llmt_linear_dw (`gradient`; act, res and pre 0),
-// or of llmt_linear_act with that activation, with a residual (`res`) and with z (`pre`).
-extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int gradient, int act, int res, int pre) {
+// Workspace of a product out [M, N] of depth K whose operands' rows lie lda and ldb elements apart, in floats (0: none is needed): of llmt_linear_dx
+// (dz, W) or llmt_linear_dw (dz, x) (`gradient`; act, res and pre 0), or of llmt_linear_act (x, W) with that activation, with a residual (`res`) and
+// with z (`pre`).
+extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre) {
   if (act < 0 || act >= kActKinds) return 0;             // refused by the launch
-  return lin_ws_floats(M, N, lin_cut(M, N, K, gradient != 0, lin_drain(act, res != 0, pre != 0)));
+  return lin_ws_floats(M, N, lin_cut(M, N, K, lin_kind(gradient != 0, lda, ldb, act, res != 0, pre != 0)));
 }
 
 // y [M, N] = act(x [M, K] W [N, K]^T + bias) + res; pre (optional, read by llmt_linear_dz) receives x W^T + bias where there is an activation.
