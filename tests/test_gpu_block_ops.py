@@ -666,3 +666,30 @@ def test_gelu_tanh_gradient_of_enormous_values():
         y = ops.linear_act(x, one, activation=act)
         dx, = torch.autograd.grad(y, x, torch.ones_like(y))
         assert (dx[:4, 0] == 8).all() and (dx[4:, 0] == 0).all(), (act, dx[:, 0])
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_linear_act_gradient_into_an_owners_buffer(act):
+    """A weight with `main_grad` gets its gradient there: written the first time, added the second, and None is returned for it; x and bias as ever."""
+    from torchllmtuner_b200 import ops
+    x, w, b = _rand(300, 200, seed=1), _rand(136, 200, seed=2, std=0.07), _rand(136, seed=3)
+    dy = _rand(300, 136, seed=4)
+
+    def grads(owned):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+        if owned:
+            leaves[1].main_grad, leaves[1].main_grad_initialized = torch.full((136, 200), 7.0, device=DEV, dtype=torch.bfloat16), False
+        out = []
+        for _ in range(2):
+            y = ops.linear_act(*leaves, activation=act)
+            out.append(torch.autograd.grad(y, leaves, dy, allow_unused=True))
+        return leaves, out
+    _, plain = grads(False)
+    leaves, owned = grads(True)
+    assert owned[0][1] is None and owned[1][1] is None
+    for i in (0, 2):
+        for got in owned:
+            assert torch.equal(got[i], plain[0][i])
+    # the sum of two equal gradients, each product rounded once: the second launch adds to the rounded first
+    want = 2 * plain[0][1].double()
+    assert ((leaves[1].main_grad.double() - want).abs() <= want.abs() * 3 * 2.0 ** -8 + want.abs().max() * 2.0 ** -16).all()

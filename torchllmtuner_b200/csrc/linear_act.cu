@@ -40,7 +40,7 @@ struct LinOut {
   int64_t ldres;
   __nv_bfloat16* pre;
   int64_t ldpre;
-  int vec;                               // every row of C, res and pre starts on 16 bytes and N is a multiple of 8
+  int vec;                               // every row of C and res starts on 16 bytes and N is a multiple of 8; those of pre always do, padded
 };
 // The tiles of a product and who computes them. A tile is kLM * CG rows by `bn` columns (a multiple of 32, at most 512): up to 256 columns by one
 // MMA per 16 deep slice, and the accumulator is double buffered in TMEM, so that a tile is drained under the next one's products; the columns
@@ -123,15 +123,15 @@ __device__ __forceinline__ void load_patch(uint8_t* stg, const LinOut& o, int ro
 }
 __device__ __forceinline__ void wait_patch() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // The staging buffer's patch to global memory, along its rows.
-__device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p, int64_t ld, const LinOut& o, int row0, int col, int end, int lane) {
-  if (o.vec) {
+__device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p, int64_t ld, bool vec, int M, int row0, int col, int end, int lane) {
+  if (vec) {
     const int cc = lane & 3;
     if (col + cc * 8 >= end) return;
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
       const int rr = it * 8 + (lane >> 2);
       const uint4 v = *reinterpret_cast<const uint4*>(stg + patch_at(rr, cc));
-      if (row0 + rr < o.M) *reinterpret_cast<uint4*>(p + (int64_t)(row0 + rr) * ld + col + cc * 8) = v;
+      if (row0 + rr < M) *reinterpret_cast<uint4*>(p + (int64_t)(row0 + rr) * ld + col + cc * 8) = v;
     }
     return;
   }
@@ -139,7 +139,7 @@ __device__ __forceinline__ void store_patch(const uint8_t* stg, __nv_bfloat16* p
   p += (int64_t)row0 * ld + col + lane;
 #pragma unroll 8
   for (int rr = 0; rr < 32; ++rr)
-    if (row0 + rr < o.M) p[rr * ld] = *reinterpret_cast<const __nv_bfloat16*>(stg + patch_at(rr, lane >> 3) + (lane & 7) * 2);
+    if (row0 + rr < M) p[rr * ld] = *reinterpret_cast<const __nv_bfloat16*>(stg + patch_at(rr, lane >> 3) + (lane & 7) * 2);
 }
 // Row `lane` of a patch, rounded, into the staging buffer.
 __device__ __forceinline__ void stage_row(uint8_t* stg, int lane, const float2* v) {
@@ -183,7 +183,7 @@ __device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int 
     __syncwarp();
     stage_row(stg, lane, acc);
     __syncwarp();
-    store_patch(stg, o.pre, o.ldpre, o, row0, col0, end, lane);
+    store_patch(stg, o.pre, o.ldpre, true, o.M, row0, col0, end, lane);
     if (RES) {
       __syncwarp();
       load_patch(stg, o, row0, col0, end, lane);
@@ -208,7 +208,7 @@ __device__ __forceinline__ void finish_patch(const LinOut& o, uint8_t* stg, int 
   __syncwarp();
   stage_row(stg, lane, acc);
   __syncwarp();
-  store_patch(stg, o.C, o.ldc, o, row0, col0, end, lane);
+  store_patch(stg, o.C, o.ldc, o.vec, o.M, row0, col0, end, lane);
 }
 
 // Says that sums have been read: they are in registers (tcgen05.wait::ld has returned, the fence before it orders the reads), so the arrival has no
@@ -783,7 +783,8 @@ static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda,
     if (make_tmap_bf16(&tb2, B, 2, dims, str, box)) return -12;
   }
   auto at16 = [](const void* q, int64_t ld) { return q == nullptr || (!(reinterpret_cast<uintptr_t>(q) & 15) && ld % 8 == 0); };
-  o.vec = o.N % 8 == 0 && at16(o.C, o.ldc) && at16(o.res, o.ldres) && at16(o.pre, o.ldpre);
+  o.vec = o.N % 8 == 0 && at16(o.C, o.ldc) && at16(o.res, o.ldres);
+  if (o.pre != nullptr && (!at16(o.pre, o.ldpre) || o.ldpre < (o.N + 7) / 8 * 8)) return -10;
   const bool split = p.splits > 1;
   if (!fwd) {
     int rc;
@@ -848,7 +849,8 @@ extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int64_t lda, int64
   return lin_ws_floats(M, N, lin_cut(M, N, K, lin_kind(gradient != 0, lda, ldb, act, res != 0, pre != 0)));
 }
 
-// y [M, N] = act(x [M, K] W [N, K]^T + bias) + res; pre (optional, read by llmt_linear_dz) receives x W^T + bias where there is an activation.
+// y [M, N] = act(x [M, K] W [N, K]^T + bias) + res; pre (optional, read by llmt_linear_dz) receives x W^T + bias where there is an activation: rows on
+// 16 bytes of at least N values rounded up to a multiple of 8.
 extern "C" int llmt_linear_act(const void* x, const void* w, void* y, const void* bias, int bias_f32, const void* res, void* pre, int act, int M, int N,
                                int K, int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, float* ws, int64_t ws_floats, int* status,
                                cudaStream_t stream) {

@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __g
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       if (live && share + i * shares < o.H) {            // a dead head's r may be infinite (eps 0)
-        const float r = rsqrtf(sq[i] * inv_d + a.eps), k = -(r * r * r * dot[i] * inv_d);
+        const float r = rsqrtf(sq[i] * inv_d + a.eps), k = -(dot[i] * inv_d * r * r * r);
         float2 x[4], out[4];
         get2(rx[i], x);
 #pragma unroll
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(256, 2) qk_norm_rope_gather_bwd_kernel(const _
         dot += __shfl_xor_sync(0xffffffffu, dot, m);
       }
       if (live && h < o.H) {                             // a dead head's r may be infinite (eps 0)
-        const float r = rsqrtf(sq / (float)s.d + a.eps), k = r * r * r * dot / (float)s.d;
+        const float r = rsqrtf(sq / (float)s.d + a.eps), k = dot / (float)s.d * r * r * r;
         float out[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_norm_rope_any_kernel(const 
         dot += g * weight(c) * x;
         buf[d + c] += g * x * r;
       }
-      const float k = r * r * r * warp_sum(dot) / (float)d;
+      const float k = warp_sum(dot) / (float)d * r * r * r;
       for (int c = lane; c < d; c += 32) {
         float x;
         load_vec<T, 1>(px + c, &x);
