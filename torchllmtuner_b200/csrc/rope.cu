@@ -246,7 +246,9 @@ static int rope_dispatch(const RopeShape& s, const RopeOperand& a, const RopeOpe
 // Wide form: a group of G lanes per head, 8 channels per lane (16 bytes of bf16). The rotation is linear, so with the weights folded into the
 // tables a channel is r (x cw + x' nw), x' its partner: in the lane itself (interleaved), or in the lane P / 8 away (half layout), from where the
 // lane's raw 16 bytes come by shuffle. A channel that passes has cw = w, nw = 0. A group takes several heads of one token, so tables and weights are
-// loaded once for them and several loads are in flight. Needs d, off and P (interleaved: 2 P) divisible by 8, d <= 256 and 16-byte addresses. Bound by memory where there are thousands of tokens.
+// loaded once for them and several loads are in flight. Needs d, off and P (interleaved: 2 P) divisible by 8, d <= 256 and 16-byte addresses.
+// 8192 tokens of 16 + 4 heads of 256, a quarter rotating: forward 32 us (168 MB, 5.2 TB/s), backward 56 us in two launches (252 MB, 4.5 TB/s). What
+// stays is instructions and the chain load - sum - scale at 16 to 32 warps an SM, not DRAM: the next chunk fetched into L2 changed nothing.
 // Gather form (below): any parts of a head up to d = 256. General form: a warp per head, the normalised head in shared memory, any d <= 1024.
 struct NormOperand {
   const void *x, *w;
@@ -264,45 +266,50 @@ struct NormArgs {
 
 // Where lane `g` of a group stands: its kind of rotation (0 passes, 1 first half, 2 second half, 3 interleaved), partner and first table column.
 struct LanePlace { int rot, partner, col; };
+template <bool PAIRS>
 __device__ __forceinline__ LanePlace lane_place(const RopeShape& s, int g) {
   const int c = g * 8;
   if (c < s.off || c >= s.off + 2 * s.P) return {0, g, 0};
-  if (s.interleaved) return {3, g, (c - s.off) / 2};
+  if (PAIRS) return {3, g, (c - s.off) / 2};
   const int step = s.P / 8;
   if (c < s.off + s.P) return {1, g + step, c - s.off};
   return {2, g - step, c - s.off - s.P};
 }
 // The factor of each of the lane's channels and of its partner, rotating forwards (sign 1) or back (-1).
-__device__ __forceinline__ void lane_tables(const RopeShape& s, const LanePlace& p, int64_t t, bool wide, float sign, float* c, float* n) {
+template <bool PAIRS>
+__device__ __forceinline__ void lane_tables(const RopeShape& s, const LanePlace& p, int64_t t, bool wide, float sign, float2* c, float2* n) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { c[i] = 1.f; n[i] = 0.f; }
+  for (int i = 0; i < 4; ++i) {
+    c[i] = make_float2(1.f, 1.f);
+    n[i] = make_float2(0.f, 0.f);
+  }
   if (p.rot == 0) return;
-  if (p.rot == 3) {
-    float c4[4], n4[4];
-    load_table<4>(s.cosb + t * s.ldt, p.col, wide, c4);
-    load_table<4>(s.sinb + t * s.ldt, p.col, wide, n4);
+  constexpr int N = PAIRS ? 4 : 8;
+  float fc[N], fn[N];
+  load_table<N>(s.cosb + t * s.ldt, p.col, wide, fc);
+  load_table<N>(s.sinb + t * s.ldt, p.col, wide, fn);
+  const float f = PAIRS || p.rot == 1 ? -sign : sign;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[2 * i] = c[2 * i + 1] = c4[i];
-      n[2 * i] = -sign * n4[i];
-      n[2 * i + 1] = sign * n4[i];
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (PAIRS) {
+      c[i] = make_float2(fc[i], fc[i]);
+      n[i] = mul2(make_float2(fn[i], fn[i]), make_float2(f, -f));
+    } else {
+      c[i] = make_float2(fc[2 * i], fc[2 * i + 1]);
+      n[i] = mul2(make_float2(fn[2 * i], fn[2 * i + 1]), make_float2(f, f));
     }
-  } else {
-    load_table<8>(s.cosb + t * s.ldt, p.col, wide, c);
-    load_table<8>(s.sinb + t * s.ldt, p.col, wide, n);
-    const float f = p.rot == 1 ? -sign : sign;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) n[i] *= f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void lane_weight(const void* w, int c, int d, float shift, float* f) {
+__device__ __forceinline__ void lane_weight(const void* w, int c, int d, float shift, float2* f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = 1.f;
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(1.f, 1.f);
   if (w == nullptr || c >= d) return;
-  load_vec<T, 8>(reinterpret_cast<const T*>(w) + c, f);
+  Raw<T, 8> r;
+  r.load(reinterpret_cast<const T*>(w) + c);
+  get2(r, f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] += shift;
+  for (int i = 0; i < 4; ++i) f[i] = add2(f[i], make_float2(shift, shift));
 }
 // The partners of the lane's 8 channels (pairs x).
 template <typename T, int G, bool PAIRS>
@@ -318,8 +325,8 @@ __device__ __forceinline__ void partners(const Raw<T, 8>& raw, const float2* x, 
   }
 }
 
-// A group takes HB heads of one token, `shares` apart; their loads are issued before the tables' and weights', so a warp waits for memory once.
-// blockIdx.y: queries or keys.
+// A group takes every shares-th head of one token, HB at a time; the loads of the next HB are issued before these are used, the first before the
+// tables' and weights'. Two at a time: four take 115 registers, and then two blocks an SM (43 us instead of 32). blockIdx.y: queries or keys.
 template <typename T, int G, bool PAIRS, int HB>
 __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid_constant__ NormArgs a, int q_shares, int k_shares) {
   const RopeShape& s = a.s;
@@ -333,158 +340,166 @@ __global__ void __launch_bounds__(256) qk_norm_rope_part_fwd_kernel(const __grid
   const int share = (int)(item - token * shares);
   const bool live = token < (unsigned)s.T, on = live && g * 8 < s.d;
   const int64_t t = live ? token : s.T - 1;             // the whole warp stays in the shuffles
-  const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + g * 8;
-  Raw<T, 8> raw[HB];
+  const T* px = reinterpret_cast<const T*>(o.x) + t * o.x_tok + share * o.x_head + g * 8;
+  T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + share * o.y_head + g * 8;
+  const int64_t x_step = o.x_head * shares, y_step = o.y_head * shares;
+  const int each = (o.H + (int)shares - 1) / (int)shares, mine = on ? (o.H - share + (int)shares - 1) / (int)shares : 0;    // heads: at most; this group's
+  Raw<T, 8> raw[HB], ahead[HB];
 #pragma unroll
   for (int i = 0; i < HB; ++i) {
     raw[i].zero();
-    if (on && share + i * (int)shares < o.H) raw[i].load(px + (int64_t)(share + i * (int)shares) * o.x_head);
+    if (i < mine) raw[i].load(px + i * x_step);
   }
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
-  const LanePlace p = lane_place(s, g);
+  const LanePlace p = lane_place<PAIRS>(s, g);
   float2 cw[4], nw[4];
   {
-    float c[8], n[8], w[8], wp[8];
-    lane_tables(s, p, t, wide, 1.f, c, n);
+    float2 w[4], wp[4];
+    lane_tables<PAIRS>(s, p, t, wide, 1.f, cw, nw);
     lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
-    lane_weight<T>(o.w, p.partner * 8, s.d, a.shift, wp);
+    if (PAIRS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wp[j] = make_float2(w[j].y, w[j].x);
+    } else {
+      lane_weight<T>(o.w, p.partner * 8, s.d, a.shift, wp);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      cw[j] = make_float2(c[2 * j] * w[2 * j], c[2 * j + 1] * w[2 * j + 1]);
-      nw[j] = make_float2(n[2 * j] * wp[PAIRS ? 2 * j + 1 : 2 * j], n[2 * j + 1] * wp[PAIRS ? 2 * j : 2 * j + 1]);
+      cw[j] = mul2(cw[j], w[j]);
+      nw[j] = mul2(nw[j], wp[j]);
     }
   }
   const float inv_d = 1.f / (float)s.d;
-  float sq[HB];
+  for (int first = 0; first < each; first += HB) {
 #pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    float2 x[4], q = make_float2(0.f, 0.f);
-    get2(raw[i], x);
+    for (int i = 0; i < HB; ++i) {
+      ahead[i].zero();
+      if (first + HB + i < mine) ahead[i].load(px + (first + HB + i) * x_step);
+    }
+    float sq[HB];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q = fma2(x[j], x[j], q);
-    sq[i] = q.x + q.y;
-  }
+    for (int i = 0; i < HB; ++i) {
+      float2 x[4], q = make_float2(0.f, 0.f);
+      get2(raw[i], x);
 #pragma unroll
-  for (int m = G / 2; m > 0; m >>= 1)
+      for (int j = 0; j < 4; ++j) q = fma2(x[j], x[j], q);
+      sq[i] = q.x + q.y;
+    }
 #pragma unroll
-    for (int i = 0; i < HB; ++i) sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
-  T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
+    for (int m = G / 2; m > 0; m >>= 1)
 #pragma unroll
-  for (int i = 0; i < HB; ++i) {
-    float2 x[4], q[4];
-    get2(raw[i], x);
-    partners<T, G, PAIRS>(raw[i], x, p.partner, q);
-    const float r = rsqrtf(sq[i] * inv_d + a.eps);
+      for (int i = 0; i < HB; ++i) sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = mul2(make_float2(r, r), fma2(x[j], cw[j], mul2(q[j], nw[j])));
-    if (on && share + i * (int)shares < o.H) store2(py + (int64_t)(share + i * (int)shares) * o.y_head, x);
+    for (int i = 0; i < HB; ++i) {
+      float2 x[4], q[4];
+      get2(raw[i], x);
+      partners<T, G, PAIRS>(raw[i], x, p.partner, q);
+      const float r = rsqrtf(sq[i] * inv_d + a.eps);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = mul2(make_float2(r, r), fma2(x[j], cw[j], mul2(q[j], nw[j])));
+      if (first + i < mine) store2(py + (first + i) * y_step, x);
+      raw[i] = ahead[i];
+    }
   }
 }
 
-// The same split for the gradient; a group walks over a run of items (token, share), reads the tables where the token changes and holds its sums of
-// the weight's gradient. The operands of the next item are fetched before this one's sums are taken.
+// The same split for the gradient. A chunk is a part (`parts` of them) of a token's shares; the groups take chunks in turn, so that neighbouring groups
+// read neighbouring memory at a time, and walk over a chunk's shares, HB heads each. The operands of the next heads are fetched before these sums
+// are taken; a group holds its sums of the weight's gradient.
 template <typename T, int G, bool PAIRS, int HB>
-__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares) {
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_part_bwd_kernel(const __grid_constant__ NormArgs a, int shares, int parts) {
   const RopeShape& s = a.s;
   const NormOperand& o = a.q;
   constexpr int GPB = 256 / G;
   __shared__ float sums[GPB][G * 8 + 4];
-  const unsigned items = (unsigned)s.T * shares, groups = gridDim.x * GPB;
+  const unsigned groups = gridDim.x * GPB, chunks = (unsigned)s.T * parts;
+  const int per = (shares + parts - 1) / parts;          // shares of a chunk
   const int g = threadIdx.x % G, grp = threadIdx.x / G;
   const bool in = g * 8 < s.d;
   const bool wide = !((reinterpret_cast<uintptr_t>(s.cosb) | reinterpret_cast<uintptr_t>(s.sinb)) & 15) && (s.ldt & 3) == 0;
-  const LanePlace p = lane_place(s, g);
+  const LanePlace p = lane_place<PAIRS>(s, g);
   const float inv_d = 1.f / (float)s.d;
-  const unsigned each = items / groups, more = items % groups, me = blockIdx.x * GPB + grp;      // the first `more` groups have one item more
-  unsigned item = me * each + (me < more ? me : more);
-  const unsigned end = item + each + (me < more ? 1 : 0), rounds = each + (more ? 1 : 0);      // rounds: the same for the whole block
   float2 dw[4], w[4], c[4], n[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) dw[i] = c[i] = n[i] = make_float2(0.f, 0.f);
+  for (int i = 0; i < 4; ++i) dw[i] = make_float2(0.f, 0.f);
+  lane_weight<T>(o.w, g * 8, s.d, a.shift, w);
   Raw<T, 8> rx[HB], rd[HB];
-  int64_t t = item / (unsigned)shares, tables_of = -1;
-  int share = (int)(item - (unsigned)t * shares);
+  // operands of the heads of `share` in token t
   auto fetch = [&](bool valid, int64_t tok, int sh, Raw<T, 8>* x, Raw<T, 8>* d) {
-    const T* px = reinterpret_cast<const T*>(o.x) + tok * o.x_tok + g * 8;
-    const T* pd = reinterpret_cast<const T*>(o.dy) + tok * o.dy_tok + g * 8;
+    const T* px = reinterpret_cast<const T*>(o.x) + tok * o.x_tok + sh * o.x_head + g * 8;
+    const T* pd = reinterpret_cast<const T*>(o.dy) + tok * o.dy_tok + sh * o.dy_head + g * 8;
 #pragma unroll
     for (int i = 0; i < HB; ++i) {
       x[i].zero();
       d[i].zero();
       if (valid && sh + i * shares < o.H) {
-        x[i].load(px + (int64_t)(sh + i * shares) * o.x_head);
-        d[i].load(pd + (int64_t)(sh + i * shares) * o.dy_head);
+        x[i].load(px + i * (shares * o.x_head));
+        d[i].load(pd + i * (shares * o.dy_head));
       }
     }
   };
-  fetch(in && item < end, t, share, rx, rd);
-  {
-    float f[8];
-    lane_weight<T>(o.w, g * 8, s.d, a.shift, f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = make_float2(f[2 * i], f[2 * i + 1]);
-  }
-  for (unsigned round = 0; round < rounds; ++round, ++item) {
-    const bool live = in && item < end;
-    if (item < end && t != tables_of) {
-      float fc[8], fn[8];
-      lane_tables(s, p, t, wide, -1.f, fc, fn);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        c[i] = make_float2(fc[2 * i], fc[2 * i + 1]);
-        n[i] = make_float2(fn[2 * i], fn[2 * i + 1]);
-      }
-      tables_of = t;
-    }
-    const bool wrap = share + 1 == shares;
-    const int64_t nt = wrap ? t + 1 : t;
-    const int nshare = wrap ? 0 : share + 1;
-    Raw<T, 8> nx[HB], nd[HB];
-    fetch(in && item + 1 < end, nt, nshare, nx, nd);
-    float2 d[HB][4];
-    float sq[HB], dot[HB];
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      float2 x[4], q[4], e[4], s2 = make_float2(0.f, 0.f), d2 = s2;
-      get2(rd[i], e);
-      partners<T, G, PAIRS>(rd[i], e, p.partner, q);
-      get2(rx[i], x);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        d[i][j] = fma2(e[j], c[j], mul2(q[j], n[j]));
-        s2 = fma2(x[j], x[j], s2);
-        d2 = fma2(mul2(d[i][j], w[j]), x[j], d2);
-      }
-      sq[i] = s2.x + s2.y;
-      dot[i] = d2.x + d2.y;
-    }
-#pragma unroll
-    for (int m = G / 2; m > 0; m >>= 1)
+  unsigned chunk = blockIdx.x * GPB + grp;
+  int64_t t = chunk / (unsigned)parts;
+  int begin = (int)(chunk - (unsigned)t * parts) * per;
+  fetch(in && chunk < chunks && begin < shares, t, begin, rx, rd);
+  // every group of the block runs as many rounds: whole warps stay in the shuffles
+  for (unsigned round = 0; round < chunks; round += groups) {
+    const bool on = in && chunk < chunks;
+    const int64_t tok = t;
+    const int from = begin;
+    chunk += groups;
+    t = chunk / (unsigned)parts;
+    begin = (int)(chunk - (unsigned)t * parts) * per;
+    lane_tables<PAIRS>(s, p, on ? tok : 0, wide, -1.f, c, n);
+    for (int step = 0; step < per; ++step) {
+      const int share = from + step;
+      const bool live = on && share < shares, last = step + 1 == per;
+      Raw<T, 8> nx[HB], nd[HB];
+      const int nshare = last ? begin : share + 1;
+      fetch(in && nshare < shares && (last ? chunk < chunks : on), last ? t : tok, nshare, nx, nd);
+      float2 d[HB][4];
+      float sq[HB], dot[HB];
 #pragma unroll
       for (int i = 0; i < HB; ++i) {
-        sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
-        dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], m);
-      }
-    T* py = reinterpret_cast<T*>(o.y) + t * o.y_tok + g * 8;
-#pragma unroll
-    for (int i = 0; i < HB; ++i) {
-      if (live && share + i * shares < o.H) {            // a dead head's r may be infinite (eps 0)
-        const float r = rsqrtf(sq[i] * inv_d + a.eps), k = -(dot[i] * inv_d * r * r * r);
-        float2 x[4], out[4];
+        float2 x[4], q[4], e[4], s2 = make_float2(0.f, 0.f), d2 = s2;
+        get2(rd[i], e);
+        partners<T, G, PAIRS>(rd[i], e, p.partner, q);
         get2(rx[i], x);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 dr = mul2(d[i][j], make_float2(r, r));
-          dw[j] = fma2(dr, x[j], dw[j]);
-          out[j] = fma2(dr, w[j], mul2(x[j], make_float2(k, k)));
+          d[i][j] = fma2(e[j], c[j], mul2(q[j], n[j]));
+          s2 = fma2(x[j], x[j], s2);
+          d2 = fma2(mul2(d[i][j], w[j]), x[j], d2);
         }
-        store2(py + (int64_t)(share + i * shares) * o.y_head, out);
+        sq[i] = s2.x + s2.y;
+        dot[i] = d2.x + d2.y;
       }
-      rx[i] = nx[i];
-      rd[i] = nd[i];
+#pragma unroll
+      for (int m = G / 2; m > 0; m >>= 1)
+#pragma unroll
+        for (int i = 0; i < HB; ++i) {
+          sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], m);
+          dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], m);
+        }
+      T* py = reinterpret_cast<T*>(o.y) + tok * o.y_tok + share * o.y_head + g * 8;
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        if (live && share + i * shares < o.H) {          // a dead head's r may be infinite (eps 0)
+          const float r = rsqrtf(sq[i] * inv_d + a.eps), k = -(dot[i] * inv_d * r * r * r);
+          float2 x[4], out[4];
+          get2(rx[i], x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 dr = mul2(d[i][j], make_float2(r, r));
+            dw[j] = fma2(dr, x[j], dw[j]);
+            out[j] = fma2(dr, w[j], mul2(x[j], make_float2(k, k)));
+          }
+          store2(py + i * (shares * o.y_head), out);
+        }
+        rx[i] = nx[i];
+        rd[i] = nd[i];
+      }
     }
-    t = nt;
-    share = nshare;
   }
   if (a.partial == nullptr) return;
   if (in) {
@@ -795,14 +810,14 @@ static int norm_form(const NormArgs& a, int size, bool bwd) {
   const bool aligned = !((reinterpret_cast<uintptr_t>(a.q.w) | reinterpret_cast<uintptr_t>(a.k.w)) & 15);
   return aligned && div_by(8, {s.d, s.off, s.interleaved ? 2 * s.P : s.P}) && norm_vec(a, size, bwd) == 16 / size ? 2 : 1;
 }
-// Heads per group: loads in flight and tables read seldom, or one where there are too few tokens to fill the machine that way. Forward up to four,
-// backward two (registers).
+// Heads per group (a power of two): loads in flight and tables read seldom, or one where there are too few tokens to fill the machine that way; more
+// than four only where the machine is filled three times. Forward up to eight, read two at a time, backward two (registers).
 static int norm_lanes(int d) { return d > 128 ? 32 : d > 64 ? 16 : 8; }
 static int norm_heads(const NormArgs& a, int H, int most) {
-  int n = H < most ? H : most;
-  if (n == 3) n = 4;
-  while (n > 1 && (int64_t)a.s.T * ((H + n - 1) / n) * norm_lanes(a.s.d) < (int64_t)sm_count() * 1024) n /= 2;
-  return n > 1 ? n : 1;
+  int n = 1;
+  while (n < most && n < H) n *= 2;
+  while (n > 1 && (int64_t)a.s.T * ((H + n - 1) / n) * norm_lanes(a.s.d) < (int64_t)sm_count() * (n > 4 ? 3072 : 1024)) n /= 2;
+  return n;
 }
 static int norm_bwd_grid(const NormArgs& a, int form) {
   const int n = norm_heads(a, a.q.H, 2), H = a.q.H;
@@ -817,7 +832,7 @@ static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
   const int form = norm_form(a, sizeof(T), false);
   if (form) {
     const int G = form == 2 ? norm_lanes(a.s.d) : a.s.d > 128 ? 32 : 16, H = a.q.H > a.k.H ? a.q.H : a.k.H;
-    const int n = form == 2 ? norm_heads(a, H, 4) : kGatherHeads;
+    const int n = form == 2 ? norm_heads(a, H, 8) : kGatherHeads, hb = n < 2 ? n : 2;
     const int qs = a.q.H ? (a.q.H + n - 1) / n : 1, ks = a.k.H ? (a.k.H + n - 1) / n : 1;
     const int64_t items = (int64_t)a.s.T * (qs > ks ? qs : ks);
     if (items > 0x7fffff00) return -10;
@@ -828,8 +843,8 @@ static int norm_fwd(const NormArgs& a, cudaStream_t stream) {
     const int s0 = a.q.H ? qs : ks, vl = norm_vec(a, sizeof(T), false);
     if (form == 2) {
 #define LLMT_QK(L, I, N) \
-  if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_fwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(b, s0, ks);
-#define LLMT_QK3(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2) LLMT_QK(L, I, 4)
+  if (G == L && (bool)a.s.interleaved == I && hb == N) qk_norm_rope_part_fwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(b, s0, ks);
+#define LLMT_QK3(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2)
       LLMT_QK3(32, true) LLMT_QK3(32, false) LLMT_QK3(16, true) LLMT_QK3(16, false) LLMT_QK3(8, true) LLMT_QK3(8, false)
 #undef LLMT_QK3
 #undef LLMT_QK
@@ -855,8 +870,11 @@ static int norm_bwd(const NormArgs& a, int P, void* dw, cudaStream_t stream) {
     const int n = form == 2 ? norm_heads(a, a.q.H, 2) : kGatherHeads, shares = (a.q.H + n - 1) / n, vl = norm_vec(a, sizeof(T), true);
     if ((int64_t)a.s.T * shares > 0x7fffff00) return -10;
     if (form == 2) {
+      // a token at a time, or parts of one while the groups have fewer than six chunks each (the last round would be a large part of the time)
+      int parts = 1;
+      while (2 * parts <= shares && (int64_t)a.s.T * parts < (int64_t)6 * grid * (256 / G)) parts *= 2;
 #define LLMT_QK(L, I, N) \
-  if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_bwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(a, shares);
+  if (G == L && (bool)a.s.interleaved == I && n == N) qk_norm_rope_part_bwd_kernel<T, L, I, N><<<grid, 256, 0, stream>>>(a, shares, parts);
 #define LLMT_QK2(L, I) LLMT_QK(L, I, 1) LLMT_QK(L, I, 2)
       LLMT_QK2(32, true) LLMT_QK2(32, false) LLMT_QK2(16, true) LLMT_QK2(16, false) LLMT_QK2(8, true) LLMT_QK2(8, false)
 #undef LLMT_QK2
