@@ -183,3 +183,14 @@ def test_scaled_qwen3_logits_are_those_of_the_library():
         got = ours(tok, ours.build_context(torch.arange(200), AttnMeta.build(torch.tensor([0, 200]), causal=True)))
         want = theirs(input_ids=tok[None], use_cache=False).logits[0]
     assert torch.allclose(got.float(), want, atol=2e-5), (got - want).abs().max()
+
+
+def test_refusals_name_what_does_not_fit():
+    from torchllmtuner_b200.errors import ConfigError
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    with pytest.raises(ConfigError, match="residual"):
+        ops.linear_act(x, w, residual=torch.zeros(5, 6))
+    with pytest.raises(ConfigError, match="positions"):
+        ops.rope_tables([0, 1, 2], 8, 1e4, scaling={"rope_type": "linear", "factor": 2.0})
+    with pytest.raises(ConfigError, match="positions"):
+        ops.rope_tables(torch.zeros(2, 3, dtype=torch.int64), 8, 1e4, scaling={"rope_type": "linear", "factor": 2.0})

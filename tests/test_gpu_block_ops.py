@@ -693,3 +693,16 @@ def test_linear_act_gradient_into_an_owners_buffer(act):
     # the sum of two equal gradients, each product rounded once: the second launch adds to the rounded first
     want = 2 * plain[0][1].double()
     assert ((leaves[1].main_grad.double() - want).abs() <= want.abs() * 3 * 2.0 ** -8 + want.abs().max() * 2.0 ** -16).all()
+
+
+def test_scaled_tables_under_another_default_device():
+    """The frequencies are kept on the host whatever device new tensors go to; a residual that fits nothing is named on the device too."""
+    from torchllmtuner_b200 import ops
+    from torchllmtuner_b200.errors import ConfigError
+    scaling = {"rope_type": "linear", "factor": 3.5}
+    with torch.device(DEV):
+        cos, sin = ops.rope_tables(torch.arange(50), 48, 5e4, scaling=scaling)
+    ang = torch.arange(50, dtype=torch.float64)[:, None] * torch.tensor([5e4 ** (-2 * j / 48) / 3.5 for j in range(24)], dtype=torch.float64)
+    assert (cos.cpu().double() - ang.cos()).abs().max() < 2.0 ** -22 and (sin.cpu().double() - ang.sin()).abs().max() < 2.0 ** -22
+    with pytest.raises(ConfigError, match="residual"):
+        ops.linear_act(_rand(4, 8), _rand(6, 8), residual=_rand(5, 6))

@@ -1349,9 +1349,12 @@ int64_t row_pitch(int64_t n) {
 }
 Tensor tma_rows(const Tensor& t) {
   if ((t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0) return t;
-  Tensor r = torch::empty({t.size(0), row_pitch(t.size(1))}, t.options()).narrow(1, 0, t.size(1));
-  r.copy_(t);
-  return r;
+  // columns first, or rows that overlap: brought to rows by the library's copy
+  const Tensor rows = (t.size(1) == 1 || t.stride(1) == 1) ? t : t.contiguous();
+  Tensor r = fresh({t.size(0), row_pitch(t.size(1))}, at::kBFloat16, t);
+  check_rc(llmt_linear_pad(rows.data_ptr(), rows.stride(0), r.data_ptr(), r.stride(0), int_of(t.size(0), "rows"), int_of(t.size(1), "features"), cur_stream()),
+           "llmt_linear_pad", t.numel() > 0);
+  return r.narrow(1, 0, t.size(1));
 }
 // Partial sums of a product that is cut along its depth; of this call alone, so graphs and streams share nothing.
 Tensor linear_workspace(int64_t M, int64_t N, int64_t K, const Tensor& a, const Tensor& b, bool gradient, int64_t act, bool res, bool pre) {

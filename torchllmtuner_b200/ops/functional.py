@@ -13,8 +13,8 @@ from torch.autograd import forward_ad
 
 from . import reference as ref
 from ..errors import ConfigError, UnsupportedCombinationError
-from .validation import (validate_attention_inputs, validate_layer_norm_inputs, validate_linear_act_inputs, validate_qk_inputs, validate_rms_norm_inputs,
-                         validate_rope_scaling, validate_rotary_inputs)
+from .validation import (require_tensor, validate_attention_inputs, validate_layer_norm_inputs, validate_linear_act_inputs, validate_qk_inputs,
+                         validate_rms_norm_inputs, validate_rope_scaling, validate_rotary_inputs)
 from .attn_meta import AttnMeta
 from .cuda_ext import load as _ext
 
@@ -387,7 +387,7 @@ def _frequencies(head_dim: int, theta: float, items: tuple):
     """Scaled inverse frequencies (64-bit tensor on the host) and the factor on both tables."""
     scaling = validate_rope_scaling(dict(items))
     inv, factor = ref.scaled_frequencies(head_dim, theta, scaling)
-    return torch.tensor(inv, dtype=torch.float64), factor
+    return torch.tensor(inv, dtype=torch.float64, device="cpu"), factor
 
 
 def rope_tables(positions, head_dim: int, theta: float, dtype=torch.float32, scaling=None):
@@ -396,8 +396,9 @@ def rope_tables(positions, head_dim: int, theta: float, dtype=torch.float32, sca
     original_max_position_embeddings, optionally beta_fast, beta_slow, truncate, attention_factor, mscale, mscale_all_dim); its angles are taken in 64 bits."""
     if scaling is None:
         return ref.rope_tables(positions, head_dim, theta, dtype)
-    if head_dim < 2 or head_dim % 2 or not theta > 1 or positions.dim() != 1:
-        raise ConfigError(f"rotary tables need positions [T], an even head width and theta > 1; got {tuple(positions.shape)}, {head_dim}, {theta}")
+    require_tensor(positions, "positions", dims=1)
+    if head_dim < 2 or head_dim % 2 or not theta > 1:
+        raise ConfigError(f"rotary tables need an even head width and theta > 1; got {head_dim} and {theta}")
     if not (positions.is_cuda and positions.dtype in (torch.int64, torch.int32) and head_dim <= 512 and _has_rules(positions)):
         return ref.rope_tables(positions, head_dim, theta, dtype, validate_rope_scaling(scaling))
     try:

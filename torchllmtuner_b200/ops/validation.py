@@ -111,6 +111,11 @@ def validate_linear_act_inputs(x, w, bias, activation, residual, activations) ->
     if residual is not None:
         require_tensor(residual, "residual")
         require_same_device(("x", x), ("residual", residual))
+        shape = (*x.shape[:-1], w.shape[0])
+        try:
+            torch.broadcast_shapes(residual.shape, shape)
+        except RuntimeError:
+            raise ConfigError(f"residual {tuple(residual.shape)} does not broadcast with the result {shape}") from None
 
 
 ROPE_SCALINGS = ("linear", "llama3", "yarn")
