@@ -490,10 +490,31 @@ __global__ void __launch_bounds__(32 * kJoinWarps) linear_join_kernel(const __gr
   finish_patch<FWD, ACT, RES>(a.out, stage[wid], lane, row0, col0, a.out.N, acc);
 }
 
-// ------------------------------------------------------------------------------------------ rows for TMA
-// Rows of any pitch and 2-byte start into rows on 16 bytes: eight columns per thread, from the five aligned words that hold them (a word has at least
-// one element of the row, so it lies in the same page), shifted by two bytes where the row starts on an odd element. Columns from N on are not
-// read by TMA. 9000 x 1001: 8 us (the library's strided copy took 24).
+// ------------------------------------------------------------------------------------------ rows of any start
+// Eight elements from p, of which `n` belong to the row: read as the five aligned words that hold them (a word is read only if it has an element of the
+// row, so it lies in the same page) and shifted by two bytes where the row starts on an odd element. Elements from `n` on are foreign.
+struct Shifted {
+  uint32_t w[5];
+  bool odd;
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = 0u;
+    odd = false;
+  }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int n) {
+    odd = reinterpret_cast<uintptr_t>(p) & 2;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+    const int have = min(n, 8) + odd;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = 2 * i < have ? q[i] : 0u;
+  }
+  __device__ __forceinline__ void get(Raw<__nv_bfloat16, 8>& r) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = odd ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  }
+};
+// Rows of any pitch and start into rows on 16 bytes, for TMA, which does not read the columns from N on. 9000 x 1001: 8 us (the library's strided
+// copy took 24).
 constexpr int kPadRows = 4;                              // rows in flight per thread
 __global__ void __launch_bounds__(256) linear_pad_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, __nv_bfloat16* __restrict__ y, int64_t ldy,
                                                          int M, int N) {
@@ -501,27 +522,18 @@ __global__ void __launch_bounds__(256) linear_pad_kernel(const __nv_bfloat16* __
   if (col >= N) return;
   const int64_t step = (int64_t)gridDim.y * 8;
   for (int64_t row = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); row < M; row += kPadRows * step) {
-    uint32_t w[kPadRows][5];
-    bool odd[kPadRows];
+    Shifted v[kPadRows];
 #pragma unroll
     for (int u = 0; u < kPadRows; ++u) {
-      const __nv_bfloat16* p = x + (row + u * step) * ldx + col;
-      odd[u] = reinterpret_cast<uintptr_t>(p) & 2;
-      const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
-      const int have = min(N - col, 8) + odd[u];         // elements from the first word's start
-#pragma unroll
-      for (int i = 0; i < 5; ++i) {
-        w[u][i] = 0u;
-        if (row + u * step < M && 2 * i < have) w[u][i] = q[i];
-      }
+      v[u].zero();
+      if (row + u * step < M) v[u].load(x + (row + u * step) * ldx + col, N - col);
     }
 #pragma unroll
     for (int u = 0; u < kPadRows; ++u) {
       if (row + u * step >= M) break;
-      uint32_t o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = odd[u] ? __funnelshift_r(w[u][i], w[u][i + 1], 16) : w[u][i];
-      *reinterpret_cast<uint4*>(y + (row + u * step) * ldy + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      Raw<__nv_bfloat16, 8> r;
+      v[u].get(r);
+      r.store(y + (row + u * step) * ldy + col);
     }
   }
 }
@@ -532,7 +544,7 @@ __global__ void __launch_bounds__(256) linear_pad_kernel(const __nv_bfloat16* __
 // sums per block go to partial [blocks][N] and linear_db_kernel adds them; clusters of eight would leave SMs idle then (a GPC's 16 or 18 SMs hold
 // two of them: half of the machine's time at 16384 x 4608).
 constexpr int kStripBlocks = 8;
-// z and dz have rows on 16 bytes (the caller's buffers); dy may lie anywhere (VEC false): then its values are read one by one.
+// z and dz have rows on 16 bytes (the caller's buffers); dy may lie anywhere (VEC false, see Shifted).
 template <bool VEC, int LANES, bool CLUSTER, int ACT>
 __global__ void __launch_bounds__(256, ACT == kActNone ? 4 : 3) linear_dz_kernel(const __nv_bfloat16* __restrict__ dy, int64_t ldy,
                                                                                 const __nv_bfloat16* __restrict__ z, int64_t ldz,
@@ -548,42 +560,34 @@ __global__ void __launch_bounds__(256, ACT == kActNone ? 4 : 3) linear_dz_kernel
 #pragma unroll
   for (int j = 0; j < W; ++j) acc[j] = make_float2(0.f, 0.f);
   if (col < N) {
-    constexpr int U = VEC ? 4 : 2;                       // rows in flight per thread
+    constexpr int U = 4;                                 // rows in flight per thread
     const int64_t step = (int64_t)ROWS * gridDim.y;
     for (int64_t row = (int64_t)blockIdx.y * ROWS + sub; row < M; row += U * step) {
-      Raw<__nv_bfloat16, V> rg[VEC ? U : 1], rz[U];
-      float gs[VEC ? 1 : U][V];
+      Raw<__nv_bfloat16, V> rg[U], rz[U];
+      Shifted sg[VEC ? 1 : U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         rz[u].zero();
         if constexpr (VEC) rg[u].zero();
-        else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) gs[u][j] = 0.f;
-        }
+        else sg[u].zero();
         if (row + u * step < M) {
           if constexpr (VEC) rg[u].load(dy + (row + u * step) * ldy + col);
-          else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-              if (col + j < N) load_vec<__nv_bfloat16, 1>(dy + (row + u * step) * ldy + col + j, &gs[u][j]);
-          }
+          else sg[u].load(dy + (row + u * step) * ldy + col, N - col);
           if (ACT != kActNone) rz[u].load(z + (row + u * step) * ldz + col);
         }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float g[V], p[V], out[V];
-        if constexpr (VEC) rg[u].get(g);
+        if constexpr (!VEC) sg[u].get(rg[u]);
+        rg[u].get(g);
         if (ACT != kActNone) rz[u].get(p);
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-          float2 v = VEC ? make_float2(g[2 * j], g[2 * j + 1]) : make_float2(gs[VEC ? 0 : u][2 * j], gs[VEC ? 0 : u][2 * j + 1]);
-          if (ACT != kActNone) {
-            v = activate_grad<ACT>(make_float2(p[2 * j], p[2 * j + 1]), v);
-            if (!VEC && col + 2 * j >= N) v.x = 0.f;     // behind the last column z was never written
-            if (!VEC && col + 2 * j + 1 >= N) v.y = 0.f;
-          }
+          float2 v = make_float2(g[2 * j], g[2 * j + 1]);
+          if (ACT != kActNone) v = activate_grad<ACT>(make_float2(p[2 * j], p[2 * j + 1]), v);
+          if (!VEC && col + 2 * j >= N) v.x = 0.f;       // behind the last column lie the next row's dy and a z that was never written
+          if (!VEC && col + 2 * j + 1 >= N) v.y = 0.f;
           acc[j] = add2(acc[j], v);                      // rows past the end were loaded as zeros: their gradient is zero
           out[2 * j] = v.x;
           out[2 * j + 1] = v.y;
