@@ -706,3 +706,18 @@ def test_scaled_tables_under_another_default_device():
     assert (cos.cpu().double() - ang.cos()).abs().max() < 2.0 ** -22 and (sin.cpu().double() - ang.sin()).abs().max() < 2.0 ** -22
     with pytest.raises(ConfigError, match="residual"):
         ops.linear_act(_rand(4, 8), _rand(6, 8), residual=_rand(5, 6))
+
+
+@pytest.mark.parametrize("start", [1, 2, 3, 8])
+@pytest.mark.parametrize("M,K,N", [(37, 1, 9), (130, 63, 40), (600, 200, 71), (9, 520, 264)])
+def test_linear_act_rows_between_foreign_values(M, K, N, start):
+    """Operands as rows of buffers whose other values are NaN, on odd and even starts and pitches: none of those may reach a result."""
+    def between(rows, cols, seed, std=1.0):
+        buf = torch.full((rows, cols + 2 * start + seed), float("nan"), device=DEV, dtype=torch.bfloat16)
+        buf[:, start:start + cols] = _rand(rows, cols, seed=seed, std=std)
+        return buf[:, start:start + cols].detach()
+    x, w, r, dy = between(M, K, 1), between(N, K, 2, K ** -0.5), between(M, N, 3), between(M, N, 4)
+    b = _rand(N, seed=5)
+    for act in (None, "gelu_tanh"):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        _linear_check(x, w, b, r, act, dy, _linear_run(*leaves, act, dy))

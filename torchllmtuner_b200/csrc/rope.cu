@@ -817,7 +817,7 @@ static int norm_lanes(int d) { return d > 128 ? 32 : d > 64 ? 16 : 8; }
 static int norm_heads(const NormArgs& a, int H, int most) {
   int n = 1;
   while (n < most && n < H) n *= 2;
-  while (n > 1 && (int64_t)a.s.T * ((H + n - 1) / n) * norm_lanes(a.s.d) < (int64_t)sm_count() * (n > 4 ? 3072 : 1024)) n /= 2;
+  while (n > 1 && (int64_t)a.s.T * ((H + n - 1) / n) * norm_lanes(a.s.d) < (int64_t)sm_count() * 1024 * (n > 4 ? 3 : 1)) n /= 2;
   return n;
 }
 static int norm_bwd_grid(const NormArgs& a, int form) {
