@@ -721,3 +721,24 @@ def test_linear_act_rows_between_foreign_values(M, K, N, start):
     for act in (None, "gelu_tanh"):
         leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
         _linear_check(x, w, b, r, act, dy, _linear_run(*leaves, act, dy))
+
+
+def test_saved_tensors_through_the_host():
+    """Offloaded saved tensors come back dense, whatever strides went out: the gradients are the same bits."""
+    from torchllmtuner_b200 import ops
+    ang = torch.rand(90, 12, device=DEV) * 6
+    cos, sin = ang.cos()[:, :10], ang.sin()[:, :10]
+
+    def run():
+        x = _rand(90, 71, seed=1)[:, :67].detach().requires_grad_()
+        w, b = _rand(132, 67, seed=2, std=0.1).requires_grad_(), _rand(132, seed=3).requires_grad_()
+        lw, lb, qw = (_rand(n, seed=i).requires_grad_() for i, n in ((4, 132), (5, 132), (6, 33)))
+        h = ops.layer_norm(ops.linear_act(x, w, b, activation="gelu"), lw, lb, 1e-5)
+        q, k = ops.qk_norm_rope(h.view(90, 4, 33)[:, :3], h.view(90, 4, 33)[:, 3:], qw, None, cos, sin, 1e-6, offset=5, norm=True)
+        y = ops.linear_act(torch.cat((q, ops.rope(k, cos, sin, layout="interleaved", offset=1)), 1).flatten(1), w.t()[:, :132])
+        return [y, *torch.autograd.grad(y, [x, w, b, lw, lb, qw], torch.ones_like(y))]
+    plain = run()
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        moved = run()
+    for i, (a, b) in enumerate(zip(plain, moved)):
+        assert torch.isfinite(a).all() and torch.equal(a, b), i

@@ -1429,7 +1429,8 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     }
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t N = w.size(0), K = w.size(1);
-    Tensor x2 = s[4].defined() ? s[4] : tma_rows(rows_2d(x)), w2 = s[5].defined() ? s[5] : tma_rows(w.stride(1) == 1 ? w : w.contiguous()),
+    // saved-tensor hooks (offload) may bring the kept copies back with other strides
+    Tensor x2 = tma_rows(s[4].defined() ? s[4] : rows_2d(x)), w2 = tma_rows(s[5].defined() ? s[5] : w.stride(1) == 1 ? w : w.contiguous()),
            dy = rows_2d(d[0]);
     const int64_t M = x2.size(0);
     if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
