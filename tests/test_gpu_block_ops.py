@@ -742,3 +742,69 @@ def test_saved_tensors_through_the_host():
         moved = run()
     for i, (a, b) in enumerate(zip(plain, moved)):
         assert torch.isfinite(a).all() and torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("op", ["linear", "layer_norm", "rope", "qk"])
+def test_offsets_past_32_bits(op):
+    """Tensors of more than 2^31 elements: the last rows are those of the same call on the last rows alone, forward and backward."""
+    from torchllmtuner_b200 import ops
+    rows, tail = (1 << 31) // 4096 + 300, 200
+    if op == "linear":
+        x, w = _rand(rows, 64, seed=1), _rand(4096, 64, seed=2, std=0.125)
+        run = lambda t: ops.linear_act(t, w, activation="silu")  # noqa: E731
+    else:
+        x = torch.empty(rows, 4096, device=DEV, dtype=torch.bfloat16).normal_()
+        ang = torch.rand(rows, 32, device=DEV)
+        lw, lb, qw = _rand(4096, seed=3), _rand(4096, seed=4), _rand(256, seed=5)
+        part = lambda t, n: ang[-n:].cos() if t else ang[-n:].sin()  # noqa: E731
+        run = {"layer_norm": lambda t: ops.layer_norm(t, lw, lb, 1e-5),
+               "rope": lambda t: ops.rope(t.view(-1, 16, 256), part(1, len(t)), part(0, len(t)), layout="interleaved", offset=8).view(t.shape),
+               "qk": lambda t: ops.qk_norm_rope(t.view(-1, 16, 256), t.view(-1, 16, 256)[:, :0], qw, None, part(1, len(t)), part(0, len(t)), 1e-6,
+                                                norm=True)[0].reshape(t.shape)}[op]
+    x.requires_grad_()
+    y = run(x)
+    assert y.numel() > 1 << 31
+    dy = torch.empty_like(y).normal_()
+    dx, = torch.autograd.grad(y, x, dy)
+    x2 = x.detach()[-tail:].clone().requires_grad_()
+    y2 = run(x2)
+    dx2, = torch.autograd.grad(y2, x2, dy[-tail:].clone())
+    for name, a, b in (("y", y[-tail:], y2), ("dx", dx[-tail:], dx2)):
+        # other tiles add in another order: each side is off by half a step of bf16, and what is rounded before (z) once more
+        assert torch.equal(a, b) if op != "linear" else (a.double() - b.double()).norm() <= 4 * 2.0 ** -8 * b.double().norm(), name
+    del y, dy, dx
+    torch.cuda.empty_cache()
+
+
+def test_two_threads_on_their_own_streams():
+    """Workspaces and cut tables belong to a call and a thread: two threads at once get the bits of one alone."""
+    import threading
+
+    from torchllmtuner_b200 import ops
+
+    def work(seed):
+        m, k, n = (300, 1200, 520) if seed else (700, 264, 136)
+        x, w, b = _rand(m, k, seed=seed).requires_grad_(), _rand(n, k, seed=seed + 1, std=k ** -0.5).requires_grad_(), _rand(n, seed=seed + 2).requires_grad_()
+        lw, lb = _rand(n, seed=seed + 3).requires_grad_(), _rand(n, seed=seed + 4).requires_grad_()
+        y = ops.layer_norm(ops.linear_act(x, w, b, activation="gelu"), lw, lb, 1e-5)
+        return [t.detach() for t in (y, *torch.autograd.grad(y, [x, w, b, lw, lb], _rand(m, n, seed=seed + 5)))]
+    alone = [work(0), work(1)]
+    got, faults = {}, []
+
+    def repeat(seed):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got[seed] = [work(seed) for _ in range(20)]
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            faults.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=repeat, args=(s,)) for s in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not faults
+    for seed in (0, 1):
+        for run in got[seed]:
+            assert all(torch.equal(a, b) for a, b in zip(run, alone[seed]))
