@@ -1363,6 +1363,12 @@ Tensor linear_workspace(int64_t M, int64_t N, int64_t K, const Tensor& a, const 
 }
 inline float* ws_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 inline int64_t ws_size(const Tensor& t) { return t.defined() ? t.numel() : 0; }
+// (CTAs of a tile, its columns, parts along the depth) of a product: which of the kernels' paths a size takes.
+std::tuple<int, int, int> linear_cut(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, bool gradient, int64_t act, bool res, bool pre) {
+  int c[3];
+  llmt_linear_cut(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), lda, ldb, gradient, (int)act, res, pre, c);
+  return {c[0], c[1], c[2]};
+}
 struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, int64_t act, bool keep) {
     c10::cuda::CUDAGuard guard(x.device());
@@ -1532,6 +1538,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope_part_max_dim", &qk_norm_rope_part_max_dim);
   m.def("qk_norm_rope_part_node", &qk_norm_rope_part_node);
   m.def("linear_act_node", &linear_act_node);
+  m.def("linear_cut", &linear_cut);
   m.def("router_topk", &router_topk);
   m.def("router_topk_bwd", &router_topk_bwd);
   m.def("moe_plan", &moe_plan);

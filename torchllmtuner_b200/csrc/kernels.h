@@ -33,6 +33,7 @@ int llmt_rmsnorm_fwd(const void* x, const void* res, const void* w, void* y, voi
 // ---- linear layers with bias, activation (activations.cuh) and residual (linear_act.cu) ----
 int llmt_linear_pad(const void* x, int64_t ldx, void* y, int64_t ldy, int M, int N, cudaStream_t stream);
 int64_t llmt_linear_ws_floats(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre);
+void llmt_linear_cut(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre, int* out);
 int llmt_linear_act(const void* x, const void* w, void* y, const void* bias, int bias_f32, const void* res, void* pre, int act, int M, int N, int K,
                     int64_t ldx, int64_t ldw, int64_t ldy, int64_t ldres, int64_t ldpre, float* ws, int64_t ws_floats, int* status,
                     cudaStream_t stream);

@@ -897,6 +897,14 @@ extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int64_t lda, int64
   return lin_ws_floats(M, N, lin_cut(M, N, K, lin_kind(gradient != 0, lda, ldb, act, res != 0, pre != 0)));
 }
 
+// How a product with the same arguments is cut: out receives the CTAs of a tile, its columns and the parts along K.
+extern "C" void llmt_linear_cut(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre, int* out) {
+  const LinCut c = lin_cut(M, N, K, lin_kind(gradient != 0, lda, ldb, act < 0 || act >= kActKinds ? 0 : act, res != 0, pre != 0));
+  out[0] = c.cg;
+  out[1] = c.bn;
+  out[2] = c.splits;
+}
+
 // y [M][ldy] = x [M][ldx] (rows of N elements, any pitch and start) for TMA: y and its pitch on 16 bytes, at least N rounded up to a multiple of 8.
 extern "C" int llmt_linear_pad(const void* x, int64_t ldx, void* y, int64_t ldy, int M, int N, cudaStream_t stream) {
   if (M < 0 || N < 0 || (ldy & 7) || ldy < (int64_t)(N + 7) / 8 * 8 || (reinterpret_cast<uintptr_t>(y) & 15) || (reinterpret_cast<uintptr_t>(x) & 1)) return -10;
