@@ -1,8 +1,8 @@
-"""Linear layers whose products take each of the kernels' cuts, special values one row each: against the formulas in 64 bits of test_gpu_block_ops.py and
-under its bounds."""
+"""Linear layers whose products take each of the kernels' cuts, gradients into an owner's buffer at any width, special values one row each: against the
+formulas in 64 bits of test_gpu_block_ops.py and under its bounds."""
 import pytest
 import torch
-from test_gpu_block_ops import DEV, E32, _act64, _linear_check, _linear_run, _rand, _u
+from test_gpu_block_ops import DEV, E32, TYPES, _act64, _linear_check, _linear_run, _near, _rand, _u
 
 pytestmark = pytest.mark.gpu
 
@@ -82,6 +82,57 @@ def test_linear_act_cuts(M, K, N, act, res, cuts):
     r = _rand(M, N, seed=4).requires_grad_() if res else None
     outs = _linear_run(x, w, b, r, act, dy)
     _linear_check(x.detach(), w.detach(), b.detach(), r.detach() if res else None, act, dy, outs)
+
+
+# -------------------------------------------------------------------------------------------- gradients with an owner
+class _Queue:
+    """A collective queue that never gives a product a slice to carry."""
+
+    def __bool__(self):
+        return True
+
+    def take(self, flops):
+        return None, ()
+
+
+@pytest.mark.parametrize("queue", [False, True], ids=["", "queue"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("M,K,N,columns_first", [(300, 201, 137, False), (300, 201, 136, False), (65, 40, 72, True), (130, 33, 7, True), (1, 8, 8, False)])
+def test_owners_buffer_at_any_width(M, K, N, columns_first, act, dtype, queue):
+    """Widths that are no multiple of 8 and weights stored columns first: the weight's gradient is written to `main_grad` by the first micro-batch and
+    added to by the second; x and bias get what they get without an owner."""
+    from torchllmtuner_b200 import ops
+    from torchllmtuner_b200.parallel import symm
+    x, b = _rand(M, K, seed=1).requires_grad_(), _rand(N, seed=3).requires_grad_()
+    w = _rand(K, N, seed=2, std=K ** -0.5).t() if columns_first else _rand(N, K, seed=2, std=K ** -0.5)
+    w = w.detach().requires_grad_()
+    dys = [_rand(M, N, seed=4), _rand(M, N, seed=5)]
+    plain = [_linear_run(x, w, b, None, act, dy) for dy in dys]
+    w.main_grad, w.main_grad_initialized = torch.full((N, K), 7.0, device=DEV, dtype=TYPES[dtype]), False
+    um, total, bound = _u(TYPES[dtype]), 0.0, 0.0
+    z = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    size = x.detach().double().abs() @ w.detach().double().abs().t() + b.detach().double().abs()
+    _, slope, curve = _act64(z, act)
+    for i, dy in enumerate(dys):
+        y = ops.linear_act(x, w, b, activation=act)
+        symm.set_active_queue(_Queue() if queue else None)
+        try:
+            dx, dw, db = torch.autograd.grad(y, (x, w, b), dy, allow_unused=True)
+        finally:
+            symm.set_active_queue(None)
+        assert dw is None and w.main_grad_initialized
+        assert torch.equal(db, plain[i]["db"])
+        # the products add in fp32 in another order: half a step of bf16 on either side of the same sum
+        assert ((dx.double() - plain[i]["dx"].double()).abs() <= 2.02 * _u(torch.bfloat16) * plain[i]["dx"].double().abs() + 2 * (N + 8) * E32 * (
+            (1.2 * dy.double().abs()) @ w.detach().double().abs())).all()
+        dz = dy.double() * slope
+        edz = _u(torch.bfloat16) * dz.abs() + dy.double().abs() * (curve * (_u(torch.bfloat16) * z.abs() + (K + 8) * E32 * size) + 16 * E32 * (1 + z.abs())) if act else torch.zeros_like(dz)
+        total = total + dz.t() @ x.detach().double()
+        # each product's error, and a rounding of the buffer each time
+        bound = bound + edz.t() @ x.detach().double().abs() + (M + 8) * E32 * ((dz.abs() + edz).t() @ x.detach().double().abs())
+        bound = bound + um * (total.abs() + bound) + 1e-30
+        _near(w.main_grad, total, bound, f"main_grad after {i + 1}")
 
 
 # --------------------------------------------------------------------------------------------------- special values

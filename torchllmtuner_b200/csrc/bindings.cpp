@@ -877,19 +877,24 @@ void set_autograd_hooks(const py::object& symm, const py::object& linears_backwa
   h.symm = a.release().ptr();
   h.linears_backward = b.release().ptr();
 }
-// With the GIL held: is a collective queue active, or does one of the weights own a gradient buffer?
-bool python_takes_backward(const variable_list& ws) {
+// With the GIL held: is a collective queue active?
+bool queue_active() {
   const PyHooks& h = py_hooks();
   TORCH_CHECK(h.symm != nullptr && h.linears_backward != nullptr, "set_autograd_hooks was not called");
   py::object active = py::reinterpret_steal<py::object>(PyObject_GetAttrString(h.symm, "_ACTIVE"));
   if (!active) throw py::error_already_set();
-  if (!active.is_none()) return true;
-  for (const Tensor& w : ws) {
-    py::object pw = py::reinterpret_steal<py::object>(THPVariable_Wrap(w));
-    if (!pw) throw py::error_already_set();
-    if (!PyObject_HasAttrString(pw.ptr(), "main_grad")) continue;
-    if (!py::object(pw.attr("main_grad")).is_none()) return true;
-  }
+  return !active.is_none();
+}
+// With the GIL held: does the weight own a gradient buffer?
+bool has_grad_buffer(const Tensor& w) {
+  py::object pw = py::reinterpret_steal<py::object>(THPVariable_Wrap(w));
+  if (!pw) throw py::error_already_set();
+  return PyObject_HasAttrString(pw.ptr(), "main_grad") && !py::object(pw.attr("main_grad")).is_none();
+}
+bool python_takes_backward(const variable_list& ws) {
+  if (queue_active()) return true;
+  for (const Tensor& w : ws)
+    if (has_grad_buffer(w)) return true;
   return false;
 }
 
@@ -1416,7 +1421,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     // needs_input_grad counts the tensors that were given
     if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(b.defined() ? 3 : 2)) out[3] = d[0];
     if (!nx && !nw && !nb) return out;
-    bool python_side = false;
+    bool queue = false, owned = false;
     {
       py::gil_scoped_acquire gil;
       if (beyond_kernels(d)) {
@@ -1427,7 +1432,8 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
         return out;
       }
       try {
-        python_side = python_takes_backward({w});
+        queue = queue_active();
+        owned = nw && has_grad_buffer(w);
       } catch (py::error_already_set& e) {
         e.restore();
         throw python_error();
@@ -1453,28 +1459,33 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
                "llmt_linear_dz", P > 0 ? 2 : 1);
     }
     if (!nx && !nw) return out;
-    if (python_side) {                     // a pending collective rides on the products, or the weight's gradient goes to its owner's buffer
+    // A product in Python: a pending collective rides on it, or the weight's gradient goes to its owner's buffer. `rows`: the weight as the product
+    // reads it, or the parameter itself, whose buffer and type the gradient has.
+    auto in_python = [&](const Tensor& rows, bool input) {
       py::gil_scoped_acquire gil;
       try {
         py::object fn = py::reinterpret_borrow<py::object>(py_hooks().linears_backward);
-        auto r = fn(x2, variable_list{w}, variable_list{dz.narrow(1, 0, N)}, nx, std::vector<bool>{nw}).cast<std::vector<OptTensor>>();
-        if (r[0].has_value()) out[0] = r[0]->reshape(x.sizes());
-        if (r[1].has_value()) out[1] = *r[1];
-        return out;
+        auto r = fn(x2, variable_list{rows}, variable_list{dz.narrow(1, 0, N)}, input, std::vector<bool>{!input}).cast<std::vector<OptTensor>>();
+        const OptTensor& t = r[input ? 0 : 1];
+        return t.has_value() ? (input ? t->reshape(x.sizes()) : *t) : Tensor();
       } catch (py::error_already_set& e) {
         e.restore();
         throw python_error();
       }
-    }
+    };
     const int64_t lddz = dz.stride(0);
-    if (nx) {
+    if (nx && queue) {
+      out[0] = in_python(w2, true);
+    } else if (nx) {
       out[0] = fresh(x.sizes(), at::kBFloat16, x);
       const Tensor ws = linear_workspace(M, K, N, dz, w2, true, 0, false, false);
       check_rc(llmt_linear_dx(dz.data_ptr(), w2.data_ptr(), out[0].data_ptr(), (int)M, (int)N, (int)K, lddz, w2.stride(0), K, ws_ptr(ws), ws_size(ws),
                               status_ptr(), cur_stream()),
                "llmt_linear_dx", ws.defined() ? 2 : 1);
     }
-    if (nw) {
+    if (nw && (queue || owned)) {
+      out[1] = in_python(w, false);
+    } else if (nw) {
       out[1] = fresh(w.sizes(), at::kBFloat16, x);
       const Tensor ws = linear_workspace(N, K, M, dz, x2, true, 0, false, false);
       check_rc(llmt_linear_dw(dz.data_ptr(), x2.data_ptr(), out[1].data_ptr(), (int)M, (int)N, (int)K, lddz, x2.stride(0), K, ws_ptr(ws), ws_size(ws),
