@@ -1096,7 +1096,12 @@ int int_of(int64_t v, const char* what) {
 }
 
 // -------- LayerNorm
-int64_t layer_norm_max_width(bool f32) { return llmt_layer_norm_max_width(f32); }
+int64_t layer_norm_max_width(bool f32, bool whole) { return llmt_layer_norm_max_width(f32, whole); }
+// Weights of the widest rows lie on 16 bytes: there is no form for them that starts elsewhere.
+Tensor norm_weight(const Tensor& w, bool f32) {
+  const Tensor c = w.contiguous();
+  return w.size(0) > llmt_layer_norm_max_width(f32, false) && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
 // Rows as the kernels take them: unit inner stride, and a row stride and start whose 16-byte granules match those of a dense result.
 Tensor norm_rows(const Tensor& t) {
   const int64_t D = t.size(-1), V = 16 / t.element_size();
@@ -1113,7 +1118,7 @@ struct NativeLayerNorm : public torch::autograd::Function<NativeLayerNorm> {
                 "weight and bias must have x's type and device");
     const int64_t D = x.size(-1);
     TORCH_CHECK(D > 0 && w.dim() == 1 && b.dim() == 1 && w.size(0) == D && b.size(0) == D, "weight and bias must have x's last size");
-    Tensor xr = norm_rows(x), wc = w.contiguous(), bc = b.contiguous();
+    Tensor xr = norm_rows(x), wc = norm_weight(w, is_f32(x)), bc = norm_weight(b, is_f32(x));
     const int R = int_of(xr.size(0), "rows");
     Tensor y = fresh(x.sizes(), x.scalar_type(), x), stats = fresh({2, R}, at::kFloat, x);
     check_rc(llmt_layer_norm_fwd(xr.data_ptr(), R > 1 ? xr.stride(0) : D, wc.data_ptr(), bc.data_ptr(), y.data_ptr(), stats.data_ptr<float>(),
@@ -1134,7 +1139,7 @@ struct NativeLayerNorm : public torch::autograd::Function<NativeLayerNorm> {
     }
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t D = x.size(-1);
-    Tensor xr = norm_rows(x), wc = w.contiguous();
+    Tensor xr = norm_rows(x), wc = norm_weight(w, is_f32(x));
     Tensor dy = d[0].to(x.scalar_type());
     if (!dy.is_contiguous() || reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16) dy = dy.clone(at::MemoryFormat::Contiguous);
     const int R = (int)xr.size(0);

@@ -67,7 +67,7 @@ int llmt_qk_norm_rope_part_partials(int T, int H, int d);
 int llmt_qk_norm_rope_part_bwd(const LlmtRopeShape* s, const LlmtHeads* x, float eps, float shift, float* partial, int P, void* dw, int f32,
                                cudaStream_t stream);
 int llmt_rope_tables(const int64_t* pos, const double* inv, int P, double factor, float* cosb, float* sinb, int64_t T, cudaStream_t stream);
-int llmt_layer_norm_max_width(int f32);
+int llmt_layer_norm_max_width(int f32, int whole);
 int llmt_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean, float* rstd, int R, int D, float eps,
                         int f32, cudaStream_t stream);
 int llmt_layer_norm_bwd_partials(int R, int D, int f32);

@@ -440,7 +440,11 @@ static int ln_partials(int R, int D) {
 
 using namespace llmt;
 
-extern "C" int llmt_layer_norm_max_width(int f32) { return f32 ? kLnMaxVecs * 4 - 6 : kLnMaxVecs * 8 - 14; }
+// Widest rows: that start anywhere, or (`whole`: 16-byte granules) whose rows and weights all start on a granule.
+extern "C" int llmt_layer_norm_max_width(int f32, int whole) {
+  const int V = f32 ? Granule<float>::V : Granule<__nv_bfloat16>::V;
+  return kLnMaxVecs * V - (whole ? 0 : 2 * (V - 1));
+}
 extern "C" int llmt_layer_norm_fwd(const void* x, int64_t ldx, const void* w, const void* b, void* y, float* mean, float* rstd, int R, int D,
                                    float eps, int f32, cudaStream_t stream) {
   return f32 ? ln_fwd<float>(x, ldx, w, b, y, mean, rstd, R, D, eps, stream) : ln_fwd<__nv_bfloat16>(x, ldx, w, b, y, mean, rstd, R, D, eps, stream);

@@ -363,15 +363,22 @@ _REFUSED = (RuntimeError, AttributeError, TypeError)
 
 @functools.cache
 def _limits():
-    """Largest LayerNorm widths (bf16, fp32) and head width of the norm with rotation that the kernels have a form for."""
+    """Head width of the norm with rotation, and by type the widest LayerNorm rows, of any width and of whole 16-byte granules, that the kernels have
+    a form for."""
     ext = _node_ext()
-    return {torch.bfloat16: ext.layer_norm_max_width(False), torch.float32: ext.layer_norm_max_width(True), "head": ext.qk_norm_rope_part_max_dim()}
+    widths = {t: (ext.layer_norm_max_width(f32, False), ext.layer_norm_max_width(f32, True)) for t, f32 in ((torch.bfloat16, False), (torch.float32, True))}
+    return {**widths, "head": ext.qk_norm_rope_part_max_dim()}
+
+
+def _norm_width_fits(x) -> bool:
+    D, (any_width, whole) = x.shape[-1], _limits()[x.dtype]
+    return 0 < D <= (any_width if D * x.element_size() % 16 else whole)
 
 
 def layer_norm(x, weight, bias, eps: float):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, statistics in fp32."""
     try:
-        if (x.is_cuda and x.dtype in _ROW_TYPES and weight.dtype == bias.dtype == x.dtype and 0 < x.shape[-1] <= _limits()[x.dtype]
+        if (x.is_cuda and x.dtype in _ROW_TYPES and weight.dtype == bias.dtype == x.dtype and _norm_width_fits(x)
                 and _has_rules(x, weight, bias)):
             return _node_ext().layer_norm_node(x, weight, bias, eps)
     except (*_REFUSED, IndexError):
