@@ -1,7 +1,7 @@
 """LayerNorm at the limits of its rows and values, against the formula in 64 bits under the bounds of test_gpu_block_ops.py."""
 import pytest
 import torch
-from test_gpu_block_ops import TYPES, _norm_check, _rand
+from test_gpu_block_ops import E32, TYPES, _near, _norm_check, _rand, _u
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +23,25 @@ def test_layer_norm_widest_rows(dtype, D, start):
     grads = torch.autograd.grad(y, (x, w, b), dy)
     assert load().launch_count() == before + 3
     _norm_check(x.detach(), w.detach(), b.detach(), dy, y.detach(), *grads, 1e-6)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_layer_norm_of_tiny_values_without_eps(dtype):
+    """Values of 2e-20 and eps 0: 1 / std is 5e19, whose square is beyond fp32. The squares are subnormal (4e-40, held to 2^-18 of themselves), so the
+    reciprocal is off by less than 2^-16 of itself; 2^-12 leaves room for the sums."""
+    from torchllmtuner_b200 import ops
+    dt = TYPES[dtype]
+    for D in (64, 200, 1152, 4096):
+        x, dy = (_rand(7, D, seed=1) * 2e-20).to(dt).requires_grad_(), _rand(7, D, seed=2, dtype=dt)
+        w, b = _rand(D, seed=3, dtype=dt, mean=1, std=0.1).requires_grad_(), _rand(D, seed=4, dtype=dt).requires_grad_()
+        y = ops.layer_norm(x, w, b, 0.0)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+        X, G, W = x.detach().double(), dy.double(), w.detach().double()
+        r = (X - X.mean(1, keepdim=True)).square().mean(1, keepdim=True).rsqrt()
+        h, g = (X - X.mean(1, keepdim=True)) * r, G * W
+        assert r.max() > 2e19
+        _near(y.detach(), h * W + b.detach().double(), _u(dt) * (h * W + b.detach().double()).abs() + 2.0 ** -12 * (h * W).abs() + 1e-6, "y")
+        ref = r * (g - g.mean(1, keepdim=True) - h * (g * h).mean(1, keepdim=True))
+        _near(dx, ref, _u(dt) * ref.abs() + 2.0 ** -12 * r * (g.abs() + g.abs().mean(1, keepdim=True) + h.abs() * (g * h).abs().mean(1, keepdim=True)), "dx")
+        _near(dw, (G * h).sum(0), _u(dt) * (G * h).sum(0).abs() + 2.0 ** -12 * (G * h).abs().sum(0) + 1e-6, "dw")
+        _near(db, G.sum(0), _u(dt) * G.sum(0).abs() + 128 * E32 * G.abs().sum(0), "db")

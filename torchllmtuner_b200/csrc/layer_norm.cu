@@ -230,8 +230,9 @@ __global__ void __launch_bounds__(THREADS, NV <= 2 ? 2 : 1) layer_norm_bwd_kerne
       r = rstd[row + step];
     }
     s = group_sum2<WARP>(s, tr, red, buf);
-    // r (g w - mean - h k) with h = x r + mr, as one polynomial in x: fewer live registers than keeping h and g
-    const float k = s.y * inv_d, c0 = rr * (s.x * inv_d + mr * k), c1 = rr * rr * k;
+    // r (g w - mean - h k) with h = x r + mr, as one polynomial in x: fewer live registers than keeping h and g. Times r at the end: r^2 leaves fp32
+    // where the values are small and eps is 0 (a spread below 5e-20)
+    const float k = s.y * inv_d, c0 = s.x * inv_d + mr * k, c1 = rr * k;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float h[V], g[V], wv[V];
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, NV <= 2 ? 2 : 1) layer_norm_bwd_kerne
       if constexpr (ALIGNED) load_weights(w, p, i, wr[i]);
       wr[i].get(wv);
 #pragma unroll
-      for (int j = 0; j < V; ++j) g[j] = rr * (g[j] * wv[j]) - (c1 * h[j] + c0);
+      for (int j = 0; j < V; ++j) g[j] = rr * (g[j] * wv[j] - (c1 * h[j] + c0));
       store_cols(dx + row * (int64_t)D, p, i, g);
     }
 #pragma unroll
