@@ -1,7 +1,7 @@
 """LayerNorm at the limits of its rows and values, against the formula in 64 bits under the bounds of test_gpu_block_ops.py."""
 import pytest
 import torch
-from test_gpu_block_ops import E32, TYPES, _near, _norm_check, _rand, _u
+from test_gpu_block_ops import DEV, E32, TYPES, _near, _norm_check, _rand, _u
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,21 @@ def test_layer_norm_of_tiny_values_without_eps(dtype):
         _near(dx, ref, _u(dt) * ref.abs() + 2.0 ** -12 * r * (g.abs() + g.abs().mean(1, keepdim=True) + h.abs() * (g * h).abs().mean(1, keepdim=True)), "dx")
         _near(dw, (G * h).sum(0), _u(dt) * (G * h).sum(0).abs() + 2.0 ** -12 * (G * h).abs().sum(0) + 1e-6, "dw")
         _near(db, G.sum(0), _u(dt) * G.sum(0).abs() + 128 * E32 * G.abs().sum(0), "db")
+
+
+def test_layer_norm_of_the_most_rows():
+    """2^31 - 1 rows of one column: without a spread y is the bias; the bias's gradient counts the rows."""
+    from torchllmtuner_b200 import ops
+    R = (1 << 31) - 1
+    x = torch.zeros(R, 1, device=DEV, dtype=torch.bfloat16)
+    x[-300:] = 3.0
+    x.requires_grad_()
+    w, b = torch.ones(1, device=DEV, dtype=torch.bfloat16).requires_grad_(), torch.full((1,), 0.75, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    y = ops.layer_norm(x, w, b, 1e-6)
+    assert (y == 0.75).all()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    del y
+    assert (dx[-1000:].abs() <= 1e-2).all() and dw.abs() <= 3 * 300 * 1000 * 2.0 ** -22      # h is off by a few steps of fp32 of 3 / sqrt(eps)
+    assert abs(db.double().item() - R) <= R * 2.0 ** -8
+    del x, dx
+    torch.cuda.empty_cache()

@@ -362,9 +362,9 @@ template <typename T>
 static int ln_bwd_grid(int R, const LnShape& s) {
   const int V = Granule<T>::V;
   const int most = sm_count() * (s.tr == 32 ? (s.nv <= 2 ? 2 : 1) : s.tr >= 256 ? 1 : 256 / s.tr);
-  const int need = (R + s.groups - 1) / s.groups;
+  const int64_t need = ((int64_t)R + s.groups - 1) / s.groups;
   if (need >= most) return most / V * V;                 // not beyond what the machine holds at once
-  return (need + V - 1) / V * V;
+  return ((int)need + V - 1) / V * V;
 }
 
 // All rows of an operand lie at row * ld; every operand has the same granule shift in the same row.
@@ -388,8 +388,8 @@ static int ln_fwd(const void* x, int64_t ldx, const void* w, const void* b, void
   const LnShape s = ln_fwd_shape(vecs);
   const int V = Granule<T>::V, threads = s.tr * s.groups;
   const int most = sm_count() * (s.tr == 32 ? (s.nv <= 2 ? 4 : s.nv <= 5 ? 2 : 1) : 1024 / threads);
-  const int need = (R + s.groups - 1) / s.groups;
-  const int grid = ((need < most ? need : most) + V - 1) / V * V;
+  const int64_t need = ((int64_t)R + s.groups - 1) / s.groups;
+  const int grid = ((int)(need < most ? need : most) + V - 1) / V * V;
   const T *xp = reinterpret_cast<const T*>(x), *wp = reinterpret_cast<const T*>(w), *bp = reinterpret_cast<const T*>(b);
 #define LLMT_LN(N, W)                                                                                                                          \
   if (s.nv == N && (s.tr == 32) == W) {                                                                                                        \
