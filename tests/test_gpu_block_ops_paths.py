@@ -157,3 +157,35 @@ def test_special_values_in_rows_of_their_own():
         want = (9 * slope)[rows]
         # dz is rounded to bf16, and so is the sum of nine
         assert ((dx.detach()[rows].double() - want).abs() <= 2.02 * _u(torch.bfloat16) * want.abs() + 9 * 16 * E32 * (1 + x.detach()[rows].double().abs().clamp(max=100))).all(), (act, dx, slope)
+
+
+# ------------------------------------------------------------------------------------------------ sizes at the limits
+def test_linear_act_refuses_sizes_past_its_range():
+    """Rows and features count up to 2^31 - 512 (a tile's end is still a 32-bit number): more is refused before anything is allocated or launched."""
+    from torchllmtuner_b200 import ops
+    most = (1 << 31) - 512
+    row, w = torch.zeros(1, 8, device=DEV, dtype=torch.bfloat16), torch.zeros(8, 8, device=DEV, dtype=torch.bfloat16)
+    before = torch.cuda.memory_allocated()
+    for rows in (most + 1, (1 << 31) - 1, 1 << 31, (1 << 32) + 5):
+        with pytest.raises(RuntimeError, match="rows"):
+            ops.linear_act(row.expand(rows, 8), w)
+        with pytest.raises(RuntimeError, match="features"):
+            ops.linear_act(row, row.expand(rows, 8))
+        with pytest.raises(RuntimeError, match="features"):
+            ops.linear_act(row[:, :1].expand(1, rows), row[:, :1].expand(8, rows))
+    assert torch.cuda.memory_allocated() == before
+
+
+def test_linear_act_of_the_most_rows():
+    """2^31 - 512 rows of one feature: every value of y and dx is a product by two, exact."""
+    from torchllmtuner_b200 import ops
+    x = torch.empty((1 << 31) - 512, 1, device=DEV, dtype=torch.bfloat16).normal_().requires_grad_()
+    w = torch.full((1, 1), 2.0, device=DEV, dtype=torch.bfloat16)
+    y = ops.linear_act(x, w)
+    with torch.no_grad():
+        assert torch.equal(y, x * 2)
+        dy = torch.empty_like(y).normal_()
+    dx, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(dx, dy * 2)
+    del x, y, dx, dy
+    torch.cuda.empty_cache()

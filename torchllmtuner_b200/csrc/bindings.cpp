@@ -1350,6 +1350,10 @@ std::vector<Tensor> rope_tables(const Tensor& positions, const Tensor& inv, doub
 }
 
 // -------- linear layers with an epilogue
+int linear_size(int64_t v, const char* what) {
+  TORCH_CHECK(v > 0 && v <= llmt_linear_max_size(), what, " is out of the kernels' range: ", v);
+  return (int)v;
+}
 // Rows as TMA reads them: unit inner stride, row stride a multiple of 8, 16-byte start; otherwise a copy with padded rows (the padding is never
 // read: the tensor map ends at the last column).
 // Rows of a buffer that TMA reads: on 128 bytes where that adds at most an eighth (a row of a box then lies in one line), else on 16.
@@ -1376,7 +1380,7 @@ inline int64_t ws_size(const Tensor& t) { return t.defined() ? t.numel() : 0; }
 // (CTAs of a tile, its columns, parts along the depth) of a product: which of the kernels' paths a size takes.
 std::tuple<int, int, int> linear_cut(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, bool gradient, int64_t act, bool res, bool pre) {
   int c[3];
-  llmt_linear_cut(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), lda, ldb, gradient, (int)act, res, pre, c);
+  llmt_linear_cut(linear_size(M, "rows"), linear_size(N, "features"), linear_size(K, "features"), lda, ldb, gradient, (int)act, res, pre, c);
   return {c[0], c[1], c[2]};
 }
 struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
@@ -1385,7 +1389,8 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
     check_bf16(x, "x");
     check_bf16(w, "w");
     TORCH_CHECK(w.dim() == 2 && x.size(-1) == w.size(1) && w.device() == x.device(), "x [..., K] and w [N, K] must agree");
-    const int64_t N = w.size(0), K = w.size(1);
+    const int64_t N = linear_size(w.size(0), "features"), K = linear_size(w.size(1), "features");
+    linear_size(x.numel() / K, "rows");                  // before anything is copied
     Tensor x2 = tma_rows(rows_2d(x)), w2 = tma_rows(w.stride(1) == 1 ? w : w.contiguous());
     const int64_t M = x2.size(0);
     auto ysizes = x.sizes().vec();
@@ -1403,7 +1408,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
       if (M > 1 && r2.stride(0) < N && r2.stride(0) != 0) r2 = r2.contiguous();
     }
     if (act != 0 && keep) pre = fresh({M, row_pitch(N)}, at::kBFloat16, x);
-    const Tensor ws = linear_workspace(int_of(M, "rows"), int_of(N, "features"), int_of(K, "features"), x2, w2, false, act, r2.defined(),
+    const Tensor ws = linear_workspace(M, N, K, x2, w2, false, act, r2.defined(),
                                        pre.defined());
     check_rc(llmt_linear_act(x2.data_ptr(), w2.data_ptr(), y.data_ptr(), bc.defined() ? bc.data_ptr() : nullptr, bc.defined() && is_f32(bc),
                              r2.defined() ? r2.data_ptr() : nullptr, pre.defined() ? pre.data_ptr() : nullptr, (int)act, (int)M,

@@ -31,6 +31,7 @@ int llmt_grouped_wgrad_bf16(const void* A, const void* B, void* C, const int* se
 int llmt_rmsnorm_fwd(const void* x, const void* res, const void* w, void* y, void* sum_out, float* rstd, int T, int D,
                      float eps, cudaStream_t st);
 // ---- linear layers with bias, activation (activations.cuh) and residual (linear_act.cu) ----
+int llmt_linear_max_size();
 int llmt_linear_pad(const void* x, int64_t ldx, void* y, int64_t ldy, int M, int N, cudaStream_t stream);
 int64_t llmt_linear_ws_floats(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre);
 void llmt_linear_cut(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre, int* out);

@@ -31,6 +31,7 @@ constexpr int kLStage = kLPatch + 128;     // and 32 bias values
 constexpr int kLSlack = 512;              // for the 1024-byte alignment of the stages; dynamic shared memory starts on 1024 bytes (checked)
 constexpr int kLSmemFixed = kLEpiWarps * kLStage + kLSlack + 512 /*barriers*/;      // leaves four stages of 128 x 256 tiles to the byte
 constexpr int kMaxWorkers = 160;
+constexpr int kLMostSize = 0x7fffffff - 511;             // rows and features: the end of the last tile is still a 32-bit number
 
 // What becomes of a product: stored as it is, or (`fwd`) with bias, activation and residual.
 struct LinOut {
@@ -799,7 +800,7 @@ static int lin_gemm(const void* A, const void* B, LinArgs a, int K, int64_t lda,
                     int64_t ws_floats, cudaStream_t stream) {
   LinOut& o = a.out;
   if (o.M <= 0 || o.N <= 0) return 0;
-  if (K <= 0 || (lda & 7) || (ldb & 7) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return -10;
+  if (K <= 0 || o.M > kLMostSize || o.N > kLMostSize || K > kLMostSize || (lda & 7) || (ldb & 7) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return -10;
   const LinCut cut = lin_cut(o.M, o.N, K, lin_kind(b_mn, lda, ldb, fwd ? act : 0, o.res != nullptr, o.pre != nullptr));
   if (lin_ws_floats(o.M, o.N, cut) > (ws == nullptr ? 0 : ws_floats) || sm_count() / cut.cg > kMaxWorkers) return -10;
   LinPlan& p = a.plan;
@@ -892,12 +893,13 @@ using namespace llmt;
 // Workspace of a product out [M, N] of depth K whose operands' rows lie lda and ldb elements apart, in floats (0: none is needed): of llmt_linear_dx
 // (dz, W) or llmt_linear_dw (dz, x) (`gradient`; act, res and pre 0), or of llmt_linear_act (x, W) with that activation, with a residual (`res`) and
 // with z (`pre`).
+extern "C" int llmt_linear_max_size() { return kLMostSize; }
 extern "C" int64_t llmt_linear_ws_floats(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre) {
-  if (act < 0 || act >= kActKinds) return 0;             // refused by the launch
+  if (act < 0 || act >= kActKinds || M <= 0 || N <= 0 || K <= 0 || M > kLMostSize || N > kLMostSize || K > kLMostSize) return 0;   // refused by the launch
   return lin_ws_floats(M, N, lin_cut(M, N, K, lin_kind(gradient != 0, lda, ldb, act, res != 0, pre != 0)));
 }
 
-// How a product with the same arguments is cut: out receives the CTAs of a tile, its columns and the parts along K.
+// How a product with the same arguments is cut: out receives the CTAs of a tile, its columns and the parts along K. Sizes as llmt_linear_act takes them.
 extern "C" void llmt_linear_cut(int M, int N, int K, int64_t lda, int64_t ldb, int gradient, int act, int res, int pre, int* out) {
   const LinCut c = lin_cut(M, N, K, lin_kind(gradient != 0, lda, ldb, act < 0 || act >= kActKinds ? 0 : act, res != 0, pre != 0));
   out[0] = c.cg;
@@ -907,7 +909,7 @@ extern "C" void llmt_linear_cut(int M, int N, int K, int64_t lda, int64_t ldb, i
 
 // y [M][ldy] = x [M][ldx] (rows of N elements, any pitch and start) for TMA: y and its pitch on 16 bytes, at least N rounded up to a multiple of 8.
 extern "C" int llmt_linear_pad(const void* x, int64_t ldx, void* y, int64_t ldy, int M, int N, cudaStream_t stream) {
-  if (M < 0 || N < 0 || (ldy & 7) || ldy < (int64_t)(N + 7) / 8 * 8 || (reinterpret_cast<uintptr_t>(y) & 15) || (reinterpret_cast<uintptr_t>(x) & 1)) return -10;
+  if (M < 0 || N < 0 || M > kLMostSize || N > kLMostSize || (ldy & 7) || ldy < (int64_t)(N + 7) / 8 * 8 || (reinterpret_cast<uintptr_t>(y) & 15) || (reinterpret_cast<uintptr_t>(x) & 1)) return -10;
   if (M == 0 || N == 0) return 0;
   const int strips = (N + 255) / 256, need = (M + 8 * kPadRows - 1) / (8 * kPadRows), fill = sm_count() * 16 / strips + 1;
   linear_pad_kernel<<<dim3(strips, need < fill ? need : fill), 256, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(x), ldx, reinterpret_cast<__nv_bfloat16*>(y), ldy, M, N);
@@ -949,12 +951,12 @@ extern "C" int llmt_linear_dw(const void* dz, const void* x, void* dw, int M, in
   return lin_gemm(dz, x, a, M, lddz, ldx, true, true, false, 0, ws, ws_floats, stream);
 }
 // Rows of `partial` ([rows][N] floats) that llmt_linear_dz needs for db; 0: none.
-extern "C" int llmt_linear_db_partials(int M, int N) { return dz_blocks(M, N); }
+extern "C" int llmt_linear_db_partials(int M, int N) { return M > kLMostSize || N <= 0 || N > kLMostSize ? 0 : dz_blocks(M, N); }
 // dz = dy act'(z) (act 0: dz = dy; dz nullptr: not written), db = column sums of dz in fp32 before rounding (nullptr: not computed). z and dz have
 // rows on 16 bytes of at least N values rounded up to a multiple of 8.
 extern "C" int llmt_linear_dz(const void* dy, int64_t ldy, const void* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db, int db_f32,
                               float* partial, int P, int M, int N, cudaStream_t stream) {
-  if (M < 0 || N <= 0 || act < 0 || act >= kActKinds || (act != 0 && z == nullptr)) return -10;
+  if (M < 0 || N <= 0 || M > kLMostSize || N > kLMostSize || act < 0 || act >= kActKinds || (act != 0 && z == nullptr)) return -10;
   const int blocks = dz_blocks(M, N);
   if (db != nullptr && blocks > 0 && (partial == nullptr || P < blocks)) return -10;
   auto at16 = [](const void* p, int64_t ld) { return p == nullptr || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % 8 == 0); };
