@@ -189,3 +189,14 @@ def test_linear_act_of_the_most_rows():
     assert torch.equal(dx, dy * 2)
     del x, y, dx, dy
     torch.cuda.empty_cache()
+
+
+def test_linear_act_one_row_whose_gradient_has_no_row_stride():
+    """A single row of the upstream gradient may carry any stride between rows, zero among them."""
+    from torchllmtuner_b200 import ops
+    x, w, b = _rand(1, 200, seed=1).requires_grad_(), _rand(136, 200, seed=2, std=0.07).requires_grad_(), _rand(136, seed=3).requires_grad_()
+    dy = _rand(136, seed=4)
+    want = torch.autograd.grad(ops.linear_act(x, w, b), (x, w, b), dy[None])
+    for stride in (0, 1, 8, 72):
+        got = torch.autograd.grad(ops.linear_act(x, w, b), (x, w, b), dy.as_strided((1, 136), (stride, 1)))
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), stride

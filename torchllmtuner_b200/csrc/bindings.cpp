@@ -1456,7 +1456,7 @@ struct NativeLinearAct : public torch::autograd::Function<NativeLinearAct> {
            dy = rows_2d(d[0]);
     const int64_t M = x2.size(0);
     if (M > 1 && dy.stride(0) < N) dy = dy.contiguous();
-    const bool tma_ok = dy.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
+    const bool tma_ok = dy.stride(0) >= N && dy.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0;
     const bool write = (nx || nw) && (act != 0 || !tma_ok);
     Tensor dz = write ? fresh({M, row_pitch(N)}, at::kBFloat16, x) : dy;
     if (write || nb) {
