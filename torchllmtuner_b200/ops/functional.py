@@ -451,7 +451,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float, *, layout: str 
     if plain and _use_cuda(q) and q.dtype == torch.bfloat16 and q.dim() == 3 and 2 * cos.shape[-1] == q.shape[-1] and q.shape[-1] in (64, 128, 256):
         return tuple(_run_node(_ext().qk_norm_rope_node, q, k, q_weight, k_weight, cos, sin, eps))
     try:
-        if _rotary_kernel(cos, sin, q, k) and not (plain and q.dtype == torch.float32):
+        if _rotary_kernel(cos, sin, q, k):
             nq, nk = norm is not False and (norm or q_weight is not None), norm is not False and (norm or k_weight is not None)
             ext, inter = _node_ext(), _INTERLEAVED[layout]
             if not nq and not nk:
