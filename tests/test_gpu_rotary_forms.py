@@ -1,4 +1,6 @@
 """Rotary positions and per-head norms in forms that test_gpu_block_ops.py does not reach, against the formulas in 64 bits under its bounds."""
+import math
+
 import pytest
 import torch
 from test_gpu_block_ops import DEV, E32, _near, _rand, _tables, _turn64
@@ -36,3 +38,14 @@ def test_default_norm_and_rotation_in_fp32_is_the_kernel(T, H, K, d, P, weights)
         _near(dx, ref, E32 * ref.abs() + 64 * E32 * r * (gs + X.abs() * r * r * (gs * X.abs()).mean(-1, keepdim=True)), "dx")
         ref = (back * X * r).sum((0, 1))
         _near(dw[0], ref, E32 * ref.abs() + (64 + T * x.shape[1] / 8) * E32 * (bsize * X.abs() * r).sum((0, 1)), "dw")
+
+
+def test_scaling_with_entries_of_other_uses():
+    """A configuration's dict may hold entries that the frequencies do not depend on, lists among them."""
+    from torchllmtuner_b200 import ops
+    scaling = {"rope_type": "linear", "factor": 3.0, "mrope_section": [8, 12, 12], "type": "linear"}
+    pos = torch.arange(70, device=DEV)
+    cos, sin = ops.rope_tables(pos, 64, 1e4, scaling=scaling)
+    ang = torch.arange(70, dtype=torch.float64)[:, None] * torch.tensor([1e4 ** (-2 * j / 64) / 3.0 for j in range(32)], dtype=torch.float64)
+    bound = (math.pi + 4) * E32 + 2.0 ** -50 * ang
+    assert ((cos.cpu().double() - ang.cos()).abs() <= bound).all() and ((sin.cpu().double() - ang.sin()).abs() <= bound).all()

@@ -389,6 +389,11 @@ def layer_norm(x, weight, bias, eps: float):
 
 
 # ----------------------------------------------------------------------------------------------- rotary positions, QK-norm + RoPE
+# What the frequencies depend on; a configuration's dict may hold more, lists among it.
+_SCALING_ENTRIES = ("rope_type", "factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor", "beta_fast", "beta_slow", "truncate",
+                    "attention_factor", "mscale", "mscale_all_dim")
+
+
 @functools.lru_cache(maxsize=64)
 def _frequencies(head_dim: int, theta: float, items: tuple):
     """Scaled inverse frequencies (64-bit tensor on the host) and the factor on both tables."""
@@ -412,7 +417,7 @@ def rope_tables(positions, head_dim: int, theta: float, dtype=torch.float32, sca
         inv, factor = _frequencies(head_dim, theta, tuple(scaling.items()))
     except _REFUSED:
         validate_rope_scaling(scaling)
-        raise
+        inv, factor = _frequencies(head_dim, theta, tuple((k, scaling[k]) for k in _SCALING_ENTRIES if k in scaling))
     cos, sin = _ext().rope_tables(positions if positions.dtype == torch.int64 else positions.long(), inv, factor)
     return (cos, sin) if dtype == torch.float32 else (cos.to(dtype), sin.to(dtype))
 
