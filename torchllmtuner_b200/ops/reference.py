@@ -85,14 +85,15 @@ def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor
 
 
 def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, layout: str = "half", offset: int = 0, inverse: bool = False) -> torch.Tensor:
-    """x [T, ..., d]: the channels [offset, offset + 2 P) rotate by cos/sin [T, P], the rest pass; arithmetic in fp32. `layout` "half" pairs
-    channel j with channel j + P of that range, "interleaved" the channels 2j and 2j + 1. `inverse` rotates back."""
+    """x [T, ..., d]: the channels [offset, offset + 2 P) rotate by cos/sin [T, P], the rest pass; arithmetic in fp32, in fp64 for operands of that
+    type. `layout` "half" pairs channel j with channel j + P of that range, "interleaved" the channels 2j and 2j + 1. `inverse` rotates back."""
     r = 2 * cos.shape[-1]
     shape = [cos.shape[0]] + [1] * (x.dim() - 2) + [cos.shape[-1]]
-    c, s = cos.float().reshape(shape), sin.float().reshape(shape)
+    wide = torch.promote_types(x.dtype, torch.float32)
+    c, s = cos.to(wide).reshape(shape), sin.to(wide).reshape(shape)
     if inverse:
         s = -s
-    t = x[..., offset:offset + r].float()
+    t = x[..., offset:offset + r].to(wide)
     if layout == "half":
         x1, x2 = t[..., :r // 2], t[..., r // 2:]
         t = torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
@@ -104,12 +105,12 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, layout: str =
 
 
 def head_norm_rope(x, weight, cos, sin, offset: int, interleaved: bool, eps: float, shift: float):
-    """x [T, H, d]: RMSNorm of every head (times weight + shift where there is a weight), then the rotation of `rope`; one rounding."""
+    """x [T, H, d]: RMSNorm of every head in fp32 (times weight + shift where there is a weight), then the rotation of `rope`; one rounding."""
     xf = x.float()
     xf = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     if weight is not None:
         xf = xf * (shift + weight.float() if shift else weight.float())
-    return rope(xf, cos, sin, layout="interleaved" if interleaved else "half", offset=offset).to(x.dtype)
+    return rope(xf.to(torch.promote_types(x.dtype, torch.float32)), cos, sin, layout="interleaved" if interleaved else "half", offset=offset).to(x.dtype)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps: float, *, layout: str = "half", offset: int = 0, norm: bool | None = None,
