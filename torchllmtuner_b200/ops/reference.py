@@ -76,14 +76,6 @@ def scaled_frequencies(head_dim: int, theta: float, scaling: dict):
     return tuple(v * (1.0 - r) + v / s * r for v, r in zip(inv, ramp)), float(factor)
 
 
-def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-    # x [T, H, d] fp32; cos/sin [T, d/2]; half rotation: (x1, x2) -> (x1 c - x2 s, x2 c + x1 s)
-    d2 = x.shape[-1] // 2
-    x1, x2 = x[..., :d2], x[..., d2:]
-    c, s = cos.float()[:, None, :], sin.float()[:, None, :]
-    return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), dim=-1)
-
-
 def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, *, layout: str = "half", offset: int = 0, inverse: bool = False) -> torch.Tensor:
     """x [T, ..., d]: the channels [offset, offset + 2 P) rotate by cos/sin [T, P], the rest pass; arithmetic in fp32, in fp64 for operands of that
     type. `layout` "half" pairs channel j with channel j + P of that range, "interleaved" the channels 2j and 2j + 1. `inverse` rotates back."""
