@@ -9,6 +9,7 @@
 //
 // Bound by the tensor pipe and by the operands' way from L2. 16384 x 1152 -> 4608 with gelu_tanh: forward 119 us (1.46 PFLOP/s; 107 plain), dx 115,
 // dW 114, dz 80 (453 MB at 5.7 TB/s).
+#include <atomic>
 #include "activations.cuh"
 #include "common.cuh"
 #include "kernels.h"
@@ -647,19 +648,20 @@ __global__ void __launch_bounds__(1024) linear_db_kernel(const float* __restrict
 }
 
 // ------------------------------------------------------------------------------------------ host
-// Function attributes belong to a device: remembered per device.
+// Function attributes belong to a device: remembered per device. Threads may launch at once (a backward runs beside a forward).
+using DeviceSet = std::atomic<uint64_t>;
 template <typename F>
-static bool allow_smem(F kern, int bytes, uint64_t& done) {
+static bool allow_smem(F kern, int bytes, DeviceSet& done) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  if (dev < 64 && (done >> dev & 1)) return true;
+  if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return true;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-  if (dev < 64) done |= 1ull << dev;
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   return true;
 }
 
 template <typename K>
-static int lin_run(K kern, uint64_t& done, int cg, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LinArgs& a, cudaStream_t stream) {
+static int lin_run(K kern, DeviceSet& done, int cg, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LinArgs& a, cudaStream_t stream) {
   if (!allow_smem(kern, kLSmem, done)) return -2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.plan.workers * cg);
@@ -675,7 +677,7 @@ static int lin_run(K kern, uint64_t& done, int cg, const CUtensorMap& ta, const 
 }
 template <bool A_MN, bool B_MN, bool SPLIT, bool FWD, int ACT, bool RES>
 static int lin_launch(int cg, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LinArgs& a, cudaStream_t stream) {
-  static uint64_t single = 0, pair = 0, wide = 0;
+  static DeviceSet single{0}, pair{0}, wide{0};
   if (cg == 1) return lin_run(linear_kernel<1, false, A_MN, B_MN, SPLIT, FWD, ACT, RES>, single, 1, ta, tb, tb2, a, stream);
   if (a.plan.bn <= 256) return lin_run(linear_kernel<2, false, A_MN, B_MN, SPLIT, FWD, ACT, RES>, pair, 2, ta, tb, tb2, a, stream);
   return lin_run(linear_kernel<2, true, A_MN, B_MN, SPLIT, FWD, ACT, RES>, wide, 2, ta, tb, tb2, a, stream);
